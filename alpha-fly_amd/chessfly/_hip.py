@@ -99,6 +99,13 @@ SIGNATURES = {
     "fly_rest_backward": (_i32, [_p, _p, _p, _p, _p, _p, _p, _f32, _i64, _p, _p, _p, _p, _p]),
     "fly_rest_products_backward": (_i32, [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64,
                                           _p, _p]),
+    "fly_quantize_rows": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p]),
+    "fly_int8_create": (_i32, [_p, _i64, _p, _p, _i64, _i64, _p, _pp]),
+    "fly_int8_destroy": (_i32, [_p]),
+    "fly_int8_workspace": (_sz, [_p, _i64]),
+    "fly_int8_linear": (_i32, [_p, _p, _i32, _i64, _p, _i64, _p, _i32, _i64, _p, _sz, _p]),
+    "fly_top_logits": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _f32, _p, _p, _p, _p]),
+    "fly_distill": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i32, _f32, _p, _p, _i64, _p, _f32, _p]),
     "fly_profile_enable": (_i32, [_i32]),
     "fly_profile_read": (_i32, [_p, _p]),
     "fly_profile_launches": (_i64, [_p, _p, _i64]),
@@ -142,6 +149,27 @@ def stream(device: torch.device) -> int:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+# torch types by their fly_type
+FLOAT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+TYPES = {**FLOAT_TYPES, torch.int8: 3}
+
+
+def device_of(t: torch.Tensor):
+    """The tensor's device as the current one, for calls whose kernels run on it."""
+    return torch.cuda.device(t.device)
+
+
+def row_major(t: torch.Tensor) -> torch.Tensor:
+    """A matrix whose rows lie apart, each contiguous: t itself where its strides allow (rows of any length apart)."""
+    rows, cols = t.shape
+    ok = (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols)
+    return t if ok else t.contiguous()
+
+
+def row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

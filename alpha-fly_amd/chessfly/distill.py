@@ -1,0 +1,158 @@
+"""Distillation from a teacher's top logits: `top_logits`, `distill_loss`, `distill_loss_and_grad`, over fly_top_logits
+and fly_distill.
+
+A teacher labels positions once: of each row of its logits the k largest are kept, and the log-sum-exp of the rest, which
+is what a replay buffer has to hold.  A student then learns from that list:
+
+    p, p_t = softmax of (values / T, tail)                     the listed moves, and one class for all others
+    q      = softmax of (logits / T) over the visible moves,   q_t = its sum over the moves not listed
+    loss   = T^2 (sum_S p log(p / q) + p_t log(p_t / q_t))
+
+Rows are independent, sums are float32 whatever the logits' type, and results do not depend on scheduling.
+No counterpart in the reference, whose training takes visit counts over all moves.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _hip
+
+FLOATS = _hip.FLOAT_TYPES
+MOST_LISTED = 256      # no chess position has over 218 legal moves
+
+
+class TopLogits(NamedTuple):
+    """A teacher's list: values (rows, k) float32 in falling order, index (rows, k) int32 (-1: no such move), and tail
+    (rows) float32, the log-sum-exp at the temperature of what is not listed (None: the list is all there is)."""
+    values: torch.Tensor
+    index: torch.Tensor
+    tail: torch.Tensor | None = None
+
+
+def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
+    _hip.require_device(logits, what)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise RuntimeError(f"{what}: logits must be (rows, columns), got {tuple(logits.shape)}")
+    if logits.dtype not in FLOATS:
+        raise RuntimeError(f"{what}: logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    return _hip.row_major(logits)
+
+
+def _legal(legal: torch.Tensor | None, logits: torch.Tensor, what: str) -> torch.Tensor | None:
+    if legal is None:
+        return None
+    if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or legal.device != logits.device:
+        raise RuntimeError(f"{what}: legal must be bool of shape {tuple(logits.shape)} on {logits.device}, "
+                           f"got {legal.dtype} {tuple(legal.shape)} on {legal.device}")
+    return _hip.row_major(legal)
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal: torch.Tensor | None = None,
+               tail: bool = True) -> TopLogits:
+    """The k (1 to 256) largest logits of each row over the legal columns, the lower column first among equals, and the
+    log-sum-exp of the others.  Rows with fewer legal columns (a column at -inf is none) end in values -inf and index -1;
+    a tail of nothing is -inf."""
+    logits = _logits(logits, "top_logits")
+    legal = _legal(legal, logits, "top_logits")
+    rows, cols = logits.shape
+    dev = logits.device
+    k = int(k)
+    if not 1 <= k <= MOST_LISTED:
+        raise RuntimeError(f"top_logits: k must lie in 1..{MOST_LISTED}, got {k}")
+    values = torch.empty(rows, k, dtype=torch.float32, device=dev)
+    index = torch.empty(rows, k, dtype=torch.int32, device=dev)
+    rest = torch.empty(rows, dtype=torch.float32, device=dev) if tail else None
+    with _hip.device_of(logits):
+        _hip.check(_hip.load().fly_top_logits(logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
+                                              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, k,
+                                              temperature, values.data_ptr(), index.data_ptr(), _hip.ptr(rest),
+                                              _hip.stream(dev)), "fly_top_logits")
+    return TopLogits(values, index, rest)
+
+
+def _teacher(teacher, logits: torch.Tensor, what: str) -> TopLogits:
+    teacher = TopLogits(*teacher)
+    rows = logits.shape[0]
+    for name, t, dtype, dims in (("values", teacher.values, torch.float32, 2), ("index", teacher.index, torch.int32, 2),
+                                 ("tail", teacher.tail, torch.float32, 1)):
+        if t is None and name == "tail":
+            continue
+        if t.dtype != dtype or t.dim() != dims or t.shape[0] != rows or t.device != logits.device:
+            raise RuntimeError(f"{what}: the teacher's {name} must be {dtype} with {rows} rows on {logits.device}, "
+                               f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if teacher.values.shape != teacher.index.shape or not 1 <= teacher.values.shape[1] <= MOST_LISTED:
+        raise RuntimeError(f"{what}: the teacher's values and index must be alike, (rows, 1..{MOST_LISTED}), got "
+                           f"{tuple(teacher.values.shape)} and {tuple(teacher.index.shape)}")
+    return TopLogits(*(t.contiguous() if t is not None else None for t in teacher))
+
+
+def _run(logits, teacher: TopLogits, temperature, legal, loss, grad, row_scale, grad_scale) -> None:
+    rows, cols = logits.shape
+    with _hip.device_of(logits):
+        _hip.check(_hip.load().fly_distill(
+            logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols, _hip.ptr(legal),
+            _hip.row_stride(legal) if legal is not None else 0, teacher.values.data_ptr(), teacher.index.data_ptr(),
+            _hip.ptr(teacher.tail), teacher.values.shape[1], temperature, _hip.ptr(loss), _hip.ptr(grad), cols,
+            _hip.ptr(row_scale), grad_scale, _hip.stream(logits.device)), "fly_distill")
+
+
+def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
+                          legal: torch.Tensor | None = None, grad_scale: float = 1.0,
+                          row_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The loss of each row (float32) and, in the same pass, grad_scale * row_scale * dloss/dlogits in the logits' type
+    (grad_scale = 1 / rows: the gradient of the mean).  For training loops: `logits.backward(grad)`."""
+    what = "distill_loss_and_grad"
+    logits = _logits(logits.detach(), what)
+    legal = _legal(legal, logits, what)
+    teacher = _teacher(teacher, logits, what)
+    rows, cols = logits.shape
+    if row_scale is not None:
+        if row_scale.dtype != torch.float32 or row_scale.shape != (rows,) or row_scale.device != logits.device:
+            raise RuntimeError(f"{what}: row_scale must be float32 of shape ({rows},) on {logits.device}, "
+                               f"got {row_scale.dtype} {tuple(row_scale.shape)} on {row_scale.device}")
+        row_scale = row_scale.contiguous()
+    loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    grad = torch.empty(rows, cols, dtype=logits.dtype, device=logits.device)
+    _run(logits, teacher, temperature, legal, loss, grad, row_scale, grad_scale)
+    return loss, grad
+
+
+class _DistillLoss(torch.autograd.Function):
+    """Rows' losses; the backward is the kernel's gradient pass over the saved logits, scaled by the rows' upstream
+    gradients."""
+
+    @staticmethod
+    def forward(ctx, logits, values, index, tail, temperature, legal):
+        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        _run(logits, TopLogits(values, index, tail), temperature, legal, loss, None, None, 1.0)
+        ctx.save_for_backward(logits, values, index, tail, legal)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        logits, values, index, tail, legal = ctx.saved_tensors
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _run(logits, TopLogits(values, index, tail), ctx.temperature, legal, None, grad, up.float().contiguous(), 1.0)
+        return grad, None, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
+                 legal: torch.Tensor | None = None, reduction: str = "mean") -> torch.Tensor:
+    """The student's loss against a teacher's list, differentiable by `logits` (the teacher's tensors get no gradient).
+    reduction: "mean" or "sum" over rows, or "none" (rows) float32.
+
+    A row without a listed legal move (index -1, or a move that `legal` hides), or whose student sees no move, has loss
+    and gradient 0.  The tail is left out where the student has no move outside the list.  A repeated index, or one past
+    the columns, makes its row NaN."""
+    if reduction not in ("mean", "sum", "none"):
+        raise RuntimeError(f"distill_loss: reduction must be mean, sum or none, got {reduction!r}")
+    logits = _logits(logits, "distill_loss")
+    legal = _legal(legal, logits, "distill_loss")
+    teacher = _teacher(teacher, logits, "distill_loss")
+    loss = _DistillLoss.apply(logits, *(t.detach() if t is not None else None for t in teacher), temperature, legal)
+    return loss if reduction == "none" else loss.mean() if reduction == "mean" else loss.sum()

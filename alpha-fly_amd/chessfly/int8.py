@@ -1,0 +1,98 @@
+"""Dense maps held in 8 bits: `quantize_rows` and `Int8Linear`, over fly_quantize_rows and fly_int8_*.
+
+    s_m = max_k |x_mk| / 127,   q_mk = rint(x_mk * (127 / max_k |x_mk|))          a scale for each token
+    y_mn = (sum_k q_mk w_nk) (s_m t_n) + b_n                                      and for each channel
+
+The sums are exact in int32; the scales and the bias are applied in float32 and the result rounds once to `out_dtype`.
+A token that holds an infinity or NaN has NaN outputs; one of zeros gives the bias.  No counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _hip
+
+FLOATS = _hip.FLOAT_TYPES
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    _hip.require_device(x, what)
+    if x.dim() != 2:
+        raise RuntimeError(f"{what}: x must have two dimensions, got {tuple(x.shape)}")
+    return _hip.row_major(x)
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """x (rows, columns) float32, float16 or bfloat16 -> int8 values (rows, columns) and float32 scales (rows)."""
+    x = _rows(x, "quantize_rows")
+    if x.dtype not in FLOATS:
+        raise RuntimeError(f"quantize_rows: x must be float32, float16 or bfloat16, got {x.dtype}")
+    rows, cols = x.shape
+    q = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with _hip.device_of(x):
+        _hip.check(_hip.load().fly_quantize_rows(x.data_ptr(), FLOATS[x.dtype], _hip.row_stride(x), rows, cols,
+                                                 q.data_ptr(), max(cols, 1), scale.data_ptr(), _hip.stream(x.device)),
+                   "fly_quantize_rows")
+    return q, scale
+
+
+class Int8Linear:
+    """y = x W^T + b with W (channels, k) in 8 bits.  The weight is laid out for the matrix cores once, here; the object
+    keeps no reference to the tensors.  Calls run on the current stream with scratch from torch's allocator."""
+
+    def __init__(self, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None):
+        weight = _rows(weight, "Int8Linear")
+        self.n, self.k = weight.shape
+        self.device = weight.device
+        if weight.dtype != torch.int8:
+            raise RuntimeError(f"Int8Linear: the weight must be int8, got {weight.dtype}")
+        for name, t in (("scale", scale), ("bias", bias)):
+            if t is not None and (t.dtype != torch.float32 or t.shape != (self.n,) or t.device != weight.device):
+                raise RuntimeError(f"Int8Linear: {name} must be float32 of shape ({self.n},) on {weight.device}, "
+                                   f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+        scale = scale.contiguous()
+        bias = bias.contiguous() if bias is not None else None
+        handle = ctypes.c_void_p()
+        with _hip.device_of(weight):
+            _hip.check(_hip.load().fly_int8_create(weight.data_ptr(), _hip.row_stride(weight), scale.data_ptr(),
+                                                   _hip.ptr(bias), self.n, self.k, _hip.stream(weight.device),
+                                                   ctypes.byref(handle)), "fly_int8_create")
+        self._plan = _hip.Handle(handle, "fly_int8_destroy")
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: torch.Tensor | None = None) -> "Int8Linear":
+        """A float weight, quantised with a scale for each channel."""
+        q, scale = quantize_rows(weight.detach())
+        return cls(q, scale, bias.detach().float() if bias is not None else None)
+
+    def __call__(self, x: torch.Tensor, out_dtype: torch.dtype = torch.float32,
+                 scale: torch.Tensor | None = None) -> torch.Tensor:
+        """x (rows, k) float32, float16 or bfloat16; or int8 with the rows' scales.  Returns (rows, channels)."""
+        x = _rows(x, "Int8Linear")
+        rows = x.shape[0]
+        if x.shape[1] != self.k or x.device != self.device:
+            raise RuntimeError(f"Int8Linear: x must be (rows, {self.k}) on {self.device}, "
+                               f"got {tuple(x.shape)} on {x.device}")
+        x_type, y_type = _hip.TYPES.get(x.dtype), FLOATS.get(out_dtype)
+        if x_type is None or y_type is None:
+            raise RuntimeError(f"Int8Linear: x must be float32, float16, bfloat16 or int8 and out_dtype one of the "
+                               f"floats, got {x.dtype} and {out_dtype}")
+        if (x.dtype == torch.int8) != (scale is not None):
+            raise RuntimeError("Int8Linear: int8 rows come with their scales, other rows without")
+        if scale is not None:
+            if scale.dtype != torch.float32 or scale.shape != (rows,) or scale.device != x.device:
+                raise RuntimeError(f"Int8Linear: scale must be float32 of shape ({rows},) on {x.device}, "
+                                   f"got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
+            scale = scale.contiguous()
+        y = torch.empty(rows, self.n, dtype=out_dtype, device=x.device)
+        lib = _hip.load()
+        ws = _hip.workspace(lib.fly_int8_workspace(self._plan.handle, rows), x.device)
+        with _hip.device_of(x):
+            _hip.check(lib.fly_int8_linear(self._plan.handle, x.data_ptr(), x_type, _hip.row_stride(x), _hip.ptr(scale),
+                                           rows, y.data_ptr(), y_type, self.n, ws.data_ptr(), ws.numel(),
+                                           _hip.stream(x.device)), "fly_int8_linear")
+        return y

@@ -45,6 +45,8 @@
  *                         gradients)
  *   fly_model_forward_static  no counterpart: the model forward for callers that cannot allocate
  *   fly_trim_memory       no counterpart: the idle device memory of destroyed objects, back to the runtime
+ *   fly_quantize_rows, fly_int8_*  no counterpart: a dense map held in 8 bits
+ *   fly_top_logits, fly_distill    no counterpart: a teacher's best moves, and a student's loss against them
  *   fly_profile_*, fly_set_tuning, fly_get_tuning  measurement and launch-shape choices (timing scripts)
  */
 #ifndef FLYEVAL_H
@@ -71,6 +73,9 @@ enum fly_mode {
     FLY_MODE_DEVIATION_F16 = 0,  /* fp16 deviation from the float32 resting trajectory (brain.py:254-280) */
     FLY_MODE_F32 = 1             /* float32 light-cone state (brain.py:295-329) */
 };
+
+/* Element types of the entry points that take more than one. */
+enum fly_type { FLY_F32 = 0, FLY_F16 = 1, FLY_BF16 = 2, FLY_I8 = 3 };
 
 typedef struct fly_cone fly_cone;
 typedef struct fly_plan fly_plan;
@@ -456,6 +461,51 @@ int fly_train_step_backward(int64_t rows, int64_t batch, const float *g_dev, int
                             const int32_t *usrc_dev, const float *hprev_dev, int64_t ldp, float h_max, float *gy_dev,
                             int64_t ldgy, float *gk_dev, float *ga_dev, float *gpdef_dev, float *gu_dev,
                             int64_t ldgu, float *ghprev_dev, int64_t ldgh, void *stream);
+
+/* ---- dense maps in 8 bits ------------------------------------------------------------------------ */
+/* No counterpart in the reference.  Rows to 8-bit integers with a scale each: q (rows, ldq) = rint(x * (127 / a)),
+ * scale = a / 127 with a = max |x| of the row, each step rounded to float32, x FLY_F32, FLY_F16 or FLY_BF16 (rows, ldx).
+ * A row that holds an infinity or NaN gets q = 0 and the scale NaN; a row below 2^-120 everywhere is zero. */
+int fly_quantize_rows(const void *x_dev, int32_t x_type, int64_t ldx, int64_t rows, int64_t cols, int8_t *q_dev,
+                      int64_t ldq, float *scale_dev, void *stream);
+
+/* A weight in 8 bits, laid out once for the matrix cores: w (n, ldw) int8 over k columns (k below 2^17), scale (n), bias
+ * (n) or NULL.  The plan copies what it needs. */
+typedef struct fly_int8 fly_int8;
+int fly_int8_create(const int8_t *w_dev, int64_t ldw, const float *scale_dev, const float *bias_dev, int64_t n,
+                    int64_t k, void *stream, fly_int8 **out);
+int fly_int8_destroy(fly_int8 *plan);
+/* y (rows, ldy) of y_type = (sum_k q[m, k] w[n, k]) (s[m] scale[n]) + bias[n]: integer sums exact, scaled in float32.
+ * x (rows, ldx) float32, float16 or bfloat16 is quantised by rows as fly_quantize_rows does (x_scale NULL); FLY_I8
+ * rows are taken as they are, with x_scale (rows).  rows below 2^20 - 16.  y must not overlap x. */
+size_t fly_int8_workspace(const fly_int8 *plan, int64_t rows);
+int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int64_t ldx, const float *x_scale_dev,
+                    int64_t rows, void *y_dev, int32_t y_type, int64_t ldy, void *workspace_dev,
+                    size_t workspace_bytes, void *stream);
+
+/* ---- distillation from a teacher's top logits ---------------------------------------------------- */
+/* No counterpart in the reference.  Logits z (rows, ldz) are FLY_F32, FLY_F16 or FLY_BF16 over cols columns (1 to 2^20); legal
+ * (rows, ldl) bytes, NULL or 0 for columns that do not exist for the row.  Columns at -inf count as not existing too.
+ * k lies in 1..256, the temperature is positive.
+ *
+ * fly_top_logits: values and index (rows, k): the k largest logits in falling order, the lower column first among
+ * equals (NaN above all), padded with -inf and -1; tail (rows) or NULL: log sum exp(z / temperature) over the columns
+ * not listed, -inf when there are none.
+ *
+ * fly_distill: from values, index (rows, k) and tail (rows; NULL: the teacher is its list alone) the loss (rows) and its
+ * gradient by z, either NULL: temperature^2 times the Kullback-Leibler divergence from the teacher's softmax to the
+ * student's at the temperature, over the listed columns and one class for all others.
+ * grad (rows, ldg) of z's type = grad_scale * row_scale[r] (NULL: 1) * dloss[r]/dz, 0 on columns that do not exist.
+ * Entries with index -1 (any negative), or on a column that does not exist by `legal`, are left out; so is the tail
+ * where the student has no column outside the list.  A row with no entry left, or whose student has no column, gives 0.
+ * A repeated index, or one at or past cols, makes the row NaN.  grad must not overlap z. */
+int fly_top_logits(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int64_t cols, const uint8_t *legal_dev,
+                   int64_t ldl, int32_t k, float temperature, float *values_dev, int32_t *index_dev, float *tail_dev,
+                   void *stream);
+int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int64_t cols, const uint8_t *legal_dev,
+                int64_t ldl, const float *values_dev, const int32_t *index_dev, const float *tail_dev, int32_t k,
+                float temperature, float *loss_dev, void *grad_dev, int64_t ldg, const float *row_scale_dev,
+                float grad_scale, void *stream);
 
 /* ---- measurement ------------------------------------------------------------------------------- */
 
