@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ x, int64
 #pragma unroll
     for (int e = 0; e < N; ++e) top = abs_max(top, p.v[e]);
   }
-  top = wave_max(top);
+  top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
   const RowScale s = row_scale(top);
   if (lane == 0) scale[row] = s.scale;
   const int64_t chunks = PACKED ? 4 * kb : (k + 15) / 16;

@@ -22,13 +22,55 @@ struct Piece {
 };
 
 template <typename T>
+constexpr uint32_t kLowest = std::is_same_v<T, float> ? 0xff800000u : std::is_same_v<T, bhalf> ? 0xff80u : 0xfc00u;   // -inf
+
+template <typename T>
 __device__ __forceinline__ float to_float(uint32_t bits) {   // the low bits hold a T
   if constexpr (std::is_same_v<T, float>) return __uint_as_float(bits);
   else if constexpr (std::is_same_v<T, bhalf>) return __uint_as_float(bits << 16);
   else return static_cast<float>(__builtin_bit_cast(_Float16, (uint16_t)bits));
 }
+template <typename T>
+__device__ __forceinline__ uint32_t to_bits(T v) {
+  if constexpr (std::is_same_v<T, float>) return __float_as_uint(v);
+  else return __builtin_bit_cast(uint16_t, v);
+}
 
-// Elements [i N, i N + N) of a row of `cols`; `fill` past its end.
+// Element e of a piece, and -inf in its place.
+template <typename T>
+__device__ __forceinline__ float element(const Raw16 &p, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(p.v[e]);
+  else if constexpr (std::is_same_v<T, bhalf>)
+    return __uint_as_float((e & 1) ? p.v[e / 2] & 0xffff0000u : p.v[e / 2] << 16);
+  else return to_float<T>((e & 1) ? p.v[e / 2] >> 16 : p.v[e / 2] & 0xffffu);
+}
+template <typename T>
+__device__ __forceinline__ void erase(Raw16 &p, int e) {
+  if constexpr (sizeof(T) == 4) p.v[e] = kLowest<T>;
+  else if (e & 1) p.v[e / 2] = (p.v[e / 2] & 0xffffu) | kLowest<T> << 16;
+  else p.v[e / 2] = (p.v[e / 2] & 0xffff0000u) | kLowest<T>;
+}
+
+// Elements [i N, i N + N) of a row of `cols`, -inf past its end.
+template <typename T>
+__device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int64_t i, int64_t cols) {
+  constexpr int N = Piece<T>::N;
+  const int64_t c = i * N;
+  if (c + N <= cols) return *reinterpret_cast<const Raw16 *>(row + c);
+  Raw16 p;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) p.v[w] = sizeof(T) == 4 ? kLowest<T> : kLowest<T> * 0x10001u;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (c + e < cols) {
+      const uint32_t b = to_bits(row[c + e]);
+      if constexpr (sizeof(T) == 4) p.v[e] = b;
+      else p.v[e / 2] = (e & 1) ? (p.v[e / 2] & 0xffffu) | b << 16 : (p.v[e / 2] & 0xffff0000u) | b;
+    }
+  return p;
+}
+
+// The same as floats, `fill` past the row's end.
 template <typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T *__restrict__ row, int64_t i, int64_t cols, float fill) {
   constexpr int N = Piece<T>::N;
@@ -37,10 +79,7 @@ __device__ __forceinline__ Piece<T> load_piece(const T *__restrict__ row, int64_
   if (c + N <= cols) {
     const Raw16 raw = *reinterpret_cast<const Raw16 *>(row + c);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if constexpr (N == 4) p.v[e] = __uint_as_float(raw.v[e]);
-      else p.v[e] = to_float<T>((e & 1) ? raw.v[e / 2] >> 16 : raw.v[e / 2] & 0xffffu);
-    }
+    for (int e = 0; e < N; ++e) p.v[e] = element<T>(raw, e);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e) p.v[e] = c + e < cols ? static_cast<float>(row[c + e]) : fill;
@@ -57,9 +96,7 @@ __device__ __forceinline__ void store_piece(T *__restrict__ row, int64_t i, int6
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if constexpr (N == 4) raw.v[w] = __float_as_uint(p.v[w]);
-      else
-        raw.v[w] = (uint32_t)__builtin_bit_cast(uint16_t, static_cast<T>(p.v[2 * w])) |
-                   (uint32_t)__builtin_bit_cast(uint16_t, static_cast<T>(p.v[2 * w + 1])) << 16;
+      else raw.v[w] = to_bits(static_cast<T>(p.v[2 * w])) | to_bits(static_cast<T>(p.v[2 * w + 1])) << 16;
     }
     *reinterpret_cast<Raw16 *>(row + c) = raw;
   } else {
@@ -71,7 +108,7 @@ __device__ __forceinline__ void store_piece(T *__restrict__ row, int64_t i, int6
 
 // Columns whose byte in `seen` (a row of the mask, any alignment) is 0 become -inf.
 template <typename T>
-__device__ __forceinline__ void mask_piece(Piece<T> &p, const uint8_t *__restrict__ seen, int64_t i, int64_t cols) {
+__device__ __forceinline__ void mask_raw(Raw16 &p, const uint8_t *__restrict__ seen, int64_t i, int64_t cols) {
   constexpr int N = Piece<T>::N;
   struct __attribute__((packed)) Bytes {
     uint32_t w[N / 4];
@@ -81,67 +118,97 @@ __device__ __forceinline__ void mask_piece(Piece<T> &p, const uint8_t *__restric
     const Bytes b = *reinterpret_cast<const Bytes *>(seen + c);
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (!((b.w[e / 4] >> (8 * (e & 3))) & 0xffu)) p.v[e] = -INFINITY;
+      if (!((b.w[e / 4] >> (8 * (e & 3))) & 0xffu)) erase<T>(p, e);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c + e < cols && !seen[c + e]) p.v[e] = -INFINITY;
+      if (c + e < cols && !seen[c + e]) erase<T>(p, e);
   }
 }
 
+// x from lane ^ 1, ^ 2 (within 4 lanes), rotated by 4 and 8 within 16, and across the 16- and 32-lane halves: six steps
+// on the vector ALU that leave a whole wave's sum or maximum in every lane.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float v, F &&f) {
+  v = f(v, dpp<0xB1>(v));    // quad_perm 1 0 3 2
+  v = f(v, dpp<0x4E>(v));    // quad_perm 2 3 0 1
+  v = f(v, dpp<0x124>(v));   // row_ror:4
+  v = f(v, dpp<0x128>(v));   // row_ror:8
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  v = f(__int_as_float(h[0]), __int_as_float(h[1]));
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return f(__int_as_float(w[0]), __int_as_float(w[1]));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  return wave_reduce(v, [](float a, float b) { return a + b; });
 }
-__device__ __forceinline__ float wave_max(float v) {   // NaN where any lane has one
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float o = __shfl_xor(v, d);
-    v = (o > v || o != o) ? o : v;
-  }
-  return v;
+__device__ __forceinline__ float wave_max(float v) {   // of numbers: NaN only where every lane has one
+  return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float nan_max(float a, float b) { return b > a || b != b ? b : a; }
+
+// sum exp2((x - top) scale): a part of a log-sum-exp.  Of nothing: {-inf, 0}.  NaN among the terms makes the sum NaN whatever
+// top is.  The maximum is taken off before the scale is put on: a type's lowest value, which masks are made of, would
+// pass the range otherwise.
+struct PartSum {
+  float top, sum;
+  __device__ __forceinline__ bool empty() const { return top == -INFINITY && sum == 0.0f; }
+};
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }   // no inf - inf
+__device__ __forceinline__ PartSum wave_part(PartSum p, float scale) {
+  const float top = wave_max(p.top);
+  p.sum = wave_sum(p.sum * exp2f((p.top - base_of(top)) * scale));
+  p.top = top;
+  return p;
 }
 
-// C values over the workgroup, in every thread; `share` holds C * (waves) floats.  Sums add in wave order.
+// x joins a part
+__device__ __forceinline__ void join(PartSum &p, float x, float scale) {
+  const float top = fmaxf(p.top, x), base = base_of(top);
+  p.sum = p.sum * exp2f((p.top - base) * scale) + exp2f((x - base) * scale);
+  p.top = top;
+}
+
+// C parts over the workgroup, in every thread; `share` holds 2 C * waves floats.  Shares add in wave order.
 template <int C>
-__device__ __forceinline__ void block_sum(float (&v)[C], float *share) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = (blockDim.x + 63) >> 6;
+__device__ __forceinline__ void block_part(PartSum (&p)[C], float scale, float *share) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) v[c] = wave_sum(v[c]);
+  for (int c = 0; c < C; ++c) p[c] = wave_part(p[c], scale);
+  const int waves = blockDim.x >> 6;
   if (waves == 1) return;
-  __syncthreads();
-  if (lane == 0)
+  if ((threadIdx.x & 63) == 0)
 #pragma unroll
-    for (int c = 0; c < C; ++c) share[c * waves + wave] = v[c];
+    for (int c = 0; c < C; ++c) {
+      share[2 * (c * waves + (threadIdx.x >> 6))] = p[c].top;
+      share[2 * (c * waves + (threadIdx.x >> 6)) + 1] = p[c].sum;
+    }
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    float s = share[c * waves];
-    for (int w = 1; w < waves; ++w) s += share[c * waves + w];
-    v[c] = s;
+    const float2 *all = reinterpret_cast<const float2 *>(share) + c * waves;
+    float top = all[0].x;
+    for (int w = 1; w < waves; ++w) top = fmaxf(top, all[w].x);
+    const float base = base_of(top);
+    float sum = 0.0f;
+    for (int w = 0; w < waves; ++w) sum += all[w].y * exp2f((all[w].x - base) * scale);
+    p[c] = {top, sum};
   }
 }
-template <int C>
-__device__ __forceinline__ void block_max(float (&v)[C], float *share) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = (blockDim.x + 63) >> 6;
-#pragma unroll
-  for (int c = 0; c < C; ++c) v[c] = wave_max(v[c]);
-  if (waves == 1) return;
+
+// v over the workgroup, in every thread; `share` holds a float for each wave.
+__device__ __forceinline__ float block_sum(float v, float *share) {
+  v = wave_sum(v);
+  const int waves = blockDim.x >> 6;
+  if (waves == 1) return v;
+  if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (lane == 0)
-#pragma unroll
-    for (int c = 0; c < C; ++c) share[c * waves + wave] = v[c];
-  __syncthreads();
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    float s = share[c * waves];
-    for (int w = 1; w < waves; ++w) {
-      const float o = share[c * waves + w];
-      s = (o > s || o != o) ? o : s;
-    }
-    v[c] = s;
-  }
+  v = share[0];
+  for (int w = 1; w < waves; ++w) v += share[w];
+  return v;
 }
 
 }  // namespace fly
