@@ -19,64 +19,110 @@ namespace {
 constexpr int kMostListed = 256;             // no chess position has over 218 legal moves
 constexpr int64_t kMostColumns = 1 << 20;    // a bit for each column in LDS: 128 KB
 
-// A row's 16-byte pieces, piece tid + j * blockDim for j < NV in a thread's registers (RES), or read again at each pass.
+// A row's 16-byte pieces, piece tid + j * blockDim for j < NV in a thread's registers (RES), or read again at each pass; a
+// last piece that is not whole belongs to thread 0.
 template <typename T, int NV, bool RES>
 struct Row {
   static constexpr int N = Piece<T>::N;
   const T *z;
   const uint8_t *seen;
-  int64_t cols, pieces;
-  Raw16 kept[RES ? NV : 1];
+  int full, left;   // whole pieces, and elements behind them
+  Raw16 kept[RES ? NV : 1], last;
 
-  __device__ __forceinline__ Row(const T *row, const uint8_t *mask, int64_t n) : z(row), seen(mask), cols(n), pieces((n + N - 1) / N) {
+  __device__ __forceinline__ Row(const T *row, const uint8_t *mask, int cols)
+      : z(row), seen(mask), full(cols / N), left(threadIdx.x == 0 ? cols % N : 0) {
     if constexpr (RES) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int64_t i = threadIdx.x + j * (int64_t)blockDim.x;
-        if (i < pieces) kept[j] = load_raw(z, i, cols);
+        const int i = threadIdx.x + j * blockDim.x;
+        kept[j] = i < full ? load_whole(z, i) : nothing();
       }
       if (seen)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int64_t i = threadIdx.x + j * (int64_t)blockDim.x;
-          if (i < pieces) mask_raw<T>(kept[j], seen, i, cols);
+          const int i = threadIdx.x + j * blockDim.x;
+          if (i < full) mask_whole<T>(kept[j], seen, i);
         }
     }
+    last = nothing();
+    if (left) {
+      last = load_last(z, full, left);
+      if (seen) mask_last<T>(last, seen, full, left);
+    }
   }
-  // f(piece number, piece) for this thread's pieces, columns that do not exist at -inf
+  // The next pass takes the pieces apart again: left alone, the compiler keeps every element of 16 bits as a float of its
+  // own from pass to pass, twice the registers.
+  __device__ __forceinline__ void forget() {
+    if constexpr (RES && sizeof(T) == 2)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(kept[j].v[w]));
+  }
+  static __device__ __forceinline__ Raw16 nothing() {
+    constexpr uint32_t w = sizeof(T) == 4 ? kLowest<T> : kLowest<T> * 0x10001u;
+    return Raw16{{w, w, w, w}};
+  }
+  // f(piece number, piece) for whole waves at once: lanes past the row's end have a piece of -inf
+  template <typename F>
+  __device__ __forceinline__ void each_wave(F &&f) {
+    const int first = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u), lane = threadIdx.x & 63;
+    if constexpr (RES) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (first + j * (int)blockDim.x < full) f(first + j * (int)blockDim.x + lane, kept[j]);
+    } else {
+      for (int i0 = first; i0 < full; i0 += blockDim.x) {
+        Raw16 p = nothing();
+        if (i0 + lane < full) {
+          p = load_whole(z, i0 + lane);
+          if (seen) mask_whole<T>(p, seen, i0 + lane);
+        }
+        f(i0 + lane, p);
+      }
+    }
+    if (first == 0 && __builtin_amdgcn_readfirstlane(left)) f(full, last);   // of -inf but in lane 0
+  }
+  // f(j, piece number, piece) for this thread's pieces, columns that do not exist at -inf; j = -1 for the last one where it
+  // is not whole (a constant after inlining)
   template <typename F>
   __device__ __forceinline__ void each(F &&f) {
     if constexpr (RES) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int64_t i = threadIdx.x + j * (int64_t)blockDim.x;
-        if (i < pieces) f(i, kept[j]);
+        const int i = threadIdx.x + j * blockDim.x;
+        if (i < full) f(j, i, kept[j]);
       }
     } else {
-      for (int64_t i = threadIdx.x; i < pieces; i += blockDim.x) {
-        Raw16 p = load_raw(z, i, cols);
-        if (seen) mask_raw<T>(p, seen, i, cols);
-        f(i, p);
+      for (int i = threadIdx.x; i < full; i += blockDim.x) {
+        Raw16 p = load_whole(z, i);
+        if (seen) mask_whole<T>(p, seen, i);
+        f(0, i, p);
       }
     }
+    if (left) f(-1, full, last);
   }
 };
 
-// How many pieces a thread keeps and how many threads a row gets: {1, 2, 4, 8} pieces, the fewest that 512 threads cover a
-// row with, or 8 on up to 1,024 threads; longer rows are read at every pass (kept = 0) by 1,024 threads.
+// How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
+// threads cover a row with.  From 1,024 rows on (4 for each CU): 8, since what a wave does once per row weighs more than
+// the waves that are left idle.  Up to 1,024 threads; longer rows are read at every pass (kept = 0).
 struct RowShape {
   int kept, threads;
 };
-RowShape row_shape(int64_t cols, size_t elem, int least) {
+RowShape row_shape(int64_t rows, int64_t cols, size_t elem, int least) {
   const int64_t pieces = (cols * (int64_t)elem + 15) / 16;
   for (int kept : {1, 2, 4, 8}) {
     const int64_t threads = std::max<int64_t>(round_up((pieces + kept - 1) / kept, 64), least);
-    if (threads <= (kept == 8 ? 1024 : 512)) return {kept, (int)threads};
+    if (kept == 8 ? threads <= 1024 : threads <= 512 && rows < 1024) return {kept, (int)threads};
   }
   return {0, 1024};
 }
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kMostFloat = 3.4028234663852886e38f;
+
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * kLog2e); }
+__device__ __forceinline__ float ln_of(float x) { return log2_of(x) * kLn2; }
 
 // ---- top logits ----------------------------------------------------------------------------------------------------
 
@@ -91,38 +137,69 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-constexpr int kMostCandidates = 1024;
+constexpr int kMostCandidates = 1024, kWaveCandidates = 128;
 
+// What a workgroup of k_top keeps in LDS besides these: 128 entries for each wave of the joined list (at most 1,024), and of
+// the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take later.
 struct TopShared {
-  union {
-    uint64_t list[kMostCandidates];
-    uint32_t hist[256];
-  };
-  float share[2 * 16];
+  alignas(16) float share[2 * 16];
   uint32_t wave[16];
   uint32_t count, prefix, need;
-  int32_t cut;
 };
+size_t top_lds(int threads) {
+  const int waves = threads / 64;
+  return 8 * (size_t)(std::min(waves * kWaveCandidates, kMostCandidates) + waves * kWaveCandidates);
+}
 
-__device__ __forceinline__ uint64_t candidate(float v, int64_t col) {   // larger is better: the key, then the lower column
+__device__ __forceinline__ uint64_t candidate(float v, int32_t col) {   // larger is better: the key, then the lower column
   return (uint64_t)order_key(v) << 32 | (uint32_t)~(uint32_t)col;
 }
 
-// The K largest of `count` candidates in their places, the others to rest(value); any number of threads.
-template <typename T, typename F>
-__device__ __forceinline__ void rank_candidates(const TopShared &s, int count, int k, const T *z, float *values,
-                                                int32_t *index, F &&rest) {
-  for (int i = threadIdx.x; i < count; i += blockDim.x) {
-    const uint64_t mine = s.list[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += s.list[j] > mine;
+// 64 candidates of a wave in falling order
+__device__ __forceinline__ uint64_t sort_wave(uint64_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int d = size >> 1; d; d >>= 1) {
+      const uint64_t o = __shfl_xor((unsigned long long)v, d);
+      const bool larger = ((lane & d) == 0) == ((lane & size) == 0 || size == 64);   // this lane keeps the larger one
+      v = (o > v) == larger ? o : v;
+    }
+  return v;
+}
+
+// The K largest of the list's `count` candidates in their places, the others to `spare`, each by its rank: the list's own
+// order is that of the waves and lanes that met its entries, and nothing may depend on it.  Each 64 are sorted by a
+// wave; an entry's rank is its place among them plus, in each of the other 64, the place that a search finds for it.
+template <typename T>
+__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int count, int k, const T *z, float *values, int32_t *index) {
+  const int lane = threadIdx.x & 63, parts = (count + 63) >> 6;
+  for (int p = threadIdx.x >> 6; p < parts; p += blockDim.x >> 6) {
+    const uint64_t v = sort_wave(p * 64 + lane < count ? list[p * 64 + lane] : 0);
+    list[p * 64 + lane] = v;
+  }
+  __syncthreads();
+  for (int p = threadIdx.x >> 6; p < parts; p += blockDim.x >> 6) {
+    const uint64_t mine = list[p * 64 + lane];
+    int rank = lane;
+    for (int o = 0; o < parts; ++o) {
+      if (o == p) continue;
+      const uint64_t *other = list + o * 64;
+      int before = 0;
+#pragma unroll
+      for (int step = 32; step; step >>= 1)
+        if (other[before + step - 1] > mine) before += step;
+      rank += before + (other[before] > mine);   // before <= 63
+    }
+    if (mine == 0) continue;   // behind the last candidate
     const int32_t col = (int32_t)~(uint32_t)mine;
     const float v = static_cast<float>(z[col]);
     if (rank < k) {
       values[rank] = v;
       index[rank] = col;
     } else {
-      rest(v);
+      spare[rank - k] = v;
     }
   }
   for (int i = count + threadIdx.x; i < k; i += blockDim.x) {
@@ -131,30 +208,31 @@ __device__ __forceinline__ void rank_candidates(const TopShared &s, int count, i
   }
 }
 
+__device__ __forceinline__ int lanes_before(uint64_t lanes) {   // of the ballot, below this lane
+  return __builtin_amdgcn_mbcnt_hi(lanes >> 32, __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
+
 // Where a bound leaves too many candidates (ties): the K-th key a byte at a time, its ties by column order, and the rest's
-// part of the tail.  The list then holds the row's K.  Reads the row again for each pass.
+// part of the tail.  The list then holds the row's K.  Reads the row again, a column at a time, for each pass.
 template <typename T>
-__device__ __forceinline__ PartSum top_by_digits(TopShared &s, const T *z, const uint8_t *seen, int64_t cols, int k, float scale) {
-  Row<T, 1, false> row(z, seen, cols);
-  constexpr int N = Piece<T>::N;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+__device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, uint32_t *hist, const T *z, const uint8_t *seen, int cols, int k, float scale) {
+  const int tid = threadIdx.x, wave = tid >> 6, waves = blockDim.x >> 6;
+  auto logit = [&](int c) { return c < cols && (!seen || seen[c]) ? static_cast<float>(z[c]) : -INFINITY; };
   uint32_t prefix = 0, need = k;
+#pragma unroll 1
   for (int shift = 24; shift >= 0; shift -= 8) {
     __syncthreads();
-    for (int i = tid; i < 256; i += blockDim.x) s.hist[i] = 0;
+    for (int i = tid; i < 256; i += blockDim.x) hist[i] = 0;
     __syncthreads();
-    row.each([&](int64_t, const Raw16 &p) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t key = order_key(element<T>(p, e));
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s.hist[(key >> shift) & 255], 1u);
-      }
-    });
+    for (int c = tid; c < cols; c += blockDim.x) {
+      const uint32_t key = order_key(logit(c));
+      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1u);
+    }
     __syncthreads();
     if (tid == 0) {
       uint32_t left = need;
       int d = 255;
-      for (; d > 0 && s.hist[d] < left; --d) left -= s.hist[d];
+      for (; d > 0 && hist[d] < left; --d) left -= hist[d];
       s.prefix = prefix | (uint32_t)d << shift;
       s.need = left;
     }
@@ -163,83 +241,55 @@ __device__ __forceinline__ PartSum top_by_digits(TopShared &s, const T *z, const
     need = s.need;
   }
   // prefix: the k-th key (0: fewer than k columns are seen); need: how many of its ties are listed, lowest column first
-  if (tid == 0) {
-    s.count = 0;
-    s.cut = -1;
-  }
-  __syncthreads();
+  if (tid == 0) s.count = 0;
+  PartSum part{-INFINITY, 0.0f};
   uint32_t before = 0;   // ties in earlier rounds
-  for (int64_t i0 = 0; i0 < row.pieces; i0 += blockDim.x) {
-    uint32_t key[N] = {}, eq = 0;
-    if (i0 + tid < row.pieces) {
-      Raw16 p = load_raw(row.z, i0 + tid, row.cols);
-      if (row.seen) mask_raw<T>(p, row.seen, i0 + tid, row.cols);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        key[e] = order_key(element<T>(p, e));
-        eq += key[e] == prefix && prefix != 0;
-      }
-    }
-    uint32_t at = eq;   // inclusive prefix sum of the ties in thread order, which is column order
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = __shfl_up(at, d);
-      if (lane >= d) at += o;
-    }
-    if (lane == 63) s.wave[wave] = at;
+#pragma unroll 1
+  for (int c0 = 0; c0 < cols; c0 += blockDim.x) {
+    const float v = logit(c0 + tid);
+    const uint32_t key = order_key(v);
+    const bool tie = key == prefix && prefix != 0;
+    const uint64_t lanes = __ballot(tie);
     __syncthreads();
-    uint32_t rank = before + at - eq;
+    if ((tid & 63) == 0) s.wave[wave] = __popcll(lanes);
+    __syncthreads();
+    uint32_t rank = before + lanes_before(lanes);   // in column order, which is thread order
     for (int w = 0; w < waves; ++w) {
       if (w < wave) rank += s.wave[w];
       before += s.wave[w];
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      bool take = key[e] > prefix;
-      const int32_t col = (int32_t)((i0 + tid) * N + e);
-      if (key[e] == prefix && prefix != 0) {
-        take = rank < need;
-        if (rank == need - 1) s.cut = col;
-        ++rank;
-      }
-      if (take) s.list[atomicAdd(&s.count, 1u)] = (uint64_t)key[e] << 32 | (uint32_t)~(uint32_t)col;
-    }
-    __syncthreads();
+    if (key > prefix || (tie && rank < need)) list[atomicAdd(&s.count, 1u)] = candidate(v, c0 + tid);
+    else if (key != 0) join(part, v, scale);
   }
-  const int32_t cut = s.cut;
-  PartSum part{-INFINITY, 0.0f};
-  row.each([&](int64_t i, const Raw16 &p) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = element<T>(p, e);
-      const uint32_t key = order_key(v);
-      if (key != 0 && (key < prefix || (key == prefix && (int32_t)(i * N + e) > cut))) join(part, v, scale);
-    }
-  });
+  __syncthreads();
   return part;
 }
 
 // One workgroup per row.  A bound from below: with W waves and c = ceil(K / W), each wave has c lanes whose largest logit
 // is at least the wave's c-th largest of those, so the least of these over the waves has at least K logits at or above
-// it.  Few more than K are (a wave's lanes hold the row interleaved): they go to a list in LDS, where each counts those
-// before it.  NaN passes every bound.  A list that would not fit is left to top_by_digits.
+// it.  Few more than K are (a wave's lanes hold the row interleaved, and it has twice as many lanes as c): each wave
+// packs its own into LDS by ballots, without atomics, and the lists are joined and ranked.  NaN passes every bound.  Lists
+// that would not fit (ties) are left to top_by_digits.
 template <typename T, int NV, bool RES>
-__global__ __launch_bounds__(1024) void k_top(const T *__restrict__ z, int64_t ldz, int64_t cols,
+__global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz, int64_t cols,
                                               const uint8_t *__restrict__ legal, int64_t ldl, int k, float inv_t,
                                               float *__restrict__ values, int32_t *__restrict__ index,
                                               float *__restrict__ tail) {
   constexpr int N = Piece<T>::N;
   __shared__ TopShared s;
+  extern __shared__ uint64_t lists[];
   const int tid = threadIdx.x, waves = blockDim.x >> 6;
   const float scale = inv_t * kLog2e;
   const int64_t r = blockIdx.x;
   const T *zr = z + r * ldz;
-  Row<T, NV, RES> row(zr, legal ? legal + r * ldl : nullptr, cols);
-  if (tid == 0) s.count = 0;
-  float top = -INFINITY;
-  row.each([&](int64_t, const Raw16 &p) {
+  Row<T, NV, RES> row(zr, legal ? legal + r * ldl : nullptr, (int)cols);
+  const int most = min(waves * kWaveCandidates, kMostCandidates);
+  uint64_t *list = lists;
+  float2 *found = reinterpret_cast<float2 *>(lists + most);
+  float top = -INFINITY;   // NaN where the lane has one
+  row.each([&](int, int, const Raw16 &p) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) top = fmaxf(top, element<T>(p, e));
+    for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, element<T>(p, e));
   });
   // the c-th largest of the wave's lanes, rounded down to its high 20 bits
   const int c = (k + waves - 1) / waves;
@@ -254,42 +304,90 @@ __global__ __launch_bounds__(1024) void k_top(const T *__restrict__ z, int64_t l
   __syncthreads();
   for (int w = 0; w < waves; ++w) bound = min(bound, s.wave[w]);
   const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
-  PartSum part{-INFINITY, 0.0f};
-  float low = -INFINITY;   // the largest logit below the bound
-  row.each([&](int64_t i, const Raw16 &p) {
+  row.forget();
+  // the candidates, into the wave's list
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int mine = 0;
+  row.each_wave([&](int i, const Raw16 &p) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float v = element<T>(p, e);
-      if (v < floor) {
-        low = fmaxf(low, v);
-      } else {
-        const uint32_t slot = atomicAdd(&s.count, 1u);
-        if (slot < kMostCandidates) s.list[slot] = candidate(v, i * N + e);
+      const uint64_t lanes = __ballot(!(v < floor));
+      if (lanes) {
+        if (!(v < floor)) {
+          const int slot = mine + lanes_before(lanes);
+          if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(i * N + e));
+        }
+        mine += __popcll(lanes);
       }
     }
   });
+  __syncthreads();   // every wave has read the others' bounds
+  if ((tid & 63) == 0) s.wave[wave] = mine;
   __syncthreads();
-  int count = (int)s.count;
-  if (count > kMostCandidates) {
-    part = top_by_digits<T>(s, zr, row.seen, cols, k, scale);
+  int count = 0, before = 0;
+  bool fits = true;
+  for (int w = 0; w < waves; ++w) {
+    const int n = s.wave[w];
+    fits &= n <= kWaveCandidates;
+    before += w < wave ? n : 0;
+    count += n;
+  }
+  fits &= count <= most;
+  if (fits) {
+    for (int i = tid & 63; i < mine; i += 64) list[before + i] = candidate(found[wave * kWaveCandidates + i].x, __float_as_int(found[wave * kWaveCandidates + i].y));
+    __syncthreads();
+  }
+  PartSum part{-INFINITY, 0.0f};
+  if (!fits) {
+    part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, row.seen, (int)cols, k, scale);
     count = (int)s.count;
   } else if (tail != nullptr) {
-    const float base = base_of(low);
+    // against the bound, which the rest stays below; where a lane's logits are so far below it that their sum would lose
+    // digits, or the bound is past what the scale allows, against the lane's own largest
+    const float shift = -floor * scale;
     float sum = 0.0f;
-    row.each([&](int64_t, const Raw16 &p) {
+    row.forget();
+    row.each([&](int, int, const Raw16 &p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float v = element<T>(p, e);
-        sum += v < floor ? exp2f((v - base) * scale) : 0.0f;
+        const float v = element<T>(p, e), x = exp2_of(fmaf(v, scale, shift));
+        sum += v < floor ? x : 0.0f;
       }
     });
-    part = {low, sum};
+    part = {floor, sum};
+    if (top != -INFINITY && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
+      float low = -INFINITY;
+      row.forget();
+      row.each([&](int, int, const Raw16 &p) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v = element<T>(p, e);
+          if (v < floor) low = fmaxf(low, v);
+        }
+      });
+      const float base = base_of(low);
+      sum = 0.0f;
+      row.forget();
+      row.each([&](int, int, const Raw16 &p) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float v = element<T>(p, e), x = exp2_of((v - base) * scale);
+          sum += v < floor ? x : 0.0f;
+        }
+      });
+      part = {low, sum};
+    } else if (top == -INFINITY) {
+      part = {-INFINITY, 0.0f};
+    }
   }
-  rank_candidates(s, count, k, zr, values + r * k, index + r * k, [&](float v) { join(part, v, scale); });
+  rank_candidates(list, reinterpret_cast<float *>(found), count, k, zr, values + r * k, index + r * k);
   if (tail == nullptr) return;
+  __syncthreads();
+  for (int i = tid; i < count - k; i += blockDim.x) join(part, reinterpret_cast<float *>(found)[i], scale);
   PartSum all[1] = {part};
   block_part(all, scale, s.share);
-  if (tid == 0) tail[r] = all[0].empty() ? -INFINITY : fmaf(base_of(all[0].top), inv_t, log2f(all[0].sum) * kLn2);
+  if (tid == 0) tail[r] = all[0].empty() ? -INFINITY : fmaf(base_of(all[0].top), inv_t, log2_of(all[0].sum) * kLn2);
 }
 
 // ---- distillation --------------------------------------------------------------------------------------------------
@@ -312,141 +410,222 @@ struct DistillArgs {
   float grad_scale;
 };
 
-// p log(p/q) - p + q for log p, log q and their exponentials; near p = q the logarithms' difference d is small and
-// p (d + exp(-d) - 1) keeps its digits.
+// p log(p/q) - p + q for log p, log q and their exponentials.  Near p = q the logarithms' difference d is small and
+// p (d + exp(-d) - 1) keeps its digits: d^2 (1/2! - d/3! + d^2/4! ...), whose terms past d^8 are below 2^-24 of it.
 __device__ __forceinline__ float divergence(float logp, float p, float logq, float q) {
   if (p == 0.0f) return q;
   const float d = logp - logq;
-  return fabsf(d) < 0.5f ? p * (d + expm1f(-d)) : p * d - p + q;
+  float s = 1.0f / 40320;
+  s = fmaf(-d, s, 1.0f / 5040);
+  s = fmaf(-d, s, 1.0f / 720);
+  s = fmaf(-d, s, 1.0f / 120);
+  s = fmaf(-d, s, 1.0f / 24);
+  s = fmaf(-d, s, 1.0f / 6);
+  s = fmaf(-d, s, 0.5f);
+  return fabsf(d) < 0.5f ? p * (d * d * s) : p * d - p + q;
 }
 
-// One workgroup per row.
+// One workgroup per row.  The first waves hold the list and compute the row's scalars; the others wait for the factor of
+// their exponentials, so what does not depend on the columns is computed once and not by every wave.
 template <typename T, int NV, bool RES>
-__global__ __launch_bounds__(1024) void k_distill(const DistillArgs<T> a) {
+__global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const DistillArgs<T> a) {
   constexpr int N = Piece<T>::N;
-  constexpr int kEntries = kMostListed / 64;   // of the list, at most, for a thread
+  constexpr bool kKeep = RES && NV * N <= 32;  // the exponentials stay in registers for the gradient
   extern __shared__ uint32_t bits[];           // one for each column: listed
-  __shared__ float share[6 * 16], share_loss[16];
-  const int tid = threadIdx.x, threads = blockDim.x;
+  __shared__ __attribute__((aligned(16))) float share[6 * 16], share_loss[2 * (kMostListed / 64)];
+  __shared__ float s_factor, s_base, s_loss;
+  __shared__ bool s_nothing;
+  // the list, an entry in a thread's care throughout: the teacher's logit, then the gradient; the student's; the column
+  __shared__ float list_v[kMostListed], list_z[kMostListed];
+  __shared__ int32_t list_c[kMostListed];
+  const int tid = threadIdx.x, threads = blockDim.x, wave = tid >> 6;
+  const int few = (min(a.k, threads) + 63) >> 6;   // waves that hold the list
   const int64_t r = blockIdx.x;
   const T *zr = a.z + r * a.ldz;
   const uint8_t *seen = a.legal ? a.legal + r * a.ldl : nullptr;
-  Row<T, NV, RES> row(zr, seen, a.cols);
-  for (int64_t w = tid; w < (a.cols + 31) / 32; w += threads) bits[w] = 0;
+  Row<T, NV, RES> row(zr, seen, (int)a.cols);
+  for (int w = tid; w < ((int)a.cols + 31) / 32; w += threads) bits[w] = 0;
   __syncthreads();
-  float av[kEntries], zs[kEntries];
-  int32_t col[kEntries];
   bool bad = false;
-#pragma unroll
-  for (int j = 0; j < kEntries; ++j) {
-    av[j] = zs[j] = -INFINITY;
-    col[j] = -1;
-    const int i = tid + j * threads;
-    if (i < a.k) {
-      const int32_t c = a.index[r * a.k + i];
-      if (c >= a.cols) {
-        bad = true;
-      } else if (c >= 0 && (!seen || seen[c])) {
+  for (int i = tid; i < a.k; i += threads) {
+    const int32_t c = a.index[r * a.k + i];
+    const float v = a.values[r * a.k + i];
+    int32_t col = -1;
+    float zc = 0.0f;
+    if (c >= a.cols) {
+      bad = true;
+    } else if (c >= 0) {
+      zc = static_cast<float>(zr[c]);   // asked for with the mask's byte, not after it
+      if (!seen || seen[c]) {
         const uint32_t bit = 1u << (c & 31);
-        if (atomicOr(&bits[c >> 5], bit) & bit) {
-          bad = true;
-        } else {
-          col[j] = c;
-          av[j] = a.values[r * a.k + i];
-          zs[j] = static_cast<float>(zr[c]);
-        }
+        if (atomicOr(&bits[c >> 5], bit) & bit) bad = true;
+        else col = c;
       }
     }
+    list_c[i] = col;
+    list_v[i] = v;
+    list_z[i] = zc;
   }
-  bad = __syncthreads_or(bad);
+  __syncthreads();
   // the rest, the teacher's list and the student's listed logits
   const float scale2 = a.inv_t * kLog2e;
   PartSum part[3] = {{-INFINITY, 0.0f}, {-INFINITY, 0.0f}, {-INFINITY, 0.0f}};
-  auto erase_listed = [&](int64_t i, Raw16 &p) {
+  auto erase_listed = [&](int i, Raw16 &p) {
     const uint32_t b = (bits[i * N >> 5] >> (i * N & 31)) & ((1u << N) - 1);
     if (b)
 #pragma unroll
       for (int e = 0; e < N; ++e)
         if ((b >> e) & 1) erase<T>(p, e);
   };
+  float kept[kKeep ? NV * N : 1];
+  float shift = 0.0f;   // of this thread's exponentials, in powers of two
   if constexpr (RES) {
     float top = -INFINITY, sum = 0.0f;
-    row.each([&](int64_t i, Raw16 &p) {
+    row.each([&](int, int i, Raw16 &p) {
       erase_listed(i, p);
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, element<T>(p, e));
     });
-    const float base = base_of(top);
-    row.each([&](int64_t, const Raw16 &p) {
+    float base = base_of(top);
+    if (fabsf(base) * scale2 > 1e37f) {
+      // the product with the scale would pass the range: near the type's lowest value the differences are exactly 0 or
+      // far beyond any exponent, so they take the logits' place
+      row.each([&](int, int, Raw16 &p) {
+        Raw16 d;
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp2f((element<T>(p, e) - base) * scale2);
+        for (int w = 0; w < 4; ++w) d.v[w] = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint32_t b = to_bits(static_cast<T>(element<T>(p, e) - base));
+          if constexpr (N == 4) d.v[e] = b;
+          else d.v[e / 2] |= b << (16 * (e & 1));
+        }
+        p = d;
+      });
+      base = 0.0f;
+    }
+    shift = -base * scale2;
+    if (!kKeep) row.forget();
+    row.each([&](int j, int, const Raw16 &p) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float x = exp2_of(fmaf(element<T>(p, e), scale2, shift));
+        if (kKeep && j >= 0) kept[kKeep && j >= 0 ? j * N + e : 0] = x;
+        sum += x;
+      }
     });
     part[0] = {top, sum};
   } else {
-    row.each([&](int64_t i, Raw16 &p) {
+    row.each([&](int, int i, Raw16 &p) {
       erase_listed(i, p);
       float top = part[0].top;
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, element<T>(p, e));
       const float base = base_of(top);
-      float sum = part[0].sum * exp2f((part[0].top - base) * scale2);
+      float sum = part[0].sum * exp2_of((part[0].top - base) * scale2);
 #pragma unroll
-      for (int e = 0; e < N; ++e) sum += exp2f((element<T>(p, e) - base) * scale2);
+      for (int e = 0; e < N; ++e) sum += exp2_of((element<T>(p, e) - base) * scale2);
       part[0] = {top, sum};
     });
   }
-#pragma unroll
-  for (int j = 0; j < kEntries; ++j)
-    if (col[j] >= 0) {
-      join(part[1], av[j], scale2);
-      join(part[2], zs[j], scale2);
+  const float own_top = part[0].top;
+  for (int i = tid; i < a.k; i += threads)
+    if (list_c[i] >= 0) {
+      join(part[1], list_v[i], scale2);
+      join(part[2], list_z[i], scale2);
     }
-  block_part(part, scale2, share);
-  // the student's normaliser, against its largest logit: log q = (z - mz) / T - ln_z
-  const bool has_rest = !part[0].empty();
-  const float mz = base_of(fmaxf(part[0].top, part[2].top)), rest_top = base_of(part[0].top);
-  const float ln_z = logf(part[0].sum * exp2f((part[0].top - mz) * scale2) + part[2].sum * exp2f((part[2].top - mz) * scale2));
-  const float logqt = has_rest ? (rest_top - mz) * a.inv_t + logf(part[0].sum) - ln_z : -INFINITY;
-  // the teacher's, its tail a scaled number already: log p = (v - mv) / T + (x - ma) - ln_a
-  const float at = a.tail && has_rest ? a.tail[r] : -INFINITY;   // no rest to put it on: the list alone
-  const float mv = base_of(part[1].top), x = part[1].empty() ? -kMostFloat : fmaxf(mv * a.inv_t, -kMostFloat);
-  const float ma = fmaxf(x, at);
-  const float ln_a = logf(part[1].sum * expf(x - ma) + expf(at - ma)), logpt = at - ma - ln_a;
-  const bool some = !(part[1].empty() && at == -INFINITY) && !(part[0].empty() && part[2].empty());
+  block_part(part, scale2, share, few);
   const float nan = __builtin_nanf("");
-  const float pt = some ? expf(logpt) : 0.0f, qt = some ? expf(logqt) : 0.0f;
-  float p[kEntries], q[kEntries], l = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kEntries; ++j) {
-    p[j] = q[j] = 0.0f;
-    if (col[j] >= 0 && some) {
-      const float logp = (av[j] - mv) * a.inv_t + (x - ma) - ln_a, logq = (zs[j] - mz) * a.inv_t - ln_z;
-      p[j] = expf(logp);
-      q[j] = expf(logq);
-      l += divergence(logp, p[j], logq, q[j]);
+  if (wave < few) {
+    // the student's normaliser, against its largest logit: log q = (z - mz) / T - ln_z
+    const bool has_rest = !part[0].empty();
+    const float mz = base_of(fmaxf(part[0].top, part[2].top)), rest_top = base_of(part[0].top);
+    const float ln_z = ln_of(part[0].sum * exp2_of((part[0].top - mz) * scale2) + part[2].sum * exp2_of((part[2].top - mz) * scale2));
+    const float logqt = has_rest ? (rest_top - mz) * a.inv_t + ln_of(part[0].sum) - ln_z : -INFINITY;
+    // the teacher's, its tail a scaled number already: log p = (v - mv) / T + (x - ma) - ln_a
+    const float at = a.tail && has_rest ? a.tail[r] : -INFINITY;   // no rest to put it on: the list alone
+    const float mv = base_of(part[1].top), x = part[1].empty() ? -kMostFloat : fmaxf(mv * a.inv_t, -kMostFloat);
+    const float ma = fmaxf(x, at);
+    const float ln_a = ln_of(part[1].sum * exp_of(x - ma) + exp_of(at - ma)), logpt = at - ma - ln_a;
+    const bool some = !(part[1].empty() && at == -INFINITY) && !(part[0].empty() && part[2].empty());
+    const float pt = some ? exp_of(logpt) : 0.0f, qt = some ? exp_of(logqt) : 0.0f;
+    const float scale = a.grad ? a.t * a.grad_scale * (a.row_scale ? a.row_scale[r] : 1.0f) : 0.0f;
+    float l = 0.0f;
+    for (int i = tid; i < a.k; i += threads)
+      if (list_c[i] >= 0 && some) {
+        const float logp = (list_v[i] - mv) * a.inv_t + (x - ma) - ln_a, logq = (list_z[i] - mz) * a.inv_t - ln_z;
+        const float p = exp_of(logp), q = exp_of(logq);
+        l += divergence(logp, p, logq, q);
+        list_v[i] = scale * (q - p);
+      }
+    l = wave_sum(l);
+    bad = __any(bad);
+    if (few > 1) {
+      if ((tid & 63) == 0) {
+        share_loss[2 * wave] = l;
+        share_loss[2 * wave + 1] = bad ? 1.0f : 0.0f;
+      }
+    }
+    if (tid == 0) {
+      s_base = rest_top;
+      s_nothing = !some;
+      s_factor = bad ? nan : has_rest ? scale * (qt - pt) / part[0].sum : 0.0f;
+      s_loss = some ? divergence(logpt, pt, logqt, qt) : 0.0f;   // the rest's share
+      if (few == 1 && a.loss) a.loss[r] = bad ? nan : a.t * a.t * (l + s_loss);
     }
   }
-  if (a.loss) {
-    l = block_sum(l, share_loss);
-    if (tid == 0)
-      a.loss[r] = bad ? nan : some ? a.t * a.t * (l + divergence(logpt, pt, logqt, qt)) : 0.0f;
+  __syncthreads();
+  float factor = s_factor;
+  if (few > 1) {
+    float l = share_loss[0], n = share_loss[1];
+    for (int w = 1; w < few; ++w) {
+      l += share_loss[2 * w];
+      n += share_loss[2 * w + 1];
+    }
+    bad = n != 0.0f;
+    if (tid == 0 && a.loss) a.loss[r] = bad ? nan : a.t * a.t * (l + s_loss);
+    if (bad) factor = nan;
   }
   if (!a.grad) return;
-  const float scale = a.t * a.grad_scale * (a.row_scale ? a.row_scale[r] : 1.0f);
-  const float coef = bad ? nan : some && has_rest ? scale * (qt - pt) / part[0].sum : 0.0f;
-  const bool nothing = !some && !bad;
   T *gr = a.grad + r * a.ldg;
-  row.each([&](int64_t i, Raw16 &v) {
-    if constexpr (!RES) erase_listed(i, v);
-    Piece<T> g;
+  auto store = [&](int j, int i, const Piece<T> &g) {
+    if (j < 0) store_last(gr, i, row.left, g);
+    else store_whole(gr, i, g);
+  };
+  if (s_nothing && factor == factor) {
+    row.each([&](int j, int i, const Raw16 &) {
+      Piece<T> g;
 #pragma unroll
-    for (int e = 0; e < N; ++e) g.v[e] = nothing ? 0.0f : exp2f((element<T>(v, e) - rest_top) * scale2) * coef;
-    store_piece(gr, i, a.cols, g);
-  });
+      for (int e = 0; e < N; ++e) g.v[e] = 0.0f;
+      store(j, i, g);
+    });
+    return;
+  }
+  if constexpr (RES) {
+    if (!kKeep) row.forget();
+    const float f = factor * exp2_of((base_of(own_top) - s_base) * scale2);
+    row.each([&](int j, int i, const Raw16 &p) {
+      Piece<T> g;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (kKeep && j >= 0) g.v[e] = kept[kKeep && j >= 0 ? j * N + e : 0] * f;
+        else g.v[e] = exp2_of(fmaf(element<T>(p, e), scale2, shift)) * f;
+      }
+      store(j, i, g);
+    });
+  } else {
+    const float base = s_base;
+    row.each([&](int j, int i, Raw16 &p) {
+      erase_listed(i, p);
+      Piece<T> g;
+#pragma unroll
+      for (int e = 0; e < N; ++e) g.v[e] = exp2_of((element<T>(p, e) - base) * scale2) * factor;
+      store(j, i, g);
+    });
+  }
   __syncthreads();   // the list's own gradients overwrite what the pass left in their columns
-#pragma unroll
-  for (int j = 0; j < kEntries; ++j)
-    if (col[j] >= 0 && some && !bad) gr[col[j]] = static_cast<T>(scale * (q[j] - p[j]));
+  for (int i = tid; i < a.k; i += threads)
+    if (list_c[i] >= 0) gr[list_c[i]] = static_cast<T>(bad ? nan : list_v[i]);
 }
 
 template <typename F>
@@ -495,9 +674,9 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
     by_type(type, [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      by_shape(row_shape(cols, sizeof(T), (int)round_up(k, 64)), [&](auto nv, auto res, int threads) {
-        hipLaunchKernelGGL((k_top<T, decltype(nv)::value, decltype(res)::value>), dim3((unsigned)rows), dim3(threads), 0,
-                           as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature,
+      by_shape(row_shape(rows, cols, sizeof(T), (int)round_up(2 * k, 64)), [&](auto nv, auto res, int threads) {
+        hipLaunchKernelGGL((k_top<T, decltype(nv)::value, decltype(res)::value>), dim3((unsigned)rows), dim3(threads),
+                           top_lds(threads), as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature,
                            values, index, tail);
       });
       check_launch("top logits");
@@ -520,7 +699,7 @@ extern "C" int fly_distill(const void *z, int32_t type, int64_t ldz, int64_t row
       const DistillArgs<T> a{static_cast<const T *>(z), ldz, cols, legal, ldl, values, index, tail, k, temperature,
                              1.0f / temperature, loss, static_cast<T *>(grad), ldg, row_scale, grad_scale};
       const size_t lds = (size_t)round_up(cols, 32) / 8;
-      by_shape(row_shape(cols, sizeof(T), 64), [&](auto nv, auto res, int threads) {
+      by_shape(row_shape(rows, cols, sizeof(T), 64), [&](auto nv, auto res, int threads) {
         constexpr auto kernel = &k_distill<T, decltype(nv)::value, decltype(res)::value>;
         if (lds > 60 * 1024)
           FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,

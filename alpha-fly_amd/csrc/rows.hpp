@@ -51,26 +51,28 @@ __device__ __forceinline__ void erase(Raw16 &p, int e) {
   else p.v[e / 2] = (p.v[e / 2] & 0xffff0000u) | kLowest<T>;
 }
 
-// Elements [i N, i N + N) of a row of `cols`, -inf past its end.
+// Whole piece i of a row, and the `left` < N elements of its last one, -inf behind them.
 template <typename T>
-__device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int64_t i, int64_t cols) {
+__device__ __forceinline__ Raw16 load_whole(const T *__restrict__ row, int i) {
+  return *reinterpret_cast<const Raw16 *>(row + (int64_t)i * Piece<T>::N);
+}
+template <typename T>
+__device__ __forceinline__ Raw16 load_last(const T *__restrict__ row, int i, int left) {
   constexpr int N = Piece<T>::N;
-  const int64_t c = i * N;
-  if (c + N <= cols) return *reinterpret_cast<const Raw16 *>(row + c);
   Raw16 p;
 #pragma unroll
   for (int w = 0; w < 4; ++w) p.v[w] = sizeof(T) == 4 ? kLowest<T> : kLowest<T> * 0x10001u;
 #pragma unroll
-  for (int e = 0; e < N; ++e)
-    if (c + e < cols) {
-      const uint32_t b = to_bits(row[c + e]);
+  for (int e = 0; e < N - 1; ++e)
+    if (e < left) {
+      const uint32_t b = to_bits(row[(int64_t)i * N + e]);
       if constexpr (sizeof(T) == 4) p.v[e] = b;
       else p.v[e / 2] = (e & 1) ? (p.v[e / 2] & 0xffffu) | b << 16 : (p.v[e / 2] & 0xffff0000u) | b;
     }
   return p;
 }
 
-// The same as floats, `fill` past the row's end.
+// Elements [i N, i N + N) of a row of `cols` as floats, `fill` past its end.
 template <typename T>
 __device__ __forceinline__ Piece<T> load_piece(const T *__restrict__ row, int64_t i, int64_t cols, float fill) {
   constexpr int N = Piece<T>::N;
@@ -88,43 +90,45 @@ __device__ __forceinline__ Piece<T> load_piece(const T *__restrict__ row, int64_
 }
 
 template <typename T>
-__device__ __forceinline__ void store_piece(T *__restrict__ row, int64_t i, int64_t cols, const Piece<T> &p) {
+__device__ __forceinline__ void store_whole(T *__restrict__ row, int i, const Piece<T> &p) {
   constexpr int N = Piece<T>::N;
-  const int64_t c = i * N;
-  if (c + N <= cols) {
-    Raw16 raw;
+  Raw16 raw;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if constexpr (N == 4) raw.v[w] = __float_as_uint(p.v[w]);
-      else raw.v[w] = to_bits(static_cast<T>(p.v[2 * w])) | to_bits(static_cast<T>(p.v[2 * w + 1])) << 16;
-    }
-    *reinterpret_cast<Raw16 *>(row + c) = raw;
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (c + e < cols) row[c + e] = static_cast<T>(p.v[e]);
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (N == 4) raw.v[w] = __float_as_uint(p.v[w]);
+    else raw.v[w] = to_bits(static_cast<T>(p.v[2 * w])) | to_bits(static_cast<T>(p.v[2 * w + 1])) << 16;
   }
+  *reinterpret_cast<Raw16 *>(row + (int64_t)i * N) = raw;
+}
+template <typename T>
+__device__ __forceinline__ void store_last(T *__restrict__ row, int i, int left, const Piece<T> &p) {
+#pragma unroll
+  for (int e = 0; e < Piece<T>::N - 1; ++e)
+    if (e < left) row[(int64_t)i * Piece<T>::N + e] = static_cast<T>(p.v[e]);
 }
 
 // Columns whose byte in `seen` (a row of the mask, any alignment) is 0 become -inf.
 template <typename T>
-__device__ __forceinline__ void mask_raw(Raw16 &p, const uint8_t *__restrict__ seen, int64_t i, int64_t cols) {
+__device__ __forceinline__ void mask_whole(Raw16 &p, const uint8_t *__restrict__ seen, int i) {
   constexpr int N = Piece<T>::N;
   struct __attribute__((packed)) Bytes {
     uint32_t w[N / 4];
   };
-  const int64_t c = i * N;
-  if (c + N <= cols) {
-    const Bytes b = *reinterpret_cast<const Bytes *>(seen + c);
+  const Bytes b = *reinterpret_cast<const Bytes *>(seen + (int64_t)i * N);
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (!((b.w[e / 4] >> (8 * (e & 3))) & 0xffu)) erase<T>(p, e);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (c + e < cols && !seen[c + e]) erase<T>(p, e);
-  }
+  for (int e = 0; e < N; ++e)
+    if (!((b.w[e / 4] >> (8 * (e & 3))) & 0xffu)) erase<T>(p, e);
 }
+template <typename T>
+__device__ __forceinline__ void mask_last(Raw16 &p, const uint8_t *__restrict__ seen, int i, int left) {
+#pragma unroll
+  for (int e = 0; e < Piece<T>::N - 1; ++e)
+    if (e < left && !seen[(int64_t)i * Piece<T>::N + e]) erase<T>(p, e);
+}
+
+// The hardware's 2^x and log2 (within an ulp or so; 2^x of less than -126 is 0).
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
 
 // x from lane ^ 1, ^ 2 (within 4 lanes), rotated by 4 and 8 within 16, and across the 16- and 32-lane halves: six steps
 // on the vector ALU that leave a whole wave's sum or maximum in every lane.
@@ -133,11 +137,15 @@ __device__ __forceinline__ float dpp(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true));
 }
 template <typename F>
-__device__ __forceinline__ float wave_reduce(float v, F &&f) {
+__device__ __forceinline__ float reduce16(float v, F &&f) {   // over each 16 lanes
   v = f(v, dpp<0xB1>(v));    // quad_perm 1 0 3 2
   v = f(v, dpp<0x4E>(v));    // quad_perm 2 3 0 1
   v = f(v, dpp<0x124>(v));   // row_ror:4
-  v = f(v, dpp<0x128>(v));   // row_ror:8
+  return f(v, dpp<0x128>(v));   // row_ror:8
+}
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float v, F &&f) {
+  v = reduce16(v, f);
   const auto h = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
   v = f(__int_as_float(h[0]), __int_as_float(h[1]));
   const auto w = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
@@ -161,7 +169,7 @@ struct PartSum {
 __device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }   // no inf - inf
 __device__ __forceinline__ PartSum wave_part(PartSum p, float scale) {
   const float top = wave_max(p.top);
-  p.sum = wave_sum(p.sum * exp2f((p.top - base_of(top)) * scale));
+  p.sum = wave_sum(p.sum * exp2_of((p.top - base_of(top)) * scale));
   p.top = top;
   return p;
 }
@@ -169,46 +177,31 @@ __device__ __forceinline__ PartSum wave_part(PartSum p, float scale) {
 // x joins a part
 __device__ __forceinline__ void join(PartSum &p, float x, float scale) {
   const float top = fmaxf(p.top, x), base = base_of(top);
-  p.sum = p.sum * exp2f((p.top - base) * scale) + exp2f((x - base) * scale);
+  p.sum = p.sum * exp2_of((p.top - base) * scale) + exp2_of((x - base) * scale);
   p.top = top;
 }
 
-// C parts over the workgroup, in every thread; `share` holds 2 C * waves floats.  Shares add in wave order.
+// C parts over the workgroup of at most 16 waves, in every thread; `share` holds 2 C * 16 floats.  Parts from c = 1 on
+// come from the first `few` waves alone.  The waves' shares lie in 16 lanes each for the second step.
 template <int C>
-__device__ __forceinline__ void block_part(PartSum (&p)[C], float scale, float *share) {
+__device__ __forceinline__ void block_part(PartSum (&p)[C], float scale, float *share, int few = 16) {
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int c = 0; c < C; ++c) p[c] = wave_part(p[c], scale);
-  const int waves = blockDim.x >> 6;
+  for (int c = 0; c < C; ++c)
+    if (c == 0 || wave < few) p[c] = wave_part(p[c], scale);
   if (waves == 1) return;
+  float2 *all = reinterpret_cast<float2 *>(share);
   if ((threadIdx.x & 63) == 0)
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      share[2 * (c * waves + (threadIdx.x >> 6))] = p[c].top;
-      share[2 * (c * waves + (threadIdx.x >> 6)) + 1] = p[c].sum;
-    }
+    for (int c = 0; c < C; ++c) all[c * 16 + wave] = make_float2(p[c].top, p[c].sum);
   __syncthreads();
+  const int l = threadIdx.x & 15;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const float2 *all = reinterpret_cast<const float2 *>(share) + c * waves;
-    float top = all[0].x;
-    for (int w = 1; w < waves; ++w) top = fmaxf(top, all[w].x);
-    const float base = base_of(top);
-    float sum = 0.0f;
-    for (int w = 0; w < waves; ++w) sum += all[w].y * exp2f((all[w].x - base) * scale);
-    p[c] = {top, sum};
+    const float2 v = l < waves ? all[c * 16 + l] : make_float2(-INFINITY, 0.0f);
+    const float top = reduce16(v.x, [](float a, float b) { return fmaxf(a, b); });
+    p[c] = {top, reduce16(v.y * exp2_of((v.x - base_of(top)) * scale), [](float a, float b) { return a + b; })};
   }
-}
-
-// v over the workgroup, in every thread; `share` holds a float for each wave.
-__device__ __forceinline__ float block_sum(float v, float *share) {
-  v = wave_sum(v);
-  const int waves = blockDim.x >> 6;
-  if (waves == 1) return v;
-  if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = share[0];
-  for (int w = 1; w < waves; ++w) v += share[w];
-  return v;
 }
 
 }  // namespace fly

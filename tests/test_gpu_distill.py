@@ -311,6 +311,19 @@ def test_distill_strides_streams_graph_and_no_rows():
     assert distill_loss(z[:0], none, reduction="none").shape == (0,)
 
 
+@pytest.mark.parametrize("rows,cols,k", [(64, 4168, 32), (9, 4168, 218), (1100, 600, 20), (3, 70000, 100)])
+def test_results_repeat_bit_for_bit(rows, cols, k):
+    """The order in which workgroups and lanes meet in LDS leaves no trace."""
+    from chessfly.distill import distill_loss_and_grad, top_logits
+    z, t = _logits(rows, cols, 1).to(DEV), _logits(rows, cols, 2).to(DEV)
+    first = top_logits(t, k, 2.0)
+    ref = distill_loss_and_grad(z, first, 2.0)
+    for _ in range(5):
+        again = top_logits(t, k, 2.0)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        assert all(torch.equal(a, b) for a, b in zip(ref, distill_loss_and_grad(z, again, 2.0)))
+
+
 def test_offsets_past_32_bits():
     """Rows over 2^31 elements apart."""
     from chessfly.distill import TopLogits, distill_loss_and_grad, top_logits
