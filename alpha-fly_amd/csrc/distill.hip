@@ -106,15 +106,19 @@ struct Row {
 
 // How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
 // threads cover a row with.  From 1,024 rows on (4 for each CU): 8, since what a wave does once per row weighs more than
-// the waves that are left idle.  Up to 1,024 threads; longer rows are read at every pass (kept = 0).
+// the waves that are left idle (16,384 x 4,168 float16 with gradient: 61 us with 8, 82 with 2).  Past 512 threads 1,024
+// of them, as two workgroups of 16 waves fill a CU evenly (bfloat16 with gradient, 2,048 x 50,256: 95 us with 1,024
+// threads, 110 with 832; 4,096 x 32,768: 111 with 1,024, 118 with 512, 133 with 640); longer rows are read at every pass
+// (kept = 0).
 struct RowShape {
   int kept, threads;
 };
 RowShape row_shape(int64_t rows, int64_t cols, size_t elem, int least) {
-  const int64_t pieces = (cols * (int64_t)elem + 15) / 16;
+  const int64_t pieces = (cols * (int64_t)elem + 15) / 16;   // whole ones at most
   for (int kept : {1, 2, 4, 8}) {
     const int64_t threads = std::max<int64_t>(round_up((pieces + kept - 1) / kept, 64), least);
-    if (kept == 8 ? threads <= 1024 : threads <= 512 && rows < 1024) return {kept, (int)threads};
+    if (threads <= 512 && (kept == 8 || rows < 1024)) return {kept, (int)threads};
+    if (kept == 8 && threads <= 1024) return {kept, 1024};
   }
   return {0, 1024};
 }
@@ -169,14 +173,14 @@ __device__ __forceinline__ uint64_t sort_wave(uint64_t v) {
   return v;
 }
 
-// The K largest of the list's `count` candidates in their places, the others to `spare`, each by its rank: the list's own
+// The K largest of the list's `count` candidates (zeros may lie between them) in their places, the others to `spare`, each by its rank: the list's own
 // order is that of the waves and lanes that met its entries, and nothing may depend on it.  Each 64 are sorted by a
 // wave; an entry's rank is its place among them plus, in each of the other 64, the place that a search finds for it.
 template <typename T>
-__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int count, int k, const T *z, float *values, int32_t *index) {
-  const int lane = threadIdx.x & 63, parts = (count + 63) >> 6;
+__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int entries, int count, int k, const T *z, float *values, int32_t *index) {
+  const int lane = threadIdx.x & 63, parts = (entries + 63) >> 6;
   for (int p = threadIdx.x >> 6; p < parts; p += blockDim.x >> 6) {
-    const uint64_t v = sort_wave(p * 64 + lane < count ? list[p * 64 + lane] : 0);
+    const uint64_t v = sort_wave(p * 64 + lane < entries ? list[p * 64 + lane] : 0);
     list[p * 64 + lane] = v;
   }
   __syncthreads();
@@ -192,7 +196,7 @@ __device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, in
         if (other[before + step - 1] > mine) before += step;
       rank += before + (other[before] > mine);   // before <= 63
     }
-    if (mine == 0) continue;   // behind the last candidate
+    if (mine == 0) continue;   // no candidate
     const int32_t col = (int32_t)~(uint32_t)mine;
     const float v = static_cast<float>(z[col]);
     if (rank < k) {
@@ -282,7 +286,8 @@ __global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *_
   const float scale = inv_t * kLog2e;
   const int64_t r = blockIdx.x;
   const T *zr = z + r * ldz;
-  Row<T, NV, RES> row(zr, legal ? legal + r * ldl : nullptr, (int)cols);
+  const uint8_t *seen = legal ? legal + r * ldl : nullptr;
+  Row<T, NV, RES> row(zr, seen, (int)cols);
   const int most = min(waves * kWaveCandidates, kMostCandidates);
   uint64_t *list = lists;
   float2 *found = reinterpret_cast<float2 *>(lists + most);
@@ -291,8 +296,8 @@ __global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *_
 #pragma unroll
     for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, element<T>(p, e));
   });
-  // the c-th largest of the wave's lanes, rounded down to its high 20 bits
-  const int c = (k + waves - 1) / waves;
+  // the c-th largest of the wave's lanes, rounded down to its high 20 bits, over the waves that have pieces
+  const int holders = min(waves, max(1, (row.full + 63) >> 6)), c = (k + holders - 1) / holders;
   const uint32_t key = order_key(top);
   uint32_t bound = 0;
 #pragma unroll
@@ -302,86 +307,105 @@ __global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *_
   }
   if ((tid & 63) == 0) s.wave[tid >> 6] = bound;
   __syncthreads();
-  for (int w = 0; w < waves; ++w) bound = min(bound, s.wave[w]);
-  const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
-  row.forget();
-  // the candidates, into the wave's list
+  bound = s.wave[0];
+  for (int w = 1; w < holders; ++w) bound = min(bound, s.wave[w]);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int mine = 0;
-  row.each_wave([&](int i, const Raw16 &p) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float v = element<T>(p, e);
-      const uint64_t lanes = __ballot(!(v < floor));
-      if (lanes) {
-        if (!(v < floor)) {
-          const int slot = mine + lanes_before(lanes);
-          if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(i * N + e));
-        }
-        mine += __popcll(lanes);
-      }
-    }
-  });
-  __syncthreads();   // every wave has read the others' bounds
-  if ((tid & 63) == 0) s.wave[wave] = mine;
-  __syncthreads();
-  int count = 0, before = 0;
-  bool fits = true;
-  for (int w = 0; w < waves; ++w) {
-    const int n = s.wave[w];
-    fits &= n <= kWaveCandidates;
-    before += w < wave ? n : 0;
-    count += n;
-  }
-  fits &= count <= most;
-  if (fits) {
-    for (int i = tid & 63; i < mine; i += 64) list[before + i] = candidate(found[wave * kWaveCandidates + i].x, __float_as_int(found[wave * kWaveCandidates + i].y));
-    __syncthreads();
-  }
   PartSum part{-INFINITY, 0.0f};
-  if (!fits) {
-    part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, row.seen, (int)cols, k, scale);
-    count = (int)s.count;
-  } else if (tail != nullptr) {
-    // against the bound, which the rest stays below; where a lane's logits are so far below it that their sum would lose
-    // digits, or the bound is past what the scale allows, against the lane's own largest
-    const float shift = -floor * scale;
-    float sum = 0.0f;
+  int count = 0, entries = 0;   // candidates, and the list's entries: those and zeros
+  if (c > 32 && cols <= most) {
+    // a bound by most of the lanes lets most of the row pass: all of it goes to the list
+    int lanes = 0;
+    for (int i0 = 0; i0 < (int)cols; i0 += blockDim.x) {
+      const int i = i0 + tid;
+      const float v = i < cols && (!seen || seen[i]) ? static_cast<float>(zr[i]) : -INFINITY;
+      if (i < most) list[i] = v == -INFINITY ? 0 : candidate(v, i);
+      lanes += __popcll(__ballot(v != -INFINITY));
+    }
+    __syncthreads();   // every wave has read the others' bounds
+    if ((tid & 63) == 0) s.wave[wave] = lanes;
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) count += s.wave[w];
+    entries = (int)cols;
+  } else {
+    const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
     row.forget();
-    row.each([&](int, int, const Raw16 &p) {
+    // the candidates, into the wave's list
+    int mine = 0;
+    row.each_wave([&](int i, const Raw16 &p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float v = element<T>(p, e), x = exp2_of(fmaf(v, scale, shift));
-        sum += v < floor ? x : 0.0f;
+        const float v = element<T>(p, e);
+        const uint64_t lanes = __ballot(!(v < floor));
+        if (lanes) {
+          if (!(v < floor)) {
+            const int slot = mine + lanes_before(lanes);
+            if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(i * N + e));
+          }
+          mine += __popcll(lanes);
+        }
       }
     });
-    part = {floor, sum};
-    if (top != -INFINITY && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
-      float low = -INFINITY;
+    __syncthreads();   // every wave has read the others' bounds
+    if ((tid & 63) == 0) s.wave[wave] = mine;
+    __syncthreads();
+    int before = 0;
+    bool fits = true;
+    for (int w = 0; w < waves; ++w) {
+      const int n = s.wave[w];
+      fits &= n <= kWaveCandidates;
+      before += w < wave ? n : 0;
+      count += n;
+    }
+    fits &= count <= most;
+    if (fits) {
+      for (int i = tid & 63; i < mine; i += 64) list[before + i] = candidate(found[wave * kWaveCandidates + i].x, __float_as_int(found[wave * kWaveCandidates + i].y));
+      __syncthreads();
+    }
+    if (!fits) {
+      part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, seen, (int)cols, k, scale);
+      count = (int)s.count;
+    } else if (tail != nullptr) {
+      // against the bound, which the rest stays below; where a lane's logits are so far below it that their sum would lose
+      // digits, or the bound is past what the scale allows, against the lane's own largest
+      const float shift = -floor * scale;
+      float sum = 0.0f;
       row.forget();
       row.each([&](int, int, const Raw16 &p) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float v = element<T>(p, e);
-          if (v < floor) low = fmaxf(low, v);
-        }
-      });
-      const float base = base_of(low);
-      sum = 0.0f;
-      row.forget();
-      row.each([&](int, int, const Raw16 &p) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float v = element<T>(p, e), x = exp2_of((v - base) * scale);
+          const float v = element<T>(p, e), x = exp2_of(fmaf(v, scale, shift));
           sum += v < floor ? x : 0.0f;
         }
       });
-      part = {low, sum};
-    } else if (top == -INFINITY) {
-      part = {-INFINITY, 0.0f};
+      part = {floor, sum};
+      if (top != -INFINITY && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
+        float low = -INFINITY;
+        row.forget();
+        row.each([&](int, int, const Raw16 &p) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float v = element<T>(p, e);
+            if (v < floor) low = fmaxf(low, v);
+          }
+        });
+        const float base = base_of(low);
+        sum = 0.0f;
+        row.forget();
+        row.each([&](int, int, const Raw16 &p) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float v = element<T>(p, e), x = exp2_of((v - base) * scale);
+            sum += v < floor ? x : 0.0f;
+          }
+        });
+        part = {low, sum};
+      } else if (top == -INFINITY) {
+        part = {-INFINITY, 0.0f};
+      }
     }
+    entries = count;
   }
-  rank_candidates(list, reinterpret_cast<float *>(found), count, k, zr, values + r * k, index + r * k);
+  rank_candidates(list, reinterpret_cast<float *>(found), entries, count, k, zr, values + r * k, index + r * k);
   if (tail == nullptr) return;
   __syncthreads();
   for (int i = tid; i < count - k; i += blockDim.x) join(part, reinterpret_cast<float *>(found)[i], scale);

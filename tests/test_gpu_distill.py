@@ -132,6 +132,14 @@ def test_top_of_ties(cols, k):
     _check_top(falling.flip(1).contiguous(), k)
 
 
+@pytest.mark.parametrize("rows", [3, 1030])
+@pytest.mark.parametrize("cols", [75, 300, 511, 700, 1024, 1500, 2100])
+@pytest.mark.parametrize("k", [60, 256])
+def test_top_of_a_large_part_of_the_row(rows, cols, k):
+    _check_top(_logits(rows, cols, cols), k, 1.0)
+    _check_top(_logits(rows, cols, cols, torch.bfloat16), k, 1.0, _mask(rows, cols, 4, 0.7))
+
+
 @pytest.mark.parametrize("cols", [37, 4168, 70000])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_top_of_odd_values(cols, dtype):
