@@ -65,38 +65,36 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal: to
     values = torch.empty(rows, k, dtype=torch.float32, device=dev)
     index = torch.empty(rows, k, dtype=torch.int32, device=dev)
     rest = torch.empty(rows, dtype=torch.float32, device=dev) if tail else None
-    with _hip.device_of(logits):
-        _hip.check(_hip.load().fly_top_logits(logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
-                                              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, k,
-                                              temperature, values.data_ptr(), index.data_ptr(), _hip.ptr(rest),
-                                              _hip.stream(dev)), "fly_top_logits")
+    _hip.call("fly_top_logits", dev, logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
+              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, k, temperature, values.data_ptr(),
+              index.data_ptr(), _hip.ptr(rest))
     return TopLogits(values, index, rest)
 
 
 def _teacher(teacher, logits: torch.Tensor, what: str) -> TopLogits:
-    teacher = TopLogits(*teacher)
-    rows = logits.shape[0]
-    for name, t, dtype, dims in (("values", teacher.values, torch.float32, 2), ("index", teacher.index, torch.int32, 2),
-                                 ("tail", teacher.tail, torch.float32, 1)):
-        if t is None and name == "tail":
+    values, index, tail = teacher = TopLogits(*teacher)
+    rows, dev = logits.shape[0], logits.device
+    for name, t, dtype, dims in (("values", values, torch.float32, 2), ("index", index, torch.int32, 2),
+                                 ("tail", tail, torch.float32, 1)):
+        if t is None and dims == 1:
             continue
-        if t.dtype != dtype or t.dim() != dims or t.shape[0] != rows or t.device != logits.device:
-            raise RuntimeError(f"{what}: the teacher's {name} must be {dtype} with {rows} rows on {logits.device}, "
+        if t.dtype is not dtype or t.dim() != dims or t.shape[0] != rows or t.device != dev:
+            raise RuntimeError(f"{what}: the teacher's {name} must be {dtype} with {rows} rows on {dev}, "
                                f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if teacher.values.shape != teacher.index.shape or not 1 <= teacher.values.shape[1] <= MOST_LISTED:
+    if values.shape != index.shape or not 1 <= values.shape[1] <= MOST_LISTED:
         raise RuntimeError(f"{what}: the teacher's values and index must be alike, (rows, 1..{MOST_LISTED}), got "
-                           f"{tuple(teacher.values.shape)} and {tuple(teacher.index.shape)}")
+                           f"{tuple(values.shape)} and {tuple(index.shape)}")
+    if values.is_contiguous() and index.is_contiguous() and (tail is None or tail.is_contiguous()):
+        return teacher
     return TopLogits(*(t.contiguous() if t is not None else None for t in teacher))
 
 
-def _run(logits, teacher: TopLogits, temperature, legal, loss, grad, row_scale, grad_scale) -> None:
+def _run(logits, values, index, tail, temperature, legal, loss, grad, row_scale, grad_scale) -> None:
     rows, cols = logits.shape
-    with _hip.device_of(logits):
-        _hip.check(_hip.load().fly_distill(
-            logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols, _hip.ptr(legal),
-            _hip.row_stride(legal) if legal is not None else 0, teacher.values.data_ptr(), teacher.index.data_ptr(),
-            _hip.ptr(teacher.tail), teacher.values.shape[1], temperature, _hip.ptr(loss), _hip.ptr(grad), cols,
-            _hip.ptr(row_scale), grad_scale, _hip.stream(logits.device)), "fly_distill")
+    _hip.call("fly_distill", logits.device, logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
+              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, values.data_ptr(), index.data_ptr(),
+              _hip.ptr(tail), values.shape[1], temperature, _hip.ptr(loss), _hip.ptr(grad), cols, _hip.ptr(row_scale),
+              grad_scale)
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
@@ -105,7 +103,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature:
     """The loss of each row (float32) and, in the same pass, grad_scale * row_scale * dloss/dlogits in the logits' type
     (grad_scale = 1 / rows: the gradient of the mean).  For training loops: `logits.backward(grad)`."""
     what = "distill_loss_and_grad"
-    logits = _logits(logits.detach(), what)
+    logits = _logits(logits, what)
     legal = _legal(legal, logits, what)
     teacher = _teacher(teacher, logits, what)
     rows, cols = logits.shape
@@ -116,7 +114,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature:
         row_scale = row_scale.contiguous()
     loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     grad = torch.empty(rows, cols, dtype=logits.dtype, device=logits.device)
-    _run(logits, teacher, temperature, legal, loss, grad, row_scale, grad_scale)
+    _run(logits, *teacher, temperature, legal, loss, grad, row_scale, grad_scale)
     return loss, grad
 
 
@@ -127,7 +125,7 @@ class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, index, tail, temperature, legal):
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        _run(logits, TopLogits(values, index, tail), temperature, legal, loss, None, None, 1.0)
+        _run(logits, values, index, tail, temperature, legal, loss, None, None, 1.0)
         ctx.save_for_backward(logits, values, index, tail, legal)
         ctx.temperature = temperature
         return loss
@@ -137,7 +135,7 @@ class _DistillLoss(torch.autograd.Function):
     def backward(ctx, up):
         logits, values, index, tail, legal = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _run(logits, TopLogits(values, index, tail), ctx.temperature, legal, None, grad, up.float().contiguous(), 1.0)
+        _run(logits, values, index, tail, ctx.temperature, legal, None, grad, up.float().contiguous(), 1.0)
         return grad, None, None, None, None, None
 
 
@@ -154,5 +152,9 @@ def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 
     logits = _logits(logits, "distill_loss")
     legal = _legal(legal, logits, "distill_loss")
     teacher = _teacher(teacher, logits, "distill_loss")
-    loss = _DistillLoss.apply(logits, *(t.detach() if t is not None else None for t in teacher), temperature, legal)
+    if logits.requires_grad and torch.is_grad_enabled():
+        loss = _DistillLoss.apply(logits, *(t.detach() if t is not None else None for t in teacher), temperature, legal)
+    else:
+        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        _run(logits, *teacher, temperature, legal, loss, None, None, 1.0)
     return loss if reduction == "none" else loss.mean() if reduction == "mean" else loss.sum()

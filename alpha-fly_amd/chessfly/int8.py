@@ -33,10 +33,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, cols = x.shape
     q = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _hip.device_of(x):
-        _hip.check(_hip.load().fly_quantize_rows(x.data_ptr(), FLOATS[x.dtype], _hip.row_stride(x), rows, cols,
-                                                 q.data_ptr(), max(cols, 1), scale.data_ptr(), _hip.stream(x.device)),
-                   "fly_quantize_rows")
+    _hip.call("fly_quantize_rows", x.device, x.data_ptr(), FLOATS[x.dtype], _hip.row_stride(x), rows, cols, q.data_ptr(),
+              max(cols, 1), scale.data_ptr())
     return q, scale
 
 
@@ -57,7 +55,7 @@ class Int8Linear:
         scale = scale.contiguous()
         bias = bias.contiguous() if bias is not None else None
         handle = ctypes.c_void_p()
-        with _hip.device_of(weight):
+        with torch.cuda.device(weight.device):
             _hip.check(_hip.load().fly_int8_create(weight.data_ptr(), _hip.row_stride(weight), scale.data_ptr(),
                                                    _hip.ptr(bias), self.n, self.k, _hip.stream(weight.device),
                                                    ctypes.byref(handle)), "fly_int8_create")
@@ -73,26 +71,25 @@ class Int8Linear:
                  scale: torch.Tensor | None = None) -> torch.Tensor:
         """x (rows, k) float32, float16 or bfloat16; or int8 with the rows' scales.  Returns (rows, channels)."""
         x = _rows(x, "Int8Linear")
-        rows = x.shape[0]
-        if x.shape[1] != self.k or x.device != self.device:
-            raise RuntimeError(f"Int8Linear: x must be (rows, {self.k}) on {self.device}, "
-                               f"got {tuple(x.shape)} on {x.device}")
+        rows, k = x.shape
+        dev = x.device
+        if k != self.k or dev != self.device:
+            raise RuntimeError(f"Int8Linear: x must be (rows, {self.k}) on {self.device}, got {tuple(x.shape)} on {dev}")
         x_type, y_type = _hip.TYPES.get(x.dtype), FLOATS.get(out_dtype)
         if x_type is None or y_type is None:
             raise RuntimeError(f"Int8Linear: x must be float32, float16, bfloat16 or int8 and out_dtype one of the "
                                f"floats, got {x.dtype} and {out_dtype}")
-        if (x.dtype == torch.int8) != (scale is not None):
+        if (x_type == 3) != (scale is not None):
             raise RuntimeError("Int8Linear: int8 rows come with their scales, other rows without")
         if scale is not None:
-            if scale.dtype != torch.float32 or scale.shape != (rows,) or scale.device != x.device:
-                raise RuntimeError(f"Int8Linear: scale must be float32 of shape ({rows},) on {x.device}, "
+            if scale.dtype != torch.float32 or scale.shape != (rows,) or scale.device != dev:
+                raise RuntimeError(f"Int8Linear: scale must be float32 of shape ({rows},) on {dev}, "
                                    f"got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
             scale = scale.contiguous()
-        y = torch.empty(rows, self.n, dtype=out_dtype, device=x.device)
-        lib = _hip.load()
-        ws = _hip.workspace(lib.fly_int8_workspace(self._plan.handle, rows), x.device)
-        with _hip.device_of(x):
-            _hip.check(lib.fly_int8_linear(self._plan.handle, x.data_ptr(), x_type, _hip.row_stride(x), _hip.ptr(scale),
-                                           rows, y.data_ptr(), y_type, self.n, ws.data_ptr(), ws.numel(),
-                                           _hip.stream(x.device)), "fly_int8_linear")
+        y = torch.empty(rows, self.n, dtype=out_dtype, device=dev)
+        handle = self._plan.handle
+        need = _hip.load().fly_int8_workspace(handle, x_type, rows)
+        ws = _hip.workspace(need, dev) if need else None
+        _hip.call("fly_int8_linear", dev, handle, x.data_ptr(), x_type, _hip.row_stride(x), _hip.ptr(scale), rows,
+                  y.data_ptr(), y_type, self.n, _hip.ptr(ws), need)
         return y

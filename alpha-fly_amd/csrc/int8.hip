@@ -8,6 +8,7 @@
 // Both operands lie in blocks of 16 rows x 64 k, in the order in which the matrix cores take them: 1 KB, lane l's 16
 // bytes at 16 l hold row l & 15, k 16 (l >> 4) .. + 15.  A wave loads a block as one contiguous kilobyte, from memory or
 // LDS, without bank conflicts.  Weights are laid out once, in the plan; tokens by the kernel that quantises them.
+#include "device.hpp"
 #include "rows.hpp"
 
 #include <cmath>
@@ -23,7 +24,8 @@ namespace fly {
 namespace {
 
 typedef int int4v __attribute__((ext_vector_type(4)));
-constexpr int64_t kMostK = 1 << 17;
+constexpr int64_t kMostK = 1 << 17;   // sums below 2^31
+constexpr int kFewBlocks = 12;   // blocks of k that a wave of k_int8_few holds
 
 // Where 16-byte piece c (k 16 c .. + 15) of row r lies among the blocks.
 __device__ __forceinline__ int64_t block_piece(int64_t r, int64_t c, int64_t kb) {
@@ -53,7 +55,7 @@ __device__ __forceinline__ float abs_max(float m, float v) {
 struct RowScale {
   float scale, inverse;
 };
-__device__ __forceinline__ RowScale row_scale(float top) {
+__device__ __forceinline__ RowScale row_scale_of(float top) {
   RowScale s;
   if (!(top <= 3.4028234663852886e38f)) {   // an infinity or NaN
     s.scale = __builtin_nanf("");
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ x, int64
     for (int e = 0; e < N; ++e) top = abs_max(top, p.v[e]);
   }
   top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
-  const RowScale s = row_scale(top);
+  const RowScale s = row_scale_of(top);
   if (lane == 0) scale[row] = s.scale;
   const int64_t chunks = PACKED ? 4 * kb : (k + 15) / 16;
   for (int64_t c = lane; c < chunks; c += 64) {
@@ -111,35 +113,302 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ x, int64
   }
 }
 
-// One wave: 16 tokens x 64 channels, fragments straight from the blocks.
-template <typename T>
-__global__ __launch_bounds__(256) void k_int8_gemm(const int4v *__restrict__ w, const int4v *__restrict__ q,
-                                                   const float *__restrict__ row_scale,
-                                                   const float *__restrict__ scale, const float *__restrict__ bias,
-                                                   int64_t rows, int64_t n, int64_t nb, int64_t kb, T *__restrict__ y,
-                                                   int64_t ldy) {
-  const int lane = threadIdx.x & 63;
-  const int64_t nb0 = (blockIdx.x * (int64_t)4 + (threadIdx.x >> 6)) * 4, mb = blockIdx.y;
-  if (nb0 >= nb) return;
-  int4v acc[4] = {};
-  for (int64_t b = 0; b < kb; ++b) {
-    const int4v fq = q[((mb * kb + b) << 6) + lane];
+// Tokens into blocks: a workgroup takes the 16 rows of a block column, a wave each, held in registers from the maximum to
+// the rounding (NP pieces of 16 bytes a lane: k up to 1,024 NP / sizeof(T)); the blocks go through LDS, so that they leave
+// as whole kilobytes.  Rows past the last are zero.
+template <typename T, int NP>
+__global__ __launch_bounds__(1024) void k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int rows, int k, int kb,
+                                                          int4v *__restrict__ out, float *__restrict__ scale) {
+  constexpr int N = Piece<T>::N;
+  extern __shared__ __attribute__((aligned(16))) int8_t lds8[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pitch = kb * 64 + 16;   // 16 rows in distinct banks
+  const int64_t row = blockIdx.x * (int64_t)16 + wave;
+  const T *xr = x + row * ldx;
+  Piece<T> p[NP];
+  float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int4v fw = w[((min(nb0 + j, nb - 1) * kb + b) << 6) + lane];
-      acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw, fq, acc[j], 0, 0, 0);
+  for (int j = 0; j < NP; ++j) {
+    const int i = lane + 64 * j;
+    if (i * N < k && row < rows) p[j] = load_piece(xr, i, k, 0.0f);
+    else
+#pragma unroll
+      for (int e = 0; e < N; ++e) p[j].v[e] = 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < NP; ++j)
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(p[j].v[e]));
+  top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
+  const RowScale s = row_scale_of(top);
+  if (lane == 0 && row < rows) scale[row] = s.scale;
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int i = lane + 64 * j;
+    if (i * N < kb * 64) {
+      uint32_t w[N / 4] = {};
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e / 4] |= quantised(p[j].v[e], s.inverse) << (8 * (e & 3));
+      uint32_t *to = reinterpret_cast<uint32_t *>(lds8 + wave * pitch + i * N);
+#pragma unroll
+      for (int d = 0; d < N / 4; ++d) to[d] = w[d];
     }
   }
-  const int64_t m = 16 * mb + (lane & 15);
-  if (m >= rows) return;
-  const float sm = row_scale[m];
+  __syncthreads();
+  for (int b = wave; b < kb; b += 16)
+    out[((int64_t)blockIdx.x * kb + b) * 64 + lane] =
+        *reinterpret_cast<const int4v *>(lds8 + (lane & 15) * pitch + b * 64 + (lane >> 4) * 16);
+}
+
+// 16 bytes a lane from memory into LDS at `to` + 16 lane, without passing through registers.
+__device__ __forceinline__ void to_lds(const int4v *from, int4v *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+// All but the last N of this wave's loads have landed, and every wave of the workgroup has come this far.
+template <int N>
+__device__ __forceinline__ void landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Workgroup L runs on XCD L mod 8: each XCD gets a contiguous run of tiles, in groups of 8 token tiles whose channel tiles
+// follow one another, so that the tiles it runs together share operands in its L2.
+__device__ __forceinline__ void int8_tile(int tiles, int mt, int nt, int &m, int &n) {
+  const int L = blockIdx.x, xcd = L & 7, slot = L >> 3, per = tiles >> 3, rem = tiles & 7;
+  const int q = xcd * per + min(xcd, rem) + slot, group = q / (8 * nt), first = group * 8, rows = min(mt - first, 8);
+  const int in = q - group * 8 * nt;
+  m = first + in % rows;
+  n = in / rows;
+}
+
+// WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.
+template <typename T, int WN, int WM, int FN, int FM, int S>
+__global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restrict__ w, const int4v *__restrict__ q,
+                                                            const float *__restrict__ row_scale,
+                                                            const float *__restrict__ scale, const float *__restrict__ bias,
+                                                            int rows, int n, int nb, int mb, int kb, int tiles, int mt,
+                                                            int nt, T *__restrict__ y, int64_t ldy) {
+  constexpr int WAVES = WN * WM, BN = WN * FN, BM = WM * FM, LOADS = (BN + BM) / WAVES;
+  static_assert((BN + BM) % WAVES == 0, "every wave loads as many blocks");
+  __shared__ __attribute__((aligned(16))) int4v lds[S][BN + BM][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tm, tn;
+  int8_tile(tiles, mt, nt, tm, tn);
+  const int n0 = tn * BN, m0 = tm * BM, wn = wave % WN, wm = wave / WN;
+  const int4v *src[LOADS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int i = 0; i < LOADS; ++i) {
+    const int b = wave * LOADS + i;   // blocks past the operands' ends load their last one, whose products go nowhere
+    src[i] = (b < BN ? w + (int64_t)min(n0 + b, nb - 1) * kb * 64 : q + (int64_t)min(m0 + b - BN, mb - 1) * kb * 64) + lane;
+  }
+  auto load = [&](int s) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t c = 16 * (nb0 + j) + 4 * (lane >> 4) + r;
-      if (c < n) y[m * ldy + c] = static_cast<T>((float)acc[j][r] * (sm * scale[c]) + bias[c]);
+    for (int i = 0; i < LOADS; ++i) {
+      to_lds(src[i], &lds[s][wave * LOADS + i][0]);
+      src[i] += 64;
     }
+  };
+  int4v acc[FN][FM];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int i = 0; i < FM; ++i) acc[j][i] = int4v{0, 0, 0, 0};
+  struct Operands {
+    int4v w[FN], q[FM];
+  };
+  auto read = [&](Operands &o, int s) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) o.q[i] = lds[s][BN + wm * FM + i][lane];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) o.w[j] = lds[s][wn * FN + j][lane];
+  };
+  const int ahead = min(S - 1, kb);
+  for (int s = 0; s < ahead; ++s) load(s);
+  // Step k multiplies block k from registers while block k + 1 comes out of LDS and block k + S - 1 goes there, in the place
+  // of block k - 1: every wave has multiplied that one when it passes the barrier of step k.
+  auto multiply = [&](const Operands &o) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[j], o.q[i], acc[j][i], 0, 0, 0);
+  };
+  Operands even, odd;
+  int k = 0;
+  if (kb >= S) {
+    landed<(S - 2) * LOADS>();
+    read(even, 0);
+    for (; k + S < kb; k += 2) {   // two steps, without a branch: the reads stay in flight over the products
+      landed<(S - 3) * LOADS>();
+      load((k + S - 1) % S);
+      read(odd, (k + 1) % S);
+      multiply(even);
+      landed<(S - 3) * LOADS>();
+      load((k + S) % S);
+      read(even, (k + 2) % S);
+      multiply(odd);
+    }
+    if (k + S == kb) {
+      landed<(S - 3) * LOADS>();
+      load((k + S - 1) % S);
+      read(odd, (k + 1) % S);
+      multiply(even);
+      even = odd;
+      ++k;
+    }
+    static_for<S - 2>([&](auto j) {   // the last steps, with ever fewer loads behind them
+      landed<(S - 3 - decltype(j)::value) * LOADS>();
+      read(odd, (k + 1) % S);
+      multiply(even);
+      even = odd;
+      ++k;
+    });
+    multiply(even);
+  } else {
+    landed<0>();
+    for (; k < kb; ++k) {
+      read(even, k);
+      multiply(even);
+    }
+  }
+  // Each wave turns its 16 tokens x 16 FN channels at a time over in LDS, so that a token's channels leave side by side: with
+  // every lane storing its own 4, the 16,384-row product into float16 spent 100 us of 237 on 32-byte pieces of rows.
+  constexpr int PITCH = 16 * FN * sizeof(T) + 16, PER = 16 / sizeof(T), LANES = 16 * FN / PER;   // lanes for a token's channels
+  static_assert(WAVES * 16 * PITCH <= sizeof(lds), "the tile's turn fits in the stages");
+  landed<0>();   // every wave has read its last operands
+  char *turn = reinterpret_cast<char *>(lds) + wave * 16 * PITCH;
+  float4 t[FN], b[FN];
+#pragma unroll
+  for (int j = 0; j < FN; ++j) {
+    const int c = 16 * min(n0 + wn * FN + j, nb - 1) + 4 * (lane >> 4);
+    t[j] = *reinterpret_cast<const float4 *>(scale + c);
+    b[j] = *reinterpret_cast<const float4 *>(bias + c);
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int first = 16 * (m0 + wm * FM + i);
+    const float sm = row_scale[min(first + (lane & 15), rows - 1)];
+    struct __attribute__((aligned(4 * sizeof(T)))) Four {
+      T v[4];
+    };
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<Four *>(turn + (lane & 15) * PITCH + (16 * j + 4 * (lane >> 4)) * sizeof(T)) =
+          Four{{static_cast<T>((float)acc[j][i][0] * (sm * t[j].x) + b[j].x),
+                static_cast<T>((float)acc[j][i][1] * (sm * t[j].y) + b[j].y),
+                static_cast<T>((float)acc[j][i][2] * (sm * t[j].z) + b[j].z),
+                static_cast<T>((float)acc[j][i][3] * (sm * t[j].w) + b[j].w)}};
+#pragma unroll
+    for (int r = 0; r < 16 * LANES; r += 64) {
+      const int token = (r + lane) / LANES, piece = (r + lane) % LANES, m = first + token;
+      const int c = 16 * (n0 + wn * FN) + piece * PER;
+      if (token >= 16 || m >= rows || c >= n) continue;
+      const Raw16 v = *reinterpret_cast<const Raw16 *>(turn + token * PITCH + piece * 16);
+      T *out = y + m * ldy + c;
+      if (c + PER <= n) *reinterpret_cast<Raw16 *>(out) = v;
+      else
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (c + e < n) out[e] = __builtin_bit_cast(T, (std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>)(v.v[e * sizeof(T) / 4] >> (8 * (e * sizeof(T) % 4))));
+    }
+  }
+}
+
+template <typename T, int WN, int WM, int FN, int FM, int S>
+void int8_gemm(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy, hipStream_t st) {
+  const int mb = (int)((rows + 15) / 16), mt = (mb + WM * FM - 1) / (WM * FM), nt = (int)((p.nb + WN * FN - 1) / (WN * FN));
+  FLY_REQUIRE((int64_t)mt * nt < INT32_MAX / 16, "product too large");
+  hipLaunchKernelGGL((k_int8_gemm<T, WN, WM, FN, FM, S>), dim3(mt * nt), dim3(64 * WN * WM), 0, st,
+                     reinterpret_cast<const int4v *>(p.w.p), q, row_scale, p.scale.p, p.bias.p, (int)rows, (int)p.n,
+                     (int)p.nb, mb, (int)p.kb, mt * nt, mt, nt, y, ldy);
+  check_launch("8-bit product");
+}
+
+// Few rows: a workgroup has 16 channels and its 4 waves every fourth block of k, whose weights go straight from memory to
+// the matrix cores; the waves' integer sums meet in LDS.  The work is the weights' way here, so their loads go first.
+// X = void: the rows come quantised from the workspace.  Else every workgroup quantises them for itself, a wave per row,
+// while its weights are on their way: one launch, and no workspace.
+template <typename X, typename T>
+__global__ __launch_bounds__(256) void k_int8_few(const int4v *__restrict__ w, const void *__restrict__ in, int64_t ldx,
+                                                  const float *__restrict__ row_scale, const float *__restrict__ scale,
+                                                  const float *__restrict__ bias, int rows, int n, int k, int kb,
+                                                  T *__restrict__ y, int64_t ldy) {
+  constexpr bool kQuantise = !std::is_void_v<X>;
+  extern __shared__ int4v blocks[];   // the quantised rows, kb blocks
+  __shared__ int4v sums[3][64];
+  __shared__ float s_scale[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int4v *wb = w + (int64_t)blockIdx.x * kb * 64 + lane;
+  int4v fw[kFewBlocks];
+  auto fetch = [&](int b0) {
+#pragma unroll
+    for (int j = 0; j < kFewBlocks; ++j)
+      if (b0 + 4 * j < kb) fw[j] = wb[(b0 + 4 * j) * 64];
+  };
+  fetch(wave);
+  if constexpr (kQuantise) {
+    constexpr int N = Piece<X>::N, kPieces = 48 / N;   // of a row, that a lane holds
+    char *bytes = reinterpret_cast<char *>(blocks);
+    for (int row = wave; row < rows; row += 4) {
+      const X *xr = static_cast<const X *>(in) + row * ldx;
+      Piece<X> p[kPieces];
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const int i = lane + 64 * j;
+        if (i * N < k) p[j] = load_piece(xr, i, k, 0.0f);
+        else
+#pragma unroll
+          for (int e = 0; e < N; ++e) p[j].v[e] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(p[j].v[e]));
+      top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
+      const RowScale s = row_scale_of(top);
+      if (lane == 0) s_scale[row] = s.scale;
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const int at = (lane + 64 * j) * N;   // k of the piece's first element
+        if (at < kb * 64) {
+          uint32_t q[N / 4] = {};
+#pragma unroll
+          for (int e = 0; e < N; ++e) q[e / 4] |= quantised(p[j].v[e], s.inverse) << (8 * (e & 3));
+          uint32_t *to = reinterpret_cast<uint32_t *>(bytes + (at >> 6) * 1024 + ((at >> 4) & 3) * 256 + row * 16 + (at & 15));
+#pragma unroll
+          for (int d = 0; d < N / 4; ++d) to[d] = q[d];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  int4v acc = int4v{0, 0, 0, 0};
+  for (int b0 = wave; b0 < kb; b0 += 4 * kFewBlocks) {
+    if (b0 != wave) fetch(b0);
+#pragma unroll
+    for (int j = 0; j < kFewBlocks; ++j)
+      if (b0 + 4 * j < kb) {
+        const int at = (b0 + 4 * j) * 64 + lane;
+        int4v fq;
+        if constexpr (kQuantise) fq = blocks[at];
+        else fq = static_cast<const int4v *>(in)[at];
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fq, acc, 0, 0, 0);
+      }
+  }
+  if (wave) sums[wave - 1][lane] = acc;
+  __syncthreads();
+  const int m = lane & 15, c = 16 * blockIdx.x + 4 * (lane >> 4);
+  if (wave || m >= rows) return;
+#pragma unroll
+  for (int o = 0; o < 3; ++o) acc += sums[o][lane];
+  const float sm = kQuantise ? s_scale[m] : row_scale[m];
+  const float4 t = *reinterpret_cast<const float4 *>(scale + c), b = *reinterpret_cast<const float4 *>(bias + c);
+  const float v[4] = {(float)acc[0] * (sm * t.x) + b.x, (float)acc[1] * (sm * t.y) + b.y,
+                      (float)acc[2] * (sm * t.z) + b.z, (float)acc[3] * (sm * t.w) + b.w};
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (c + r < n) y[m * ldy + c + r] = static_cast<T>(v[r]);
 }
 
 template <typename F>
@@ -160,10 +429,63 @@ void pack(const int8_t *src, int64_t ld, int64_t rows, int64_t k, int64_t kb, vo
   check_launch("8-bit blocks");
 }
 
+// Rows into blocks and their scales: from registers up to 3,072 columns, whose 16 rows also fit LDS (16,384 rows of 2,333
+// float32 41 us against 87 by the kernel that reads them twice and stores 16 bytes at a time).
+template <typename X>
+void quantise_blocks(const fly_int8 &p, const X *x, int64_t ldx, int64_t rows, int4v *out, float *scale, hipStream_t st) {
+  const int64_t per = 1024 / (int64_t)sizeof(X), span = p.kb * 64;   // elements of a wave's 64 pieces, and of a row
+  auto held = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(blocks_for(rows, 16)), dim3(1024), 16 * (size_t)(span + 16), st, x, ldx, (int)rows,
+                       (int)p.k, (int)p.kb, out, scale);
+  };
+  constexpr int kMost = sizeof(X) == 4 ? 12 : 6;
+  if (span <= kMost / 3 * per) held(k_quantize_blocks<X, kMost / 3>);
+  else if (span <= kMost * per) held(k_quantize_blocks<X, kMost>);
+  else
+    hipLaunchKernelGGL((k_quantize<X, true>), dim3(blocks_for(rows, 4)), dim3(256), 0, st, x, ldx, rows, p.k, p.kb,
+                       reinterpret_cast<int8_t *>(out), (int64_t)0, scale);
+  check_launch("quantised rows");
+}
+
 size_t token_bytes(const fly_int8 &p, int64_t rows) { return (size_t)round_up(rows, 16) * p.kb * 64; }
 
 size_t int8_ws(const fly_int8 &p, int64_t rows) {
   return align256(token_bytes(p, rows)) + align256((size_t)rows * sizeof(float));
+}
+
+// Whether a call quantises its rows in the product itself (k_int8_few): up to 8 rows, of at most 3,072 columns (a wave's
+// registers; 48 KB of blocks), and up to 512 workgroups.  Measured, us with and without: 4,168 channels over 2,333: 1 row 6.2 against
+// 9.5 in two launches, 8 rows 8.6 against 10, 16 rows 12.0 against 11.0; 17,937 channels over 838: 1 row 16.4 against 9.9.
+bool quantises_few(const fly_int8 &p, int32_t x_type, int64_t rows) {
+  return x_type != FLY_I8 && rows <= 8 && p.nb <= 512 && p.kb <= 48;
+}
+
+template <typename X, typename T>
+void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_scale, int64_t rows, T *y, int64_t ldy,
+              hipStream_t st) {
+  hipLaunchKernelGGL((k_int8_few<X, T>), dim3((unsigned)p.nb), dim3(256), std::is_void_v<X> ? 0 : (size_t)p.kb * 1024, st,
+                     reinterpret_cast<const int4v *>(p.w.p), x, ldx, row_scale, p.scale.p, p.bias.p, (int)rows, (int)p.n,
+                     (int)p.k, (int)p.kb, y, ldy);
+  check_launch("8-bit product of few rows");
+}
+
+// The product of rows in blocks.  Measured, us of the product:
+// * up to 16 rows, a workgroup for each 16 channels (k_int8_few): 16 rows of 2,333 into 4,168 5.9;
+// * tiles of 64 x 64 while there are at most 512 of them: 384 rows 12.0 against 13.5 (128 x 128), 1,120 rows of 200 into 500
+//   4.2 against 5.4; but 512 rows 14.7 against 13.5;
+// * 256 x 256 from 512 tiles on that fill at least 70% of their rounds of 256 workgroups (one per CU): 16,384 rows 175
+//   against 193 (128 x 128), 16,384 rows of 1,024 into 4,096 94 against 109, 8,192 rows 100 against 107; but 4,096 rows
+//   (53% of two rounds) 65 against 50;
+// * else 128 x 128, two workgroups of 8 waves per CU: 1,120 rows 21 against 33 (256 x 256) and 24 (64 x 64).
+template <typename T>
+void int8_product(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy,
+                  hipStream_t st) {
+  auto tiles = [&](int side) { return ((rows + side - 1) / side) * ((p.n + side - 1) / side); };
+  const int64_t large = tiles(256);
+  if (rows <= 16) int8_few<void, T>(p, q, 0, row_scale, rows, y, ldy, st);
+  else if (tiles(64) <= 512) int8_gemm<T, 2, 2, 2, 2, 6>(p, q, row_scale, rows, y, ldy, st);
+  else if (large >= 512 && large * 100 >= round_up(large, 256) * 70) int8_gemm<T, 4, 4, 4, 4, 4>(p, q, row_scale, rows, y, ldy, st);
+  else int8_gemm<T, 2, 4, 4, 2, 4>(p, q, row_scale, rows, y, ldy, st);
 }
 
 }  // namespace
@@ -217,7 +539,9 @@ extern "C" int fly_int8_destroy(fly_int8 *p) {
   return guard([&] { delete p; });
 }
 
-extern "C" size_t fly_int8_workspace(const fly_int8 *p, int64_t rows) { return p && rows > 0 ? int8_ws(*p, rows) : 0; }
+extern "C" size_t fly_int8_workspace(const fly_int8 *p, int32_t x_type, int64_t rows) {
+  return p && rows > 0 && !quantises_few(*p, x_type, rows) ? int8_ws(*p, rows) : 0;
+}
 
 extern "C" int fly_int8_linear(const fly_int8 *p, const void *x, int32_t x_type, int64_t ldx, const float *x_scale,
                                int64_t rows, void *y, int32_t y_type, int64_t ldy, void *ws, size_t ws_bytes,
@@ -225,31 +549,28 @@ extern "C" int fly_int8_linear(const fly_int8 *p, const void *x, int32_t x_type,
   return guard([&] {
     FLY_REQUIRE(p != nullptr, "the 8-bit plan is null");
     FLY_REQUIRE(current_device() == p->device, "the 8-bit plan lives on another device");
-    FLY_REQUIRE(rows >= 0 && rows < (int64_t)65535 * 16, "rows out of range");
+    FLY_REQUIRE(rows >= 0 && rows < (int64_t)1 << 24, "rows out of range");
+    FLY_REQUIRE(x_type >= FLY_F32 && x_type <= FLY_I8, "x must be float32, float16, bfloat16 or int8");
     FLY_REQUIRE((x_type == FLY_I8) == (x_scale != nullptr), "8-bit rows come with their scales, other rows without");
     if (!rows) return;
     FLY_REQUIRE(x && y && ldx >= p->k && ldy >= p->n, "bad argument");
-    FLY_REQUIRE(ws && ws_bytes >= int8_ws(*p, rows) && aligned(ws, 256), "workspace too small or misaligned");
     hipStream_t st = as_stream(stream);
-    float *made = reinterpret_cast<float *>(static_cast<char *>(ws) + align256(token_bytes(*p, rows)));
-    if (x_type == FLY_I8) {
-      pack(static_cast<const int8_t *>(x), ldx, rows, p->k, p->kb, ws, st);
-    } else {
-      by_float(x_type, "x must be float32, float16, bfloat16 or int8", [&](auto t) {
-        using T = decltype(t);
-        hipLaunchKernelGGL((k_quantize<T, true>), dim3(blocks_for(rows, 4)), dim3(256), 0, st,
-                           static_cast<const T *>(x), ldx, rows, p->k, p->kb, static_cast<int8_t *>(ws), (int64_t)0,
-                           made);
-        check_launch("quantised tokens");
-      });
-    }
-    by_float(y_type, "y must be float32, float16 or bfloat16", [&](auto t) {
-      using T = decltype(t);
-      hipLaunchKernelGGL(k_int8_gemm<T>, dim3(blocks_for(p->nb, 16), blocks_for(rows, 16)), dim3(256), 0, st,
-                         reinterpret_cast<const int4v *>(p->w.p), static_cast<const int4v *>(ws),
-                         x_scale ? x_scale : made, p->scale.p, p->bias.p, rows, p->n, p->nb, p->kb,
-                         static_cast<T *>(y), ldy);
-      check_launch("8-bit product");
+    by_float(y_type, "y must be float32, float16 or bfloat16", [&](auto yt) {
+      using T = decltype(yt);
+      if (quantises_few(*p, x_type, rows)) {
+        by_float(x_type, "", [&](auto xt) {
+          int8_few<decltype(xt), T>(*p, x, ldx, nullptr, rows, static_cast<T *>(y), ldy, st);
+        });
+        return;
+      }
+      FLY_REQUIRE(ws && ws_bytes >= int8_ws(*p, rows) && aligned(ws, 256), "workspace too small or misaligned");
+      float *made = reinterpret_cast<float *>(static_cast<char *>(ws) + align256(token_bytes(*p, rows)));
+      if (x_type == FLY_I8) pack(static_cast<const int8_t *>(x), ldx, rows, p->k, p->kb, ws, st);
+      else
+        by_float(x_type, "", [&](auto xt) {
+          quantise_blocks(*p, static_cast<const decltype(xt) *>(x), ldx, rows, static_cast<int4v *>(ws), made, st);
+        });
+      int8_product<T>(*p, static_cast<const int4v *>(ws), x_scale ? x_scale : made, rows, static_cast<T *>(y), ldy, st);
     });
   });
 }

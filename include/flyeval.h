@@ -477,8 +477,9 @@ int fly_int8_create(const int8_t *w_dev, int64_t ldw, const float *scale_dev, co
 int fly_int8_destroy(fly_int8 *plan);
 /* y (rows, ldy) of y_type = (sum_k q[m, k] w[n, k]) (s[m] scale[n]) + bias[n]: integer sums exact, scaled in float32.
  * x (rows, ldx) float32, float16 or bfloat16 is quantised by rows as fly_quantize_rows does (x_scale NULL); FLY_I8
- * rows are taken as they are, with x_scale (rows).  rows below 2^20 - 16.  y must not overlap x. */
-size_t fly_int8_workspace(const fly_int8 *plan, int64_t rows);
+ * rows are taken as they are, with x_scale (rows).  rows below 2^24.  y must not overlap x.  The workspace, 256-byte
+ * aligned, may be NULL where the query says 0 (few rows). */
+size_t fly_int8_workspace(const fly_int8 *plan, int32_t x_type, int64_t rows);
 int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int64_t ldx, const float *x_scale_dev,
                     int64_t rows, void *y_dev, int32_t y_type, int64_t ldy, void *workspace_dev,
                     size_t workspace_bytes, void *stream);

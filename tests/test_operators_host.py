@@ -42,7 +42,7 @@ def test_int8_create_refuses(lib):
     _refused(call(k=1 << 17, ldw=1 << 17), lib, b"size")
     _refused(call(ldw=7), lib, b"size")
     _refused(call(out=None), lib, b"out")
-    assert lib.fly_int8_workspace(None, 4) == 0
+    assert lib.fly_int8_workspace(None, 0, 4) == 0
     assert lib.fly_int8_linear(None, P, 0, 8, None, 1, P, 0, 8, P, 1 << 20, None) == 1
 
 
