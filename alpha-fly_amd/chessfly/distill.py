@@ -1,5 +1,5 @@
 """Distillation from a teacher's top logits: `top_logits`, `distill_loss`, `distill_loss_and_grad`, over fly_top_logits
-and fly_distill.
+and fly_distill, and `label`, which runs a teacher.
 
 A teacher labels positions once: of each row of its logits the k largest are kept, and the log-sum-exp of the rest, which
 is what a replay buffer has to hold.  A student then learns from that list:
@@ -158,3 +158,14 @@ def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
         _run(logits, *teacher, temperature, legal, loss, None, None, 1.0)
     return loss if reduction == "none" else loss.mean() if reduction == "mean" else loss.sum()
+
+
+@torch.no_grad()
+def label(teacher, x: torch.Tensor, k: int, temperature: float = 1.0,
+          legal: torch.Tensor | None = None) -> tuple[TopLogits, torch.Tensor]:
+    """What a replay buffer keeps of a teacher network (in eval mode; head_dtype int8 does for it) on boards x: its k best
+    legal moves with the rest's log-sum-exp, and its WDL logits."""
+    if teacher.training:
+        raise RuntimeError("label: the teacher must be in eval mode")
+    logits, wdl = teacher(x)
+    return top_logits(logits, k, temperature, legal), wdl

@@ -8,7 +8,7 @@ load_weights): same constructor, parameters, state_dict keys and forward signatu
 mode, autograd off) FlyChessNet.forward runs as one call into libflyeval.so (fly_model_forward): the encoder
 GEMM on the matrix cores, the light-cone recurrence (float16 deviation path when `infer_dtype` is float16,
 float32 otherwise), and the head GEMMs whose operand loader gathers the output neurons and applies the
-eval-mode normaliser in place.  In training it runs the same layers separately, differentiably, with the
+eval-mode normaliser in place.  With `head_dtype` int8 the heads run as 8-bit products instead.  In training it runs the same layers separately, differentiably, with the
 recurrence's sparse products on the device (ConnectomeRNN.forward_io under autograd).
 """
 
@@ -25,6 +25,7 @@ from . import _hip
 from .brain import ConnectomeRNN
 from .connectome import Connectome
 from .encoding import N_BASE, N_FEATURES, N_MOVES, move_squares
+from .int8 import Int8Linear, quantize_rows
 
 READOUT_SUPERCLASSES = ("descending_neuron",)   # plus every efferent neuron (model.py:23)
 
@@ -75,6 +76,10 @@ class FlyChessNet(nn.Module):
         # The reference always evaluates through the light cone; False computes every neuron at every step
         # (the same function, pruning off) for measurement.
         self.light_cone_pruning = True
+        # float32 reads the outputs out in float32 accuracy; int8 holds the policy and WDL maps in 8 bits with a scale
+        # for each move and quantises each position's outputs (chessfly/int8.py): for a network that labels positions
+        # (chessfly/distill.py), whose kept logits need no more than that.  Evaluation only.
+        self.head_dtype = torch.float32
         if cfg.shuffled:
             conn = conn.shuffled()
         self.brain = ConnectomeRNN(conn, bias_init=cfg.bias_init, global_scale=cfg.weight_scale)
@@ -132,6 +137,39 @@ class FlyChessNet(nn.Module):
         self._dense_cache = _hip.Handle(handle, "fly_dense_destroy", key)
         return self._dense_cache
 
+    def _int8_heads(self) -> tuple[Int8Linear, Int8Linear]:
+        """The policy and WDL maps in 8 bits, rebuilt when their weights change.  A move's logit is linear in the
+        outputs, its from- and to-square terms included, so their rows are added before the rounding."""
+        maps = (self.policy, self.policy_from, self.policy_to, self.value)
+        key = tuple((t._version, t.data_ptr()) for m in maps for t in (m.weight, m.bias))
+        cached = getattr(self, "_int8_cache", None)
+        if cached is None or cached[0] != key:
+            self._int8_cache = None
+            add = lambda a, b, c: a + b[self.move_from] + c[self.move_to]
+            with torch.no_grad():
+                policy = Int8Linear.from_float(add(*(m.weight for m in maps[:3])), add(*(m.bias for m in maps[:3])))
+                cached = (key, policy, Int8Linear.from_float(self.value.weight, self.value.bias))
+            self._int8_cache = cached
+        return cached[1], cached[2]
+
+    def _forward_int8_head(self, x: torch.Tensor, plan, dense, half: bool) -> tuple[torch.Tensor, torch.Tensor]:
+        """Encoder and recurrence as in the fused forward (the drive in the state's dtype, as forward_io takes it), then
+        the maps in 8 bits on the normalised outputs, quantised once for both."""
+        lib, dev, batch = _hip.load(), x.device, x.shape[0]
+        policy, value = self._int8_heads()
+        if not batch:
+            return x.new_zeros(0, N_MOVES, dtype=torch.float32), x.new_zeros(0, 3, dtype=torch.float32)
+        u = torch.empty(len(self.in_idx), batch, dtype=torch.float16 if half else torch.float32, device=dev)
+        ws = _hip.workspace(lib.fly_encoder_workspace(dense.handle, batch), dev)
+        _hip.call("fly_encoder", dev, dense.handle, x.data_ptr(), int(x.dtype == torch.float16), _hip.row_stride(x), batch,
+                  float(self.cfg.input_gain), u.data_ptr(), batch, int(half), ws.data_ptr(), ws.numel())
+        r = torch.empty(len(self.out_idx), batch, dtype=torch.float32, device=dev)
+        ws = _hip.workspace(lib.fly_forward_io_workspace(plan.handle, batch), dev)
+        _hip.call("fly_forward_io", dev, plan.handle, u.data_ptr(), batch, batch, r.data_ptr(), batch, ws.data_ptr(),
+                  ws.numel())
+        q, scale = quantize_rows(self.norm(r.T))
+        return policy(q, scale=scale), value(q, scale=scale)
+
     def _forward_layers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The forward as separate differentiable layers (chessfly/model.py:95-105): training, or any call
         with autograd enabled.  Under autograd the recurrence is float32 (its sparse products on the device);
@@ -159,6 +197,8 @@ class FlyChessNet(nn.Module):
         dtype = self.infer_dtype
         if dtype not in (torch.float16, torch.float32):
             raise RuntimeError(f"infer_dtype must be float16 or float32, got {dtype}")
+        if self.head_dtype not in (torch.float32, torch.int8):
+            raise RuntimeError(f"head_dtype must be float32 or int8, got {self.head_dtype}")
         k = N_FEATURES if self.cfg.attack_planes else N_BASE
         if x.dim() != 2 or x.shape[1] < k:
             raise RuntimeError(f"FlyChessNet.forward: x must be (B, >= {k}), got {tuple(x.shape)}")
@@ -172,6 +212,8 @@ class FlyChessNet(nn.Module):
         mode = _hip.MODE_DEVIATION_F16 if dtype == torch.float16 else _hip.MODE_F32
         plan = brain._cone_plan(cone, mode)
         dense = self._dense(k)
+        if self.head_dtype == torch.int8:
+            return self._forward_int8_head(x, plan, dense, mode == _hip.MODE_DEVIATION_F16)
         batch = x.shape[0]
         logits = torch.empty(batch, N_MOVES, dtype=torch.float32, device=x.device)
         wdl = torch.empty(batch, 3, dtype=torch.float32, device=x.device)

@@ -35,15 +35,31 @@ __device__ __forceinline__ int64_t block_piece(int64_t r, int64_t c, int64_t kb)
 // int8 rows into blocks, zero past k and past the rows; one thread per 16-byte piece.
 __global__ __launch_bounds__(256) void k_int8_pack(const int8_t *__restrict__ src, int64_t ld, int64_t rows, int64_t k,
                                                    int64_t kb, int64_t pieces, int4v *__restrict__ out) {
+  struct __attribute__((packed)) Bytes {
+    uint32_t w[4];
+  };
   const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
   if (i >= pieces) return;
   const int64_t r = i / (4 * kb), c = i - r * 4 * kb;
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (r < rows)
+  Bytes p = {};
+  if (r < rows && 16 * c + 16 <= k) {
+    p = *reinterpret_cast<const Bytes *>(src + r * ld + 16 * c);
+  } else if (r < rows) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (16 * c + e < k) w[e / 4] |= (uint32_t)(uint8_t)src[r * ld + 16 * c + e] << (8 * (e & 3));
-  out[block_piece(r, c, kb)] = int4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    for (int e = 0; e < 15; ++e)
+      if (16 * c + e < k) p.w[e / 4] |= (uint32_t)(uint8_t)src[r * ld + 16 * c + e] << (8 * (e & 3));
+  }
+  out[block_piece(r, c, kb)] = int4v{(int)p.w[0], (int)p.w[1], (int)p.w[2], (int)p.w[3]};
+}
+
+// A plan's scales and bias (zero without one), zero past n.
+__global__ __launch_bounds__(256) void k_int8_scales(const float *__restrict__ scale, const float *__restrict__ bias,
+                                                     int64_t n, int64_t padded, float *__restrict__ out_scale,
+                                                     float *__restrict__ out_bias) {
+  const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
+  if (i >= padded) return;
+  out_scale[i] = i < n ? scale[i] : 0.0f;
+  out_bias[i] = bias && i < n ? bias[i] : 0.0f;
 }
 
 // max |v| of a row piece into a running maximum that keeps NaN
@@ -106,8 +122,13 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ x, int64
     }
     if constexpr (PACKED) {
       reinterpret_cast<int4v *>(q)[block_piece(row, c, kb)] = int4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    } else if (16 * c + 16 <= k) {
+      struct __attribute__((packed)) Bytes {
+        uint32_t w[4];
+      };
+      *reinterpret_cast<Bytes *>(q + row * ldq + 16 * c) = Bytes{{w[0], w[1], w[2], w[3]}};
     } else {
-      for (int e = 0; e < 16; ++e)
+      for (int e = 0; e < 15; ++e)
         if (16 * c + e < k) q[row * ldq + 16 * c + e] = (int8_t)(w[e / 4] >> (8 * (e & 3)));
     }
   }
@@ -526,10 +547,9 @@ extern "C" int fly_int8_create(const int8_t *w, int64_t ldw, const float *scale,
     pack(w, ldw, n, k, p->kb, p->w.p, st);
     p->scale.alloc((size_t)p->nb * 16);
     p->bias.alloc((size_t)p->nb * 16);
-    FLY_HIP(hipMemsetAsync(p->scale.p, 0, p->nb * 16 * sizeof(float), st));
-    FLY_HIP(hipMemsetAsync(p->bias.p, 0, p->nb * 16 * sizeof(float), st));
-    FLY_HIP(hipMemcpyAsync(p->scale.p, scale, n * sizeof(float), hipMemcpyDeviceToDevice, st));
-    if (bias) FLY_HIP(hipMemcpyAsync(p->bias.p, bias, n * sizeof(float), hipMemcpyDeviceToDevice, st));
+    hipLaunchKernelGGL(k_int8_scales, dim3(blocks_for(p->nb * 16, 256)), dim3(256), 0, st, scale, bias, n, p->nb * 16,
+                       p->scale.p, p->bias.p);
+    check_launch("8-bit scales");
     FLY_HIP(hipStreamSynchronize(st));
     *out = p.release();
   });
