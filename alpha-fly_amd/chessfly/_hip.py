@@ -160,27 +160,33 @@ TYPES = {**FLOAT_TYPES, torch.int8: 3}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def call(name: str, device: torch.device, *args) -> None:
-    """One asynchronous entry point on the device's current stream, which it takes as its last argument."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        status = getattr(_lib or load(), name)(*args, _raw_stream(index))
+_one_device = None
+
+
+def call(name: str, index: int, *args) -> None:
+    """One asynchronous entry point on the current stream of device `index`, which it takes as its last argument."""
+    global _one_device
+    if _one_device is None:
+        load()
+        _one_device = torch.cuda.device_count() == 1
+    if _one_device or index == torch.cuda.current_device():
+        status = getattr(_lib, name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = getattr(_lib or load(), name)(*args, _raw_stream(index))
+            status = getattr(_lib, name)(*args, _raw_stream(index))
     if status:
         check(status, name)
 
 
-def row_major(t: torch.Tensor) -> torch.Tensor:
-    """A matrix whose rows lie apart, each contiguous: t itself where its strides allow (rows of any length apart)."""
+def row_major(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """A matrix whose rows lie apart, each contiguous, and their distance: t itself where its strides allow."""
     rows, cols = t.shape
-    ok = (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols)
-    return t if ok else t.contiguous()
-
-
-def row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    if t.is_contiguous():
+        return t, cols or 1
+    ld, step = t.stride()
+    if (cols <= 1 or step == 1) and (rows <= 1 or ld >= cols):
+        return t, ld if rows > 1 else cols or 1
+    return t.contiguous(), cols or 1
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -32,7 +32,7 @@ class TopLogits(NamedTuple):
     tail: torch.Tensor | None = None
 
 
-def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
+def _logits(logits: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:
     _hip.require_device(logits, what)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise RuntimeError(f"{what}: logits must be (rows, columns), got {tuple(logits.shape)}")
@@ -41,9 +41,9 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     return _hip.row_major(logits)
 
 
-def _legal(legal: torch.Tensor | None, logits: torch.Tensor, what: str) -> torch.Tensor | None:
+def _legal(legal: torch.Tensor | None, logits: torch.Tensor, what: str) -> tuple[torch.Tensor | None, int]:
     if legal is None:
-        return None
+        return None, 0
     if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or legal.device != logits.device:
         raise RuntimeError(f"{what}: legal must be bool of shape {tuple(logits.shape)} on {logits.device}, "
                            f"got {legal.dtype} {tuple(legal.shape)} on {legal.device}")
@@ -55,8 +55,8 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal: to
     """The k (1 to 256) largest logits of each row over the legal columns, the lower column first among equals, and the
     log-sum-exp of the others.  Rows with fewer legal columns (a column at -inf is none) end in values -inf and index -1;
     a tail of nothing is -inf."""
-    logits = _logits(logits, "top_logits")
-    legal = _legal(legal, logits, "top_logits")
+    logits, ld = _logits(logits, "top_logits")
+    legal, ld_legal = _legal(legal, logits, "top_logits")
     rows, cols = logits.shape
     dev = logits.device
     k = int(k)
@@ -65,22 +65,20 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal: to
     values = torch.empty(rows, k, dtype=torch.float32, device=dev)
     index = torch.empty(rows, k, dtype=torch.int32, device=dev)
     rest = torch.empty(rows, dtype=torch.float32, device=dev) if tail else None
-    _hip.call("fly_top_logits", dev, logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
-              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, k, temperature, values.data_ptr(),
-              index.data_ptr(), _hip.ptr(rest))
+    _hip.call("fly_top_logits", dev.index, logits.data_ptr(), FLOATS[logits.dtype], ld, rows, cols, _hip.ptr(legal),
+              ld_legal, k, temperature, values.data_ptr(), index.data_ptr(), _hip.ptr(rest))
     return TopLogits(values, index, rest)
 
 
 def _teacher(teacher, logits: torch.Tensor, what: str) -> TopLogits:
-    values, index, tail = teacher = TopLogits(*teacher)
+    values, index, tail = teacher = teacher if type(teacher) is TopLogits else TopLogits(*teacher)
     rows, dev = logits.shape[0], logits.device
-    for name, t, dtype, dims in (("values", values, torch.float32, 2), ("index", index, torch.int32, 2),
-                                 ("tail", tail, torch.float32, 1)):
-        if t is None and dims == 1:
-            continue
-        if t.dtype is not dtype or t.dim() != dims or t.shape[0] != rows or t.device != dev:
-            raise RuntimeError(f"{what}: the teacher's {name} must be {dtype} with {rows} rows on {dev}, "
-                               f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if not (values.dtype is torch.float32 and index.dtype is torch.int32 and values.dim() == 2 and values.shape[0] == rows
+            and values.device == dev and index.device == dev
+            and (tail is None or (tail.dtype is torch.float32 and tail.shape == (rows,) and tail.device == dev))):
+        raise RuntimeError(f"{what}: the teacher's values, index and tail must be float32, int32 and float32 (or None) with "
+                           f"{rows} rows on {dev}, got " + ", ".join(
+                               "None" if t is None else f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in teacher))
     if values.shape != index.shape or not 1 <= values.shape[1] <= MOST_LISTED:
         raise RuntimeError(f"{what}: the teacher's values and index must be alike, (rows, 1..{MOST_LISTED}), got "
                            f"{tuple(values.shape)} and {tuple(index.shape)}")
@@ -89,12 +87,11 @@ def _teacher(teacher, logits: torch.Tensor, what: str) -> TopLogits:
     return TopLogits(*(t.contiguous() if t is not None else None for t in teacher))
 
 
-def _run(logits, values, index, tail, temperature, legal, loss, grad, row_scale, grad_scale) -> None:
+def _run(logits, ld, values, index, tail, temperature, legal, ld_legal, loss, grad, row_scale, grad_scale) -> None:
     rows, cols = logits.shape
-    _hip.call("fly_distill", logits.device, logits.data_ptr(), FLOATS[logits.dtype], _hip.row_stride(logits), rows, cols,
-              _hip.ptr(legal), _hip.row_stride(legal) if legal is not None else 0, values.data_ptr(), index.data_ptr(),
-              _hip.ptr(tail), values.shape[1], temperature, _hip.ptr(loss), _hip.ptr(grad), cols, _hip.ptr(row_scale),
-              grad_scale)
+    _hip.call("fly_distill", logits.device.index, logits.data_ptr(), FLOATS[logits.dtype], ld, rows, cols,
+              _hip.ptr(legal), ld_legal, values.data_ptr(), index.data_ptr(), _hip.ptr(tail), values.shape[1], temperature,
+              _hip.ptr(loss), _hip.ptr(grad), cols, _hip.ptr(row_scale), grad_scale)
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
@@ -103,8 +100,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature:
     """The loss of each row (float32) and, in the same pass, grad_scale * row_scale * dloss/dlogits in the logits' type
     (grad_scale = 1 / rows: the gradient of the mean).  For training loops: `logits.backward(grad)`."""
     what = "distill_loss_and_grad"
-    logits = _logits(logits, what)
-    legal = _legal(legal, logits, what)
+    logits, ld = _logits(logits, what)
+    legal, ld_legal = _legal(legal, logits, what)
     teacher = _teacher(teacher, logits, what)
     rows, cols = logits.shape
     if row_scale is not None:
@@ -114,7 +111,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature:
         row_scale = row_scale.contiguous()
     loss = torch.empty(rows, dtype=torch.float32, device=logits.device)
     grad = torch.empty(rows, cols, dtype=logits.dtype, device=logits.device)
-    _run(logits, *teacher, temperature, legal, loss, grad, row_scale, grad_scale)
+    _run(logits, ld, *teacher, temperature, legal, ld_legal, loss, grad, row_scale, grad_scale)
     return loss, grad
 
 
@@ -123,11 +120,11 @@ class _DistillLoss(torch.autograd.Function):
     gradients."""
 
     @staticmethod
-    def forward(ctx, logits, values, index, tail, temperature, legal):
+    def forward(ctx, logits, ld, values, index, tail, temperature, legal, ld_legal):
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        _run(logits, values, index, tail, temperature, legal, loss, None, None, 1.0)
+        _run(logits, ld, values, index, tail, temperature, legal, ld_legal, loss, None, None, 1.0)
         ctx.save_for_backward(logits, values, index, tail, legal)
-        ctx.temperature = temperature
+        ctx.rest = ld, temperature, ld_legal
         return loss
 
     @staticmethod
@@ -135,8 +132,9 @@ class _DistillLoss(torch.autograd.Function):
     def backward(ctx, up):
         logits, values, index, tail, legal = ctx.saved_tensors
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _run(logits, values, index, tail, ctx.temperature, legal, None, grad, up.float().contiguous(), 1.0)
-        return grad, None, None, None, None, None
+        ld, temperature, ld_legal = ctx.rest
+        _run(logits, ld, values, index, tail, temperature, legal, ld_legal, None, grad, up.float().contiguous(), 1.0)
+        return (grad,) + (None,) * 7
 
 
 def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
@@ -149,14 +147,15 @@ def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 
     the columns, makes its row NaN."""
     if reduction not in ("mean", "sum", "none"):
         raise RuntimeError(f"distill_loss: reduction must be mean, sum or none, got {reduction!r}")
-    logits = _logits(logits, "distill_loss")
-    legal = _legal(legal, logits, "distill_loss")
+    logits, ld = _logits(logits, "distill_loss")
+    legal, ld_legal = _legal(legal, logits, "distill_loss")
     teacher = _teacher(teacher, logits, "distill_loss")
     if logits.requires_grad and torch.is_grad_enabled():
-        loss = _DistillLoss.apply(logits, *(t.detach() if t is not None else None for t in teacher), temperature, legal)
+        loss = _DistillLoss.apply(logits, ld, *(t.detach() if t is not None else None for t in teacher), temperature, legal,
+                                  ld_legal)
     else:
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        _run(logits, *teacher, temperature, legal, loss, None, None, 1.0)
+        _run(logits, ld, *teacher, temperature, legal, ld_legal, loss, None, None, 1.0)
     return loss if reduction == "none" else loss.mean() if reduction == "mean" else loss.sum()
 
 

@@ -18,7 +18,7 @@ from . import _hip
 FLOATS = _hip.FLOAT_TYPES
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+def _rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:
     _hip.require_device(x, what)
     if x.dim() != 2:
         raise RuntimeError(f"{what}: x must have two dimensions, got {tuple(x.shape)}")
@@ -27,13 +27,13 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x (rows, columns) float32, float16 or bfloat16 -> int8 values (rows, columns) and float32 scales (rows)."""
-    x = _rows(x, "quantize_rows")
+    x, ld = _rows(x, "quantize_rows")
     if x.dtype not in FLOATS:
         raise RuntimeError(f"quantize_rows: x must be float32, float16 or bfloat16, got {x.dtype}")
     rows, cols = x.shape
     q = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _hip.call("fly_quantize_rows", x.device, x.data_ptr(), FLOATS[x.dtype], _hip.row_stride(x), rows, cols, q.data_ptr(),
+    _hip.call("fly_quantize_rows", x.device.index, x.data_ptr(), FLOATS[x.dtype], ld, rows, cols, q.data_ptr(),
               max(cols, 1), scale.data_ptr())
     return q, scale
 
@@ -43,7 +43,7 @@ class Int8Linear:
     keeps no reference to the tensors.  Calls run on the current stream with scratch from torch's allocator."""
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None):
-        weight = _rows(weight, "Int8Linear")
+        weight, ld = _rows(weight, "Int8Linear")
         self.n, self.k = weight.shape
         self.device = weight.device
         if weight.dtype != torch.int8:
@@ -56,9 +56,9 @@ class Int8Linear:
         bias = bias.contiguous() if bias is not None else None
         handle = ctypes.c_void_p()
         with torch.cuda.device(weight.device):
-            _hip.check(_hip.load().fly_int8_create(weight.data_ptr(), _hip.row_stride(weight), scale.data_ptr(),
-                                                   _hip.ptr(bias), self.n, self.k, _hip.stream(weight.device),
-                                                   ctypes.byref(handle)), "fly_int8_create")
+            _hip.check(_hip.load().fly_int8_create(weight.data_ptr(), ld, scale.data_ptr(), _hip.ptr(bias), self.n,
+                                                   self.k, _hip.stream(weight.device), ctypes.byref(handle)),
+                       "fly_int8_create")
         self._plan = _hip.Handle(handle, "fly_int8_destroy")
 
     @classmethod
@@ -70,7 +70,7 @@ class Int8Linear:
     def __call__(self, x: torch.Tensor, out_dtype: torch.dtype = torch.float32,
                  scale: torch.Tensor | None = None) -> torch.Tensor:
         """x (rows, k) float32, float16 or bfloat16; or int8 with the rows' scales.  Returns (rows, channels)."""
-        x = _rows(x, "Int8Linear")
+        x, ld = _rows(x, "Int8Linear")
         rows, k = x.shape
         dev = x.device
         if k != self.k or dev != self.device:
@@ -90,6 +90,6 @@ class Int8Linear:
         handle = self._plan.handle
         need = _hip.load().fly_int8_workspace(handle, x_type, rows)
         ws = _hip.workspace(need, dev) if need else None
-        _hip.call("fly_int8_linear", dev, handle, x.data_ptr(), x_type, _hip.row_stride(x), _hip.ptr(scale), rows,
-                  y.data_ptr(), y_type, self.n, _hip.ptr(ws), need)
+        _hip.call("fly_int8_linear", dev.index, handle, x.data_ptr(), x_type, ld, _hip.ptr(scale), rows, y.data_ptr(),
+                  y_type, self.n, _hip.ptr(ws), need)
         return y

@@ -161,11 +161,12 @@ class FlyChessNet(nn.Module):
             return x.new_zeros(0, N_MOVES, dtype=torch.float32), x.new_zeros(0, 3, dtype=torch.float32)
         u = torch.empty(len(self.in_idx), batch, dtype=torch.float16 if half else torch.float32, device=dev)
         ws = _hip.workspace(lib.fly_encoder_workspace(dense.handle, batch), dev)
-        _hip.call("fly_encoder", dev, dense.handle, x.data_ptr(), int(x.dtype == torch.float16), _hip.row_stride(x), batch,
-                  float(self.cfg.input_gain), u.data_ptr(), batch, int(half), ws.data_ptr(), ws.numel())
+        _hip.call("fly_encoder", dev.index, dense.handle, x.data_ptr(), int(x.dtype == torch.float16),
+                  x.stride(0) if batch > 1 else x.shape[1], batch, float(self.cfg.input_gain), u.data_ptr(), batch,
+                  int(half), ws.data_ptr(), ws.numel())
         r = torch.empty(len(self.out_idx), batch, dtype=torch.float32, device=dev)
         ws = _hip.workspace(lib.fly_forward_io_workspace(plan.handle, batch), dev)
-        _hip.call("fly_forward_io", dev, plan.handle, u.data_ptr(), batch, batch, r.data_ptr(), batch, ws.data_ptr(),
+        _hip.call("fly_forward_io", dev.index, plan.handle, u.data_ptr(), batch, batch, r.data_ptr(), batch, ws.data_ptr(),
                   ws.numel())
         q, scale = quantize_rows(self.norm(r.T))
         return policy(q, scale=scale), value(q, scale=scale)
