@@ -185,10 +185,13 @@ __device__ __forceinline__ void to_lds(const int4v *from, int4v *to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                    (__attribute__((address_space(3))) void *)to, 16, 0, 0);
 }
-// All but the last N of this wave's loads have landed, and every wave of the workgroup has come this far.
-template <int N>
-__device__ __forceinline__ void landed() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+// All but the last N of this wave's loads have landed, and all but the last R of its LDS reads are done.
+template <int N, int R>
+__device__ __forceinline__ void wait_for() {
+  static_assert(N < 64 && R < 16, "the counters' range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(%1)" ::"n"(N), "n"(R) : "memory");
+}
+__device__ __forceinline__ void meet() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -203,6 +206,9 @@ __device__ __forceinline__ void int8_tile(int tiles, int mt, int nt, int &m, int
   n = in / rows;
 }
 
+template <int N>
+using Stages = std::integral_constant<int, N>;
+
 // WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.
 template <typename T, int WN, int WM, int FN, int FM, int S>
 __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restrict__ w, const int4v *__restrict__ q,
@@ -210,8 +216,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
                                                             const float *__restrict__ scale, const float *__restrict__ bias,
                                                             int rows, int n, int nb, int mb, int kb, int tiles, int mt,
                                                             int nt, T *__restrict__ y, int64_t ldy) {
-  constexpr int WAVES = WN * WM, BN = WN * FN, BM = WM * FM, LOADS = (BN + BM) / WAVES;
-  static_assert((BN + BM) % WAVES == 0, "every wave loads as many blocks");
+  constexpr int WAVES = WN * WM, BN = WN * FN, BM = WM * FM;
+  constexpr int LOADS = (BN + BM + WAVES - 1) / WAVES, FEWER = (WAVES - (BN + BM) % WAVES) % WAVES;   // waves with one load less
   __shared__ __attribute__((aligned(16))) int4v lds[S][BN + BM][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
@@ -220,15 +226,30 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
   const int4v *src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    const int b = wave * LOADS + i;   // blocks past the operands' ends load their last one, whose products go nowhere
+    // blocks past the operands' ends load their last one, whose products go nowhere
+    const int b = min(wave + i * WAVES, BN + BM - 1);
     src[i] = (b < BN ? w + (int64_t)min(n0 + b, nb - 1) * kb * 64 : q + (int64_t)min(m0 + b - BN, mb - 1) * kb * 64) + lane;
   }
+  const bool fewer = FEWER > 0 && wave >= WAVES - FEWER;
   auto load = [&](int s) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      to_lds(src[i], &lds[s][wave * LOADS + i][0]);
-      src[i] += 64;
+    for (int i = 0; i < LOADS; ++i)
+      if (i < LOADS - 1 || !fewer) {
+        to_lds(src[i], &lds[s][wave + i * WAVES][0]);
+        src[i] += 64;
+      }
+  };
+  // all but the last `stages` of this wave's stages are in LDS, all but its last block's operands out of it, and every wave
+  // has come this far.  The products need those operands anyway, but nothing else keeps them on this side of the barrier.
+  auto landed = [&](auto stages) {
+    constexpr int n = decltype(stages)::value;
+    if constexpr (FEWER > 0 && n > 0) {
+      if (fewer) wait_for<n * (LOADS - 1), FN + FM>();
+      else wait_for<n * LOADS, FN + FM>();
+    } else {
+      wait_for<n * LOADS, FN + FM>();
     }
+    meet();
   };
   int4v acc[FN][FM];
 #pragma unroll
@@ -247,7 +268,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
   const int ahead = min(S - 1, kb);
   for (int s = 0; s < ahead; ++s) load(s);
   // Step k multiplies block k from registers while block k + 1 comes out of LDS and block k + S - 1 goes there, in the place
-  // of block k - 1: every wave has multiplied that one when it passes the barrier of step k.
+  // of block k - 1: every wave has read that one when it passes the barrier of step k.
   auto multiply = [&](const Operands &o) {
 #pragma unroll
     for (int j = 0; j < FN; ++j)
@@ -257,20 +278,20 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
   Operands even, odd;
   int k = 0;
   if (kb >= S) {
-    landed<(S - 2) * LOADS>();
+    landed(Stages<S - 2>{});
     read(even, 0);
     for (; k + S < kb; k += 2) {   // two steps, without a branch: the reads stay in flight over the products
-      landed<(S - 3) * LOADS>();
+      landed(Stages<S - 3>{});
       load((k + S - 1) % S);
       read(odd, (k + 1) % S);
       multiply(even);
-      landed<(S - 3) * LOADS>();
+      landed(Stages<S - 3>{});
       load((k + S) % S);
       read(even, (k + 2) % S);
       multiply(odd);
     }
     if (k + S == kb) {
-      landed<(S - 3) * LOADS>();
+      landed(Stages<S - 3>{});
       load((k + S - 1) % S);
       read(odd, (k + 1) % S);
       multiply(even);
@@ -278,7 +299,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
       ++k;
     }
     static_for<S - 2>([&](auto j) {   // the last steps, with ever fewer loads behind them
-      landed<(S - 3 - decltype(j)::value) * LOADS>();
+      landed(Stages<S - 3 - decltype(j)::value>{});
       read(odd, (k + 1) % S);
       multiply(even);
       even = odd;
@@ -286,7 +307,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
     });
     multiply(even);
   } else {
-    landed<0>();
+    landed(Stages<0>{});
     for (; k < kb; ++k) {
       read(even, k);
       multiply(even);
@@ -296,7 +317,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
   // every lane storing its own 4, the 16,384-row product into float16 spent 100 us of 237 on 32-byte pieces of rows.
   constexpr int PITCH = 16 * FN * sizeof(T) + 16, PER = 16 / sizeof(T), LANES = 16 * FN / PER;   // lanes for a token's channels
   static_assert(WAVES * 16 * PITCH <= sizeof(lds), "the tile's turn fits in the stages");
-  landed<0>();   // every wave has read its last operands
+  wait_for<0, 0>();
+  meet();   // every wave has read its last operands
   char *turn = reinterpret_cast<char *>(lds) + wave * 16 * PITCH;
   float4 t[FN], b[FN];
 #pragma unroll
@@ -319,6 +341,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
                 static_cast<T>((float)acc[j][i][1] * (sm * t[j].y) + b[j].y),
                 static_cast<T>((float)acc[j][i][2] * (sm * t[j].z) + b[j].z),
                 static_cast<T>((float)acc[j][i][3] * (sm * t[j].w) + b[j].w)}};
+    asm volatile("" ::: "memory");   // other lanes read what this one wrote: a wave's LDS accesses keep their order
 #pragma unroll
     for (int r = 0; r < 16 * LANES; r += 64) {
       const int token = (r + lane) / LANES, piece = (r + lane) % LANES, m = first + token;
@@ -330,8 +353,11 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
       else
 #pragma unroll
         for (int e = 0; e < PER; ++e)
-          if (c + e < n) out[e] = __builtin_bit_cast(T, (std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>)(v.v[e * sizeof(T) / 4] >> (8 * (e * sizeof(T) % 4))));
+          if (c + e < n)
+            out[e] = __builtin_bit_cast(T, (std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>)(
+                                               v.v[e * sizeof(T) / 4] >> (8 * (e * sizeof(T) % 4))));
     }
+    asm volatile("" ::: "memory");
   }
 }
 
@@ -490,23 +516,25 @@ void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_sc
   check_launch("8-bit product of few rows");
 }
 
-// The product of rows in blocks.  Measured, us of the product:
-// * up to 16 rows, a workgroup for each 16 channels (k_int8_few): 16 rows of 2,333 into 4,168 5.9;
+// The product of rows in blocks.  Measured, us of the product (2,333 into 4,168 where nothing else is said):
+// * up to 16 rows, a workgroup for each 16 channels (k_int8_few): 16 rows 5.9;
 // * tiles of 64 x 64 while there are at most 512 of them: 384 rows 12.0 against 13.5 (128 x 128), 1,120 rows of 200 into 500
 //   4.2 against 5.4; but 512 rows 14.7 against 13.5;
-// * 256 x 256 from 512 tiles on that fill at least 70% of their rounds of 256 workgroups (one per CU): 16,384 rows 175
-//   against 193 (128 x 128), 16,384 rows of 1,024 into 4,096 94 against 109, 8,192 rows 100 against 107; but 4,096 rows
-//   (53% of two rounds) 65 against 50;
-// * else 128 x 128, two workgroups of 8 waves per CU: 1,120 rows 21 against 33 (256 x 256) and 24 (64 x 64).
+// * 128 x 128 while there are at most 256, one for each CU: 600 rows 14.0 against 17.6 (192 x 128); but 900 rows 20.2 against
+//   19.2;
+// * else 192 channels x 128 tokens (float32: 1,120 rows 19.4 against 21.2 with 128 x 128, 2,048 rows 28.9 against 31.9) or 128 x
+//   192 (16 bits, so that a wave's share of a token is still 128 bytes: 517 rows of 838 into 17,937 16.6 against 17.6 with
+//   192 x 128, 16,384 rows of 1,024 into 4,096 99 against 108), two workgroups of 8 waves per CU.  256 x 256 in one
+//   workgroup of 16 waves: 16,384 rows 178 against 181, 4,096 rows 65 against 48.
 template <typename T>
 void int8_product(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy,
                   hipStream_t st) {
   auto tiles = [&](int side) { return ((rows + side - 1) / side) * ((p.n + side - 1) / side); };
-  const int64_t large = tiles(256);
   if (rows <= 16) int8_few<void, T>(p, q, 0, row_scale, rows, y, ldy, st);
   else if (tiles(64) <= 512) int8_gemm<T, 2, 2, 2, 2, 6>(p, q, row_scale, rows, y, ldy, st);
-  else if (large >= 512 && large * 100 >= round_up(large, 256) * 70) int8_gemm<T, 4, 4, 4, 4, 4>(p, q, row_scale, rows, y, ldy, st);
-  else int8_gemm<T, 2, 4, 4, 2, 4>(p, q, row_scale, rows, y, ldy, st);
+  else if (tiles(128) <= 256) int8_gemm<T, 2, 4, 4, 2, 4>(p, q, row_scale, rows, y, ldy, st);
+  else if constexpr (sizeof(T) == 4) int8_gemm<T, 4, 2, 3, 4, 4>(p, q, row_scale, rows, y, ldy, st);
+  else int8_gemm<T, 2, 4, 4, 3, 4>(p, q, row_scale, rows, y, ldy, st);
 }
 
 }  // namespace
