@@ -329,15 +329,19 @@ __global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *_
   } else {
     const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
     row.forget();
-    // the candidates, into the wave's list
+    // The candidates go into the wave's list; the rest adds up for the tail, against the bound, which it stays below.
+    const float shift = -floor * scale;
+    float sum = 0.0f;
     int mine = 0;
     row.each_wave([&](int i, const Raw16 &p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const float v = element<T>(p, e);
-        const uint64_t lanes = __ballot(!(v < floor));
+        const bool rest = v < floor;
+        const uint64_t lanes = __ballot(!rest);
+        if (tail != nullptr) sum += rest ? exp2_of(fmaf(v, scale, shift)) : 0.0f;
         if (lanes) {
-          if (!(v < floor)) {
+          if (!rest) {
             const int slot = mine + lanes_before(lanes);
             if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(i * N + e));
           }
@@ -365,19 +369,9 @@ __global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *_
       part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, seen, (int)cols, k, scale);
       count = (int)s.count;
     } else if (tail != nullptr) {
-      // against the bound, which the rest stays below; where a lane's logits are so far below it that their sum would lose
-      // digits, or the bound is past what the scale allows, against the lane's own largest
-      const float shift = -floor * scale;
-      float sum = 0.0f;
-      row.forget();
-      row.each([&](int, int, const Raw16 &p) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float v = element<T>(p, e), x = exp2_of(fmaf(v, scale, shift));
-          sum += v < floor ? x : 0.0f;
-        }
-      });
       part = {floor, sum};
+      // Where a lane's logits are so far below the bound that their sum would lose digits, or the bound is past what the
+      // scale allows, against the lane's own largest.
       if (top != -INFINITY && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
         float low = -INFINITY;
         row.forget();
@@ -612,9 +606,11 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
   }
   if (!a.grad) return;
   T *gr = a.grad + r * a.ldg;
+  // A row past the registers reads its logits again here: its gradients go around the caches, which so still hold them
+  // (2,048 x 70,000 bfloat16 140 us against 155).  Rows in registers gain nothing (16,384 x 4,168 float16 65 against 61).
   auto store = [&](int j, int i, const Piece<T> &g) {
     if (j < 0) store_last(gr, i, row.left, g);
-    else store_whole(gr, i, g);
+    else store_whole<T, !RES>(gr, i, g);
   };
   if (s_nothing && factor == factor) {
     row.each([&](int j, int i, const Raw16 &) {

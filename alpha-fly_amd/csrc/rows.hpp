@@ -89,7 +89,8 @@ __device__ __forceinline__ Piece<T> load_piece(const T *__restrict__ row, int64_
   return p;
 }
 
-template <typename T>
+// PAST: around the caches.
+template <typename T, bool PAST>
 __device__ __forceinline__ void store_whole(T *__restrict__ row, int i, const Piece<T> &p) {
   constexpr int N = Piece<T>::N;
   Raw16 raw;
@@ -98,7 +99,11 @@ __device__ __forceinline__ void store_whole(T *__restrict__ row, int i, const Pi
     if constexpr (N == 4) raw.v[w] = __float_as_uint(p.v[w]);
     else raw.v[w] = to_bits(static_cast<T>(p.v[2 * w])) | to_bits(static_cast<T>(p.v[2 * w + 1])) << 16;
   }
-  *reinterpret_cast<Raw16 *>(row + (int64_t)i * N) = raw;
+  typedef uint32_t words __attribute__((ext_vector_type(4), aligned(2)));
+  if constexpr (PAST)
+    __builtin_nontemporal_store(words{raw.v[0], raw.v[1], raw.v[2], raw.v[3]},
+                                reinterpret_cast<words *>(row + (int64_t)i * N));
+  else *reinterpret_cast<Raw16 *>(row + (int64_t)i * N) = raw;
 }
 template <typename T>
 __device__ __forceinline__ void store_last(T *__restrict__ row, int i, int left, const Piece<T> &p) {
