@@ -83,6 +83,23 @@ struct Row {
     }
     if (first == 0 && __builtin_amdgcn_readfirstlane(left)) f(full, last);   // of -inf but in lane 0
   }
+  // f(logit, column)
+  template <typename F>
+  __device__ __forceinline__ void values(F &&f) {
+    each([&](int, int i, const Raw16 &p) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(element<T>(p, e), i * N + e);
+    });
+  }
+  template <typename F>
+  __device__ __forceinline__ void values_wave(F &&f) {
+    each_wave([&](int i, const Raw16 &p) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f(element<T>(p, e), i * N + e);
+    });
+  }
+  // waves that hold whole pieces
+  __device__ __forceinline__ int holders() const { return min((int)blockDim.x >> 6, max(1, (full + 63) >> 6)); }
   // f(j, piece number, piece) for this thread's pieces, columns that do not exist at -inf; j = -1 for the last one where it
   // is not whole (a constant after inlining)
   template <typename F>
@@ -102,6 +119,29 @@ struct Row {
     }
     if (left) f(-1, full, last);
   }
+};
+
+// A short row, column tid + j * blockDim for j < E in a thread's registers: every wave holds as many.
+template <typename T, int E>
+struct Spread {
+  float kept[E];
+  int cols;
+  __device__ __forceinline__ Spread(const T *z, const uint8_t *seen, int n) : cols(n) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int c = threadIdx.x + j * blockDim.x;
+      kept[j] = c < cols && (!seen || seen[c]) ? static_cast<float>(z[c]) : -INFINITY;
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void values(F &&f) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) f(kept[j], threadIdx.x + j * blockDim.x);
+  }
+  template <typename F>
+  __device__ __forceinline__ void values_wave(F &&f) { values(f); }
+  __device__ __forceinline__ int holders() const { return min((int)blockDim.x >> 6, (cols + 63) >> 6); }
+  __device__ __forceinline__ void forget() {}
 };
 
 // How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
@@ -143,16 +183,15 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 
 constexpr int kMostCandidates = 1024, kWaveCandidates = 128;
 
-// What a workgroup of k_top keeps in LDS besides these: 128 entries for each wave of the joined list (at most 1,024), and of
-// the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take later.
+// What a workgroup of k_top keeps in LDS besides these, 128 entries for each wave (at most 1,024 in the first): the joined list,
+// and the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take later.
 struct TopShared {
   alignas(16) float share[2 * 16];
   uint32_t wave[16];
   uint32_t count, prefix, need;
 };
-size_t top_lds(int threads) {
-  const int waves = threads / 64;
-  return 8 * (size_t)(std::min(waves * kWaveCandidates, kMostCandidates) + waves * kWaveCandidates);
+__host__ __device__ inline int top_list(int waves) {
+  return waves * kWaveCandidates < kMostCandidates ? waves * kWaveCandidates : kMostCandidates;
 }
 
 __device__ __forceinline__ uint64_t candidate(float v, int32_t col) {   // larger is better: the key, then the lower column
@@ -173,14 +212,14 @@ __device__ __forceinline__ uint64_t sort_wave(uint64_t v) {
   return v;
 }
 
-// The K largest of the list's `count` candidates (zeros may lie between them) in their places, the others to `spare`, each by its rank: the list's own
+// The K largest of the list's `count` candidates in their places, the others to `spare`, each by its rank: the list's own
 // order is that of the waves and lanes that met its entries, and nothing may depend on it.  Each 64 are sorted by a
 // wave; an entry's rank is its place among them plus, in each of the other 64, the place that a search finds for it.
 template <typename T>
-__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int entries, int count, int k, const T *z, float *values, int32_t *index) {
-  const int lane = threadIdx.x & 63, parts = (entries + 63) >> 6;
+__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int count, int k, const T *z, float *values, int32_t *index) {
+  const int lane = threadIdx.x & 63, parts = (count + 63) >> 6;
   for (int p = threadIdx.x >> 6; p < parts; p += blockDim.x >> 6) {
-    const uint64_t v = sort_wave(p * 64 + lane < entries ? list[p * 64 + lane] : 0);
+    const uint64_t v = sort_wave(p * 64 + lane < count ? list[p * 64 + lane] : 0);
     list[p * 64 + lane] = v;
   }
   __syncthreads();
@@ -196,7 +235,7 @@ __device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, in
         if (other[before + step - 1] > mine) before += step;
       rank += before + (other[before] > mine);   // before <= 63
     }
-    if (mine == 0) continue;   // no candidate
+    if (mine == 0) continue;   // behind the last candidate
     const int32_t col = (int32_t)~(uint32_t)mine;
     const float v = static_cast<float>(z[col]);
     if (rank < k) {
@@ -269,137 +308,109 @@ __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, u
   return part;
 }
 
-// One workgroup per row.  A bound from below: with W waves and c = ceil(K / W), each wave has c lanes whose largest logit
-// is at least the wave's c-th largest of those, so the least of these over the waves has at least K logits at or above
-// it.  Few more than K are (a wave's lanes hold the row interleaved, and it has twice as many lanes as c): each wave
-// packs its own into LDS by ballots, without atomics, and the lists are joined and ranked.  NaN passes every bound.  Lists
-// that would not fit (ties) are left to top_by_digits.
-template <typename T, int NV, bool RES>
-__global__ __launch_bounds__(1024, RES && NV == 8 ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz, int64_t cols,
+// One workgroup per row.  A bound from below: with W waves and c = ceil(K / W), the least over the waves of a logit that each
+// has c at or above has at least K at or above it.  A wave takes the c-th largest of its lanes' largest (it holds the row
+// interleaved, so few more than c logits pass it), or of all its logits (EXACT) where c is most of the lanes.  What passes
+// is packed by ballots, without atomics, into the wave's list in LDS, and the lists are joined and ranked.  NaN passes
+// every bound.  Lists that would not fit (ties) are left to top_by_digits.
+// Bound by the row's bytes where k is small (4,096 x 32,000 bfloat16: k = 8 59 us, k = 64 64 us, 51 us at the rate of a copy),
+// by the instructions per candidate where it is not (k = 256 91 us).
+template <typename T, typename R, bool EXACT>
+__global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz, int64_t cols,
                                               const uint8_t *__restrict__ legal, int64_t ldl, int k, float inv_t,
                                               float *__restrict__ values, int32_t *__restrict__ index,
                                               float *__restrict__ tail) {
-  constexpr int N = Piece<T>::N;
   __shared__ TopShared s;
   extern __shared__ uint64_t lists[];
-  const int tid = threadIdx.x, waves = blockDim.x >> 6;
+  const int tid = threadIdx.x, waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float scale = inv_t * kLog2e;
   const int64_t r = blockIdx.x;
   const T *zr = z + r * ldz;
   const uint8_t *seen = legal ? legal + r * ldl : nullptr;
-  Row<T, NV, RES> row(zr, seen, (int)cols);
-  const int most = min(waves * kWaveCandidates, kMostCandidates);
+  R row(zr, seen, (int)cols);
+  const int holders = row.holders(), c = (k + holders - 1) / holders, most = top_list(waves);
   uint64_t *list = lists;
   float2 *found = reinterpret_cast<float2 *>(lists + most);
   float top = -INFINITY;   // NaN where the lane has one
-  row.each([&](int, int, const Raw16 &p) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, element<T>(p, e));
-  });
-  // the c-th largest of the wave's lanes, rounded down to its high 20 bits, over the waves that have pieces
-  const int holders = min(waves, max(1, (row.full + 63) >> 6)), c = (k + holders - 1) / holders;
+  row.values([&](float v, int) { top = __builtin_elementwise_maximum(top, v); });
+  // the c-th largest, rounded down to its key's high 20 bits
   const uint32_t key = order_key(top);
   uint32_t bound = 0;
 #pragma unroll
   for (int bit = 31; bit >= 12; --bit) {
     const uint32_t next = bound | 1u << bit;
-    if (__popcll(__ballot(key >= next)) >= c) bound = next;
+    int passing = 0;
+    if constexpr (EXACT) {
+      const float x = key_value(next);
+      if (next >= 0x00800000u && next <= 0xff800000u)   // a number or +inf
+        row.values([&](float v, int) { passing += __popcll(__ballot(!(v < x))); });
+    } else {
+      passing = __popcll(__ballot(key >= next));
+    }
+    if (passing >= c) bound = next;
   }
-  if ((tid & 63) == 0) s.wave[tid >> 6] = bound;
+  if ((tid & 63) == 0) s.wave[wave] = bound;
   __syncthreads();
   bound = s.wave[0];
   for (int w = 1; w < holders; ++w) bound = min(bound, s.wave[w]);
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
+  row.forget();
+  // The candidates go into the wave's list; the rest adds up for the tail, against the bound, which it stays below.
   PartSum part{-INFINITY, 0.0f};
-  int count = 0, entries = 0;   // candidates, and the list's entries: those and zeros
-  if (c > 32 && cols <= most) {
-    // a bound by most of the lanes lets most of the row pass: all of it goes to the list
-    int lanes = 0;
-    for (int i0 = 0; i0 < (int)cols; i0 += blockDim.x) {
-      const int i = i0 + tid;
-      const float v = i < cols && (!seen || seen[i]) ? static_cast<float>(zr[i]) : -INFINITY;
-      if (i < most) list[i] = v == -INFINITY ? 0 : candidate(v, i);
-      lanes += __popcll(__ballot(v != -INFINITY));
-    }
-    __syncthreads();   // every wave has read the others' bounds
-    if ((tid & 63) == 0) s.wave[wave] = lanes;
-    __syncthreads();
-    for (int w = 0; w < waves; ++w) count += s.wave[w];
-    entries = (int)cols;
-  } else {
-    const float floor = bound < 0x00800000u ? -kMostFloat : key_value(bound);   // below it: not seen
-    row.forget();
-    // The candidates go into the wave's list; the rest adds up for the tail, against the bound, which it stays below.
-    const float shift = -floor * scale;
-    float sum = 0.0f;
-    int mine = 0;
-    row.each_wave([&](int i, const Raw16 &p) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float v = element<T>(p, e);
-        const bool rest = v < floor;
-        const uint64_t lanes = __ballot(!rest);
-        if (tail != nullptr) sum += rest ? exp2_of(fmaf(v, scale, shift)) : 0.0f;
-        if (lanes) {
-          if (!rest) {
-            const int slot = mine + lanes_before(lanes);
-            if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(i * N + e));
-          }
-          mine += __popcll(lanes);
-        }
+  const float shift = -floor * scale;
+  float sum = 0.0f;
+  int mine = 0;
+  row.values_wave([&](float v, int col) {
+    const bool rest = v < floor;
+    const uint64_t lanes = __ballot(!rest);
+    if (tail != nullptr) sum += rest ? exp2_of(fmaf(v, scale, shift)) : 0.0f;
+    if (lanes) {
+      if (!rest) {
+        const int slot = mine + lanes_before(lanes);
+        if (slot < kWaveCandidates) found[wave * kWaveCandidates + slot] = make_float2(v, __int_as_float(col));
       }
-    });
-    __syncthreads();   // every wave has read the others' bounds
-    if ((tid & 63) == 0) s.wave[wave] = mine;
-    __syncthreads();
-    int before = 0;
-    bool fits = true;
-    for (int w = 0; w < waves; ++w) {
-      const int n = s.wave[w];
-      fits &= n <= kWaveCandidates;
-      before += w < wave ? n : 0;
-      count += n;
+      mine += __popcll(lanes);
     }
-    fits &= count <= most;
-    if (fits) {
-      for (int i = tid & 63; i < mine; i += 64) list[before + i] = candidate(found[wave * kWaveCandidates + i].x, __float_as_int(found[wave * kWaveCandidates + i].y));
-      __syncthreads();
-    }
-    if (!fits) {
-      part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, seen, (int)cols, k, scale);
-      count = (int)s.count;
-    } else if (tail != nullptr) {
-      part = {floor, sum};
-      // Where a lane's logits are so far below the bound that their sum would lose digits, or the bound is past what the
-      // scale allows, against the lane's own largest.
-      if (top != -INFINITY && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
-        float low = -INFINITY;
-        row.forget();
-        row.each([&](int, int, const Raw16 &p) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float v = element<T>(p, e);
-            if (v < floor) low = fmaxf(low, v);
-          }
-        });
-        const float base = base_of(low);
-        sum = 0.0f;
-        row.forget();
-        row.each([&](int, int, const Raw16 &p) {
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float v = element<T>(p, e), x = exp2_of((v - base) * scale);
-            sum += v < floor ? x : 0.0f;
-          }
-        });
-        part = {low, sum};
-      } else if (top == -INFINITY) {
-        part = {-INFINITY, 0.0f};
-      }
-    }
-    entries = count;
+  });
+  __syncthreads();   // every wave has read the others' bounds
+  if ((tid & 63) == 0) s.wave[wave] = mine;
+  __syncthreads();
+  int count = 0, before = 0;
+  bool fits = true;
+  for (int w = 0; w < waves; ++w) {
+    const int n = s.wave[w];
+    fits &= n <= kWaveCandidates;
+    before += w < wave ? n : 0;
+    count += n;
   }
-  rank_candidates(list, reinterpret_cast<float *>(found), entries, count, k, zr, values + r * k, index + r * k);
+  if (fits && count <= most) {
+    for (int i = tid & 63; i < mine; i += 64) {
+      const float2 f = found[wave * kWaveCandidates + i];
+      list[before + i] = candidate(f.x, __float_as_int(f.y));
+    }
+    __syncthreads();
+    part = {floor, sum};
+    if (top == -INFINITY) {
+      part = {-INFINITY, 0.0f};
+    } else if (tail != nullptr && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
+      // the lane's logits are so far below the bound that their sum would lose digits, or the bound is past what the scale
+      // allows: against the lane's own largest
+      float low = -INFINITY;
+      row.forget();
+      row.values([&](float v, int) {
+        if (v < floor) low = fmaxf(low, v);
+      });
+      const float base = base_of(low);
+      sum = 0.0f;
+      row.forget();
+      row.values([&](float v, int) { sum += v < floor ? exp2_of((v - base) * scale) : 0.0f; });
+      part = {low, sum};
+    }
+  } else {
+    part = top_by_digits<T>(s, list, reinterpret_cast<uint32_t *>(found), zr, seen, (int)cols, k, scale);
+    count = (int)s.count;
+  }
+  rank_candidates(list, reinterpret_cast<float *>(found), count, k, zr, values + r * k, index + r * k);
   if (tail == nullptr) return;
   __syncthreads();
   for (int i = tid; i < count - k; i += blockDim.x) join(part, reinterpret_cast<float *>(found)[i], scale);
@@ -694,11 +705,23 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
     by_type(type, [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      by_shape(row_shape(rows, cols, sizeof(T), (int)round_up(2 * k, 64)), [&](auto nv, auto res, int threads) {
-        hipLaunchKernelGGL((k_top<T, decltype(nv)::value, decltype(res)::value>), dim3((unsigned)rows), dim3(threads),
-                           top_lds(threads), as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature,
-                           values, index, tail);
-      });
+      // Twice as many lanes as k (16,384 x 4,168 float16, k = 200: 241 us against 267 with as many; 4,000 x 20,000 80
+      // against 195).  A row too short to give half of them a piece is spread over 4 waves column by column.
+      const int least = (int)round_up(2 * k, 64), full = (int)(cols * (int64_t)sizeof(T) / 16);
+      auto run = [&](auto kernel, int threads) {
+        const int waves = threads / 64;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 8 * (size_t)(top_list(waves) + waves * kWaveCandidates),
+                           as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature, values,
+                           index, tail);
+      };
+      const RowShape shape = row_shape(rows, cols, sizeof(T), least);
+      const int holders = std::min(shape.threads / 64, std::max(1, (full + 63) / 64));
+      if (k > 32 * holders && cols <= 1024) run(k_top<T, Spread<T, 4>, true>, 256);
+      else if (k > 32 * holders && cols <= 4096) run(k_top<T, Spread<T, 16>, true>, 256);
+      else
+        by_shape(shape, [&](auto nv, auto res, int threads) {
+          run(k_top<T, Row<T, decltype(nv)::value, decltype(res)::value>, false>, threads);
+        });
       check_launch("top logits");
     });
   });
