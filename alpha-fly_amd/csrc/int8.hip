@@ -371,32 +371,35 @@ void int8_gemm(const fly_int8 &p, const int4v *q, const float *row_scale, int64_
   check_launch("8-bit product");
 }
 
-// Few rows: a workgroup has 16 channels and its 4 waves every fourth block of k, whose weights go straight from memory to
-// the matrix cores; the waves' integer sums meet in LDS.  The work is the weights' way here, so their loads go first.
-// X = void: the rows come quantised from the workspace.  Else every workgroup quantises them for itself, a wave per row,
-// while its weights are on their way: one launch, and no workspace.
-template <typename X, typename T>
-__global__ __launch_bounds__(256) void k_int8_few(const int4v *__restrict__ w, const void *__restrict__ in, int64_t ldx,
-                                                  const float *__restrict__ row_scale, const float *__restrict__ scale,
-                                                  const float *__restrict__ bias, int rows, int n, int k, int kb,
-                                                  T *__restrict__ y, int64_t ldy) {
+// Few rows, R blocks of 16 of them: a workgroup has C blocks of 16 channels, 4 waves for each, and a wave every fourth block
+// of k, whose weights go straight from memory to the matrix cores; the waves' integer sums meet in LDS.  The work is the
+// weights' way here, so their loads go first.  X = void: the rows come quantised from the workspace.  Else every workgroup
+// quantises them for itself, a wave per row, while its weights are on their way: one launch, and no workspace.  C = 1 up to 8
+// rows, 261 workgroups for 4,168 channels (8 rows of 2,333 8.4 us, C = 4 9.0); C = 4 past that, whose 16 waves share the rows
+// (16 rows 10.5 us against 11.9).
+template <typename X, typename T, int C, int R>
+__global__ __launch_bounds__(256 * C) void k_int8_few(const int4v *__restrict__ w, const void *__restrict__ in, int64_t ldx,
+                                                      const float *__restrict__ row_scale,
+                                                      const float *__restrict__ scale, const float *__restrict__ bias,
+                                                      int rows, int n, int k, int nb, int kb, T *__restrict__ y,
+                                                      int64_t ldy) {
   constexpr bool kQuantise = !std::is_void_v<X>;
-  extern __shared__ int4v blocks[];   // the quantised rows, kb blocks
-  __shared__ int4v sums[3][64];
-  __shared__ float s_scale[16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int4v *wb = w + (int64_t)blockIdx.x * kb * 64 + lane;
+  extern __shared__ int4v blocks[];   // the quantised rows, R x kb blocks
+  __shared__ int4v sums[C][4][R][64];
+  __shared__ float s_scale[16 * R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave & 3, cb = blockIdx.x * C + (wave >> 2);
+  const int4v *wb = w + (int64_t)min(cb, nb - 1) * kb * 64 + lane;
   int4v fw[kFewBlocks];
   auto fetch = [&](int b0) {
 #pragma unroll
     for (int j = 0; j < kFewBlocks; ++j)
       if (b0 + 4 * j < kb) fw[j] = wb[(b0 + 4 * j) * 64];
   };
-  fetch(wave);
+  fetch(part);
   if constexpr (kQuantise) {
     constexpr int N = Piece<X>::N, kPieces = 48 / N;   // of a row, that a lane holds
     char *bytes = reinterpret_cast<char *>(blocks);
-    for (int row = wave; row < rows; row += 4) {
+    for (int row = wave; row < rows; row += 4 * C) {
       const X *xr = static_cast<const X *>(in) + row * ldx;
       Piece<X> p[kPieces];
       float top = 0.0f;
@@ -415,6 +418,7 @@ __global__ __launch_bounds__(256) void k_int8_few(const int4v *__restrict__ w, c
       top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
       const RowScale s = row_scale_of(top);
       if (lane == 0) s_scale[row] = s.scale;
+      char *to_row = bytes + (row >> 4) * kb * 1024 + (row & 15) * 16;
 #pragma unroll
       for (int j = 0; j < kPieces; ++j) {
         const int at = (lane + 64 * j) * N;   // k of the piece's first element
@@ -422,7 +426,7 @@ __global__ __launch_bounds__(256) void k_int8_few(const int4v *__restrict__ w, c
           uint32_t q[N / 4] = {};
 #pragma unroll
           for (int e = 0; e < N; ++e) q[e / 4] |= quantised(p[j].v[e], s.inverse) << (8 * (e & 3));
-          uint32_t *to = reinterpret_cast<uint32_t *>(bytes + (at >> 6) * 1024 + ((at >> 4) & 3) * 256 + row * 16 + (at & 15));
+          uint32_t *to = reinterpret_cast<uint32_t *>(to_row + (at >> 6) * 1024 + ((at >> 4) & 3) * 256 + (at & 15));
 #pragma unroll
           for (int d = 0; d < N / 4; ++d) to[d] = q[d];
         }
@@ -430,29 +434,35 @@ __global__ __launch_bounds__(256) void k_int8_few(const int4v *__restrict__ w, c
     }
     __syncthreads();
   }
-  int4v acc = int4v{0, 0, 0, 0};
-  for (int b0 = wave; b0 < kb; b0 += 4 * kFewBlocks) {
-    if (b0 != wave) fetch(b0);
+  int4v acc[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) acc[i] = int4v{0, 0, 0, 0};
+  for (int b0 = part; b0 < kb; b0 += 4 * kFewBlocks) {
+    if (b0 != part) fetch(b0);
 #pragma unroll
     for (int j = 0; j < kFewBlocks; ++j)
-      if (b0 + 4 * j < kb) {
-        const int at = (b0 + 4 * j) * 64 + lane;
-        int4v fq;
-        if constexpr (kQuantise) fq = blocks[at];
-        else fq = static_cast<const int4v *>(in)[at];
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fq, acc, 0, 0, 0);
-      }
-  }
-  if (wave) sums[wave - 1][lane] = acc;
-  __syncthreads();
-  const int m = lane & 15, c = 16 * blockIdx.x + 4 * (lane >> 4);
-  if (wave || m >= rows) return;
+      if (b0 + 4 * j < kb)
 #pragma unroll
-  for (int o = 0; o < 3; ++o) acc += sums[o][lane];
+        for (int i = 0; i < R; ++i) {
+          const int at = (i * kb + b0 + 4 * j) * 64 + lane;
+          int4v fq;
+          if constexpr (kQuantise) fq = blocks[at];
+          else fq = static_cast<const int4v *>(in)[at];
+          acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[j], fq, acc[i], 0, 0, 0);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) sums[wave >> 2][part][i][lane] = acc[i];
+  __syncthreads();
+  const int m = 16 * part + (lane & 15), c = 16 * cb + 4 * (lane >> 4);   // a wave for each block of rows
+  if (part >= R || cb >= nb || m >= rows) return;
+  int4v sum = sums[wave >> 2][0][part][lane];
+#pragma unroll
+  for (int o = 1; o < 4; ++o) sum += sums[wave >> 2][o][part][lane];
   const float sm = kQuantise ? s_scale[m] : row_scale[m];
   const float4 t = *reinterpret_cast<const float4 *>(scale + c), b = *reinterpret_cast<const float4 *>(bias + c);
-  const float v[4] = {(float)acc[0] * (sm * t.x) + b.x, (float)acc[1] * (sm * t.y) + b.y,
-                      (float)acc[2] * (sm * t.z) + b.z, (float)acc[3] * (sm * t.w) + b.w};
+  const float v[4] = {(float)sum[0] * (sm * t.x) + b.x, (float)sum[1] * (sm * t.y) + b.y,
+                      (float)sum[2] * (sm * t.z) + b.z, (float)sum[3] * (sm * t.w) + b.w};
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (c + r < n) y[m * ldy + c + r] = static_cast<T>(v[r]);
@@ -500,19 +510,24 @@ size_t int8_ws(const fly_int8 &p, int64_t rows) {
   return align256(token_bytes(p, rows)) + align256((size_t)rows * sizeof(float));
 }
 
-// Whether a call quantises its rows in the product itself (k_int8_few): up to 8 rows, of at most 3,072 columns (a wave's
-// registers; 48 KB of blocks), and up to 512 workgroups.  Measured, us with and without: 4,168 channels over 2,333: 1 row 6.2 against
-// 9.5 in two launches, 8 rows 8.6 against 10, 16 rows 12.0 against 11.0; 17,937 channels over 838: 1 row 16.4 against 9.9.
+// Whether a call quantises its rows in the product itself (k_int8_few): up to 32 rows of at most 3,072 columns (a wave's
+// registers; 96 KB of blocks) into at most 8,192 channels, over which every workgroup repeats the work.  Measured, us of the
+// kernels against the two of the other path: 4,168 channels over 2,333: 1 row 6.0 against 9.5, 8 rows 8.4 against 10, 16
+// rows 10.5 against 11.5, 32 rows 13.8 against 13.2; the second launch costs the host another 4.  17,937 channels over 838:
+// 1 row 12.8 against 9.9.
 bool quantises_few(const fly_int8 &p, int32_t x_type, int64_t rows) {
-  return x_type != FLY_I8 && rows <= 8 && p.nb <= 512 && p.kb <= 48;
+  return x_type != FLY_I8 && rows <= 32 && p.nb <= 512 && p.kb <= 48;
 }
 
-template <typename X, typename T>
+template <typename X, typename T, int C, int R>
 void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_scale, int64_t rows, T *y, int64_t ldy,
               hipStream_t st) {
-  hipLaunchKernelGGL((k_int8_few<X, T>), dim3((unsigned)p.nb), dim3(256), std::is_void_v<X> ? 0 : (size_t)p.kb * 1024, st,
-                     reinterpret_cast<const int4v *>(p.w.p), x, ldx, row_scale, p.scale.p, p.bias.p, (int)rows, (int)p.n,
-                     (int)p.k, (int)p.kb, y, ldy);
+  const size_t lds = std::is_void_v<X> ? 0 : (size_t)R * p.kb * 1024;
+  constexpr auto kernel = &k_int8_few<X, T, C, R>;
+  if (lds > 48 * 1024)
+    FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  hipLaunchKernelGGL(kernel, dim3(blocks_for(p.nb, C)), dim3(256 * C), lds, st, reinterpret_cast<const int4v *>(p.w.p), x,
+                     ldx, row_scale, p.scale.p, p.bias.p, (int)rows, (int)p.n, (int)p.k, (int)p.nb, (int)p.kb, y, ldy);
   check_launch("8-bit product of few rows");
 }
 
@@ -530,7 +545,7 @@ template <typename T>
 void int8_product(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy,
                   hipStream_t st) {
   auto tiles = [&](int side) { return ((rows + side - 1) / side) * ((p.n + side - 1) / side); };
-  if (rows <= 16) int8_few<void, T>(p, q, 0, row_scale, rows, y, ldy, st);
+  if (rows <= 16) int8_few<void, T, 1, 1>(p, q, 0, row_scale, rows, y, ldy, st);
   else if (tiles(64) <= 512) int8_gemm<T, 2, 2, 2, 2, 6>(p, q, row_scale, rows, y, ldy, st);
   else if (tiles(128) <= 256) int8_gemm<T, 2, 4, 4, 2, 4>(p, q, row_scale, rows, y, ldy, st);
   else if constexpr (sizeof(T) == 4) int8_gemm<T, 4, 2, 3, 4, 4>(p, q, row_scale, rows, y, ldy, st);
@@ -607,7 +622,11 @@ extern "C" int fly_int8_linear(const fly_int8 *p, const void *x, int32_t x_type,
       using T = decltype(yt);
       if (quantises_few(*p, x_type, rows)) {
         by_float(x_type, "", [&](auto xt) {
-          int8_few<decltype(xt), T>(*p, x, ldx, nullptr, rows, static_cast<T *>(y), ldy, st);
+          using X = decltype(xt);
+          T *out = static_cast<T *>(y);
+          if (rows <= 8) int8_few<X, T, 1, 1>(*p, x, ldx, nullptr, rows, out, ldy, st);
+          else if (rows <= 16) int8_few<X, T, 4, 1>(*p, x, ldx, nullptr, rows, out, ldy, st);
+          else int8_few<X, T, 4, 2>(*p, x, ldx, nullptr, rows, out, ldy, st);
         });
         return;
       }

@@ -86,6 +86,19 @@ def test_product_types(rows, dtype, out):
     _check(y, *O.quantize(x.float().numpy()), w, t / 100, b, out)
 
 
+# Few rows are quantised in the product itself: each count of rows' blocks, a row's length and the channels on both sides
+# of where that ends.
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 31, 32, 33])
+@pytest.mark.parametrize("n,k,dtype", [(70, 3050, torch.float32), (70, 3050, torch.float16), (70, 3090, torch.bfloat16),
+                                       (8190, 100, torch.float16), (8210, 100, torch.float32)])
+def test_few_rows(rows, n, k, dtype):
+    from chessfly.int8 import Int8Linear
+    x = _x(rows, k, rows + 1, dtype)
+    w, t, b = _weight(n, k, rows + n, bias=rows % 2 == 1)
+    y = Int8Linear(w.to(DEV), t.to(DEV), None if b is None else b.to(DEV))(x.to(DEV))
+    _check(y, *O.quantize(x.float().numpy()), w, t, b, torch.float32)
+
+
 @pytest.mark.parametrize("rows,n,k", [(1, 4168, 2333), (21, 4168, 2333), (250, 4168, 2333), (1120, 4168, 2333),
                                       (517, 17937, 838), (2100, 1030, 700)])
 def test_product_at_full_size(rows, n, k):
