@@ -228,7 +228,7 @@ def profile_launches() -> list[tuple[str, float]]:
 
 
 class Handle:
-    """Owner of a library object (cone, plan, dense plan or sweep tables): destroyed with the matching C call."""
+    """Owner of a library object (cone, plan, dense plan, sweep tables or 8-bit plan): destroyed with the matching C call."""
 
     def __init__(self, handle: ctypes.c_void_p, destroy: str, key=None):
         self.handle, self._destroy, self.key = handle, destroy, key

@@ -8,8 +8,9 @@ load_weights): same constructor, parameters, state_dict keys and forward signatu
 mode, autograd off) FlyChessNet.forward runs as one call into libflyeval.so (fly_model_forward): the encoder
 GEMM on the matrix cores, the light-cone recurrence (float16 deviation path when `infer_dtype` is float16,
 float32 otherwise), and the head GEMMs whose operand loader gathers the output neurons and applies the
-eval-mode normaliser in place.  With `head_dtype` int8 the heads run as 8-bit products instead.  In training it runs the same layers separately, differentiably, with the
-recurrence's sparse products on the device (ConnectomeRNN.forward_io under autograd).
+eval-mode normaliser in place.  With `head_dtype` int8 the heads run as 8-bit products instead.  In training
+it runs the same layers separately, differentiably, with the recurrence's sparse products on the device
+(ConnectomeRNN.forward_io under autograd).
 """
 
 from __future__ import annotations

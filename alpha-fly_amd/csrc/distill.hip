@@ -183,8 +183,9 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 
 constexpr int kMostCandidates = 1024, kWaveCandidates = 128;
 
-// What a workgroup of k_top keeps in LDS besides these, 128 entries for each wave (at most 1,024 in the first): the joined list,
-// and the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take later.
+// What a workgroup of k_top keeps in LDS besides these, 128 entries for each wave (at most 1,024 in the first): the joined
+// list, and the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take
+// later.
 struct TopShared {
   alignas(16) float share[2 * 16];
   uint32_t wave[16];
@@ -216,7 +217,8 @@ __device__ __forceinline__ uint64_t sort_wave(uint64_t v) {
 // order is that of the waves and lanes that met its entries, and nothing may depend on it.  Each 64 are sorted by a
 // wave; an entry's rank is its place among them plus, in each of the other 64, the place that a search finds for it.
 template <typename T>
-__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int count, int k, const T *z, float *values, int32_t *index) {
+__device__ __forceinline__ void rank_candidates(uint64_t *list, float *spare, int count, int k, const T *z, float *values,
+                                                int32_t *index) {
   const int lane = threadIdx.x & 63, parts = (count + 63) >> 6;
   for (int p = threadIdx.x >> 6; p < parts; p += blockDim.x >> 6) {
     const uint64_t v = sort_wave(p * 64 + lane < count ? list[p * 64 + lane] : 0);
@@ -258,7 +260,8 @@ __device__ __forceinline__ int lanes_before(uint64_t lanes) {   // of the ballot
 // Where a bound leaves too many candidates (ties): the K-th key a byte at a time, its ties by column order, and the rest's
 // part of the tail.  The list then holds the row's K.  Reads the row again, a column at a time, for each pass.
 template <typename T>
-__device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, uint32_t *hist, const T *z, const uint8_t *seen, int cols, int k, float scale) {
+__device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, uint32_t *hist, const T *z, const uint8_t *seen,
+                                                 int cols, int k, float scale) {
   const int tid = threadIdx.x, wave = tid >> 6, waves = blockDim.x >> 6;
   auto logit = [&](int c) { return c < cols && (!seen || seen[c]) ? static_cast<float>(z[c]) : -INFINITY; };
   uint32_t prefix = 0, need = k;
@@ -316,7 +319,8 @@ __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, u
 // Bound by the row's bytes where k is small (4,096 x 32,000 bfloat16: k = 8 59 us, k = 64 64 us, 51 us at the rate of a copy),
 // by the instructions per candidate where it is not (k = 256 91 us).
 template <typename T, typename R, bool EXACT>
-__global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz, int64_t cols,
+__global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz,
+                                              int64_t cols,
                                               const uint8_t *__restrict__ legal, int64_t ldl, int k, float inv_t,
                                               float *__restrict__ values, int32_t *__restrict__ index,
                                               float *__restrict__ tail) {
@@ -455,7 +459,10 @@ __device__ __forceinline__ float divergence(float logp, float p, float logq, flo
 }
 
 // One workgroup per row.  The first waves hold the list and compute the row's scalars; the others wait for the factor of
-// their exponentials, so what does not depend on the columns is computed once and not by every wave.
+// their exponentials, so what does not depend on the columns is computed once and not by every wave.  Bound by the row's
+// bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 61 us, 4.5 TB/s of the 5.1 that a copy
+// reaches; 2,048 x 50,256 bfloat16 94 us, 4.4 TB/s; x 50,257, whose rows' pieces lie across the lines, 104 us), by a row's
+// chain of load, two reductions, list and store where there are few (256 x 4,168 float32 7.2 us).
 template <typename T, int NV, bool RES>
 __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const DistillArgs<T> a) {
   constexpr int N = Piece<T>::N;
@@ -569,7 +576,8 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
     // the student's normaliser, against its largest logit: log q = (z - mz) / T - ln_z
     const bool has_rest = !part[0].empty();
     const float mz = base_of(fmaxf(part[0].top, part[2].top)), rest_top = base_of(part[0].top);
-    const float ln_z = ln_of(part[0].sum * exp2_of((part[0].top - mz) * scale2) + part[2].sum * exp2_of((part[2].top - mz) * scale2));
+    const float ln_z = ln_of(part[0].sum * exp2_of((part[0].top - mz) * scale2) +
+                             part[2].sum * exp2_of((part[2].top - mz) * scale2));
     const float logqt = has_rest ? (rest_top - mz) * a.inv_t + ln_of(part[0].sum) - ln_z : -INFINITY;
     // the teacher's, its tail a scaled number already: log p = (v - mv) / T + (x - ma) - ln_a
     const float at = a.tail && has_rest ? a.tail[r] : -INFINITY;   // no rest to put it on: the list alone

@@ -136,7 +136,8 @@ __global__ __launch_bounds__(256) void k_quantize(const T *__restrict__ x, int64
 
 // Tokens into blocks: a workgroup takes the 16 rows of a block column, a wave each, held in registers from the maximum to
 // the rounding (NP pieces of 16 bytes a lane: k up to 1,024 NP / sizeof(T)); the blocks go through LDS, so that they leave
-// as whole kilobytes.  Rows past the last are zero.
+// as whole kilobytes.  Rows past the last are zero.  Bound by memory, 16,384 float32 rows of 2,333 41 us (4.7 TB/s in and
+// out); few rows by a row's chain of load, maximum and store (21 rows 5 us).
 template <typename T, int NP>
 __global__ __launch_bounds__(1024) void k_quantize_blocks(const T *__restrict__ x, int64_t ldx, int rows, int k, int kb,
                                                           int4v *__restrict__ out, float *__restrict__ scale) {
@@ -209,7 +210,10 @@ __device__ __forceinline__ void int8_tile(int tiles, int mt, int nt, int &m, int
 template <int N>
 using Stages = std::integral_constant<int, N>;
 
-// WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.
+// WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.  Large
+// products are bound by the matrix cores at the clock that random operands leave them: 16,384 rows of 2,333 into 4,168 run
+// at 1.79e15 operations a second, 178 us, and the main loop alone on a long k at 2.83e15 (3.52e15 with constant operands).
+// Small ones are bound by the tiles' chain of loads, products and stores: 1,120 rows 20 us, where the bytes take 7.6.
 template <typename T, int WN, int WM, int FN, int FM, int S>
 __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restrict__ w, const int4v *__restrict__ q,
                                                             const float *__restrict__ row_scale,
@@ -217,7 +221,8 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
                                                             int rows, int n, int nb, int mb, int kb, int tiles, int mt,
                                                             int nt, T *__restrict__ y, int64_t ldy) {
   constexpr int WAVES = WN * WM, BN = WN * FN, BM = WM * FM;
-  constexpr int LOADS = (BN + BM + WAVES - 1) / WAVES, FEWER = (WAVES - (BN + BM) % WAVES) % WAVES;   // waves with one load less
+  constexpr int LOADS = (BN + BM + WAVES - 1) / WAVES;
+  constexpr int FEWER = (WAVES - (BN + BM) % WAVES) % WAVES;   // waves with one load less
   __shared__ __attribute__((aligned(16))) int4v lds[S][BN + BM][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tm, tn;
@@ -537,9 +542,9 @@ void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_sc
 //   4.2 against 5.4; but 512 rows 14.7 against 13.5;
 // * 128 x 128 while there are at most 256, one for each CU: 600 rows 14.0 against 17.6 (192 x 128); but 900 rows 20.2 against
 //   19.2;
-// * else 192 channels x 128 tokens (float32: 1,120 rows 19.4 against 21.2 with 128 x 128, 2,048 rows 28.9 against 31.9) or 128 x
-//   192 (16 bits, so that a wave's share of a token is still 128 bytes: 517 rows of 838 into 17,937 16.6 against 17.6 with
-//   192 x 128, 16,384 rows of 1,024 into 4,096 99 against 108), two workgroups of 8 waves per CU.  256 x 256 in one
+// * else 192 channels x 128 tokens (float32: 1,120 rows 19.4 against 21.2 with 128 x 128, 2,048 rows 28.9 against 31.9) or
+//   128 x 192 (16 bits, so that a wave's share of a token is still 128 bytes: 517 rows of 838 into 17,937 16.6 against 17.6
+//   with 192 x 128, 16,384 rows of 1,024 into 4,096 99 against 108), two workgroups of 8 waves per CU.  256 x 256 in one
 //   workgroup of 16 waves: 16,384 rows 178 against 181, 4,096 rows 65 against 48.
 template <typename T>
 void int8_product(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy,

@@ -4,9 +4,9 @@
  * Every entry point returns an int status (FLY_OK = 0) and never throws; on failure
  * fly_last_error() returns a message for the calling thread.  Pointers named *_dev are device
  * pointers owned by the caller (torch tensors on the Python side); the library never frees them.
- * The library owns only what its create functions return (cones, plans, dense plans, sweeps) and
- * releases it in the matching destroy (see fly_trim_memory).  `stream` is a hipStream_t passed as void* (torch's current stream); every
- * launch goes on it.  Only the create functions synchronise (they read sizes back to the host);
+ * The library owns only what its create functions return (cones, plans, dense plans, sweeps, 8-bit plans)
+ * and releases it in the matching destroy (see fly_trim_memory).  `stream` is a hipStream_t passed as void*
+ * (torch's current stream); every launch goes on it.  Only the create functions synchronise (they read sizes back to the host);
  * the forward entry points are asynchronous.  Index arrays are int32, the graph is CSR of
  * W[post, pre] (row = postsynaptic neuron).  A created object is immutable apart from the cone's cache of sweep
  * tables and a sweep's tables for one or two positions, which take locks: plans may be created and forwards run from several threads, each with its own
