@@ -259,6 +259,8 @@ __device__ __forceinline__ int lanes_before(uint64_t lanes) {   // of the ballot
 
 // Where a bound leaves too many candidates (ties): the K-th key a byte at a time, its ties by column order, and the rest's
 // part of the tail.  The list then holds the row's K.  Reads the row again, a column at a time, for each pass.
+// Lanes with the first one's byte count together (rows of one value, 16,384 x 4,168 float16: 449 us, 1,168 with an atomic
+// for each lane and one thread searching the bins; 54 us without ties).
 template <typename T>
 __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, uint32_t *hist, const T *z, const uint8_t *seen,
                                                  int cols, int k, float scale) {
@@ -272,15 +274,37 @@ __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, u
     __syncthreads();
     for (int c = tid; c < cols; c += blockDim.x) {
       const uint32_t key = order_key(logit(c));
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1u);
+      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) {
+        const uint32_t digit = (key >> shift) & 255, first = __builtin_amdgcn_readfirstlane(digit);
+        const uint64_t same = __ballot(digit == first);   // of the lanes that are here: most of them where a row ties
+        if (digit != first) atomicAdd(&hist[digit], 1u);
+        else if (lanes_before(same) == 0) atomicAdd(&hist[first], (uint32_t)__popcll(same));
+      }
     }
     __syncthreads();
-    if (tid == 0) {
-      uint32_t left = need;
-      int d = 255;
-      for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-      s.prefix = prefix | (uint32_t)d << shift;
-      s.need = left;
+    if (wave == 0) {   // lane l: bins 255 - 4 l and the three below
+      uint32_t n[4], above = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) above += n[j] = hist[255 - 4 * tid - j];
+      const uint32_t own = above;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(above, d);
+        above += tid >= d ? o : 0;
+      }
+      // the last lane: fewer than K are seen, and the rest are those that are not, in bin 0
+      if (above - own < need && (above >= need || tid == 63)) {
+        uint32_t left = need - (above - own);
+        int d = 255 - 4 * tid;
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (d == 255 - 4 * tid - j && n[j] < left) {
+            left -= n[j];
+            --d;
+          }
+        s.prefix = prefix | (uint32_t)d << shift;
+        s.need = left;
+      }
     }
     __syncthreads();
     prefix = s.prefix;
