@@ -185,6 +185,14 @@ __global__ __launch_bounds__(1024) void k_quantize_blocks(const T *__restrict__ 
         *reinterpret_cast<const int4v *>(lds8 + (lane & 15) * pitch + b * 64 + (lane >> 4) * 16);
 }
 
+// An output in float32, from which it rounds to its type.  The value stands for itself: the compiler would round some kernels'
+// float16 outputs from the exact product and sum instead, and a row's bits would depend on the batch around it.
+__device__ __forceinline__ float scaled(int sum, float scale, float bias) {
+  float v = fmaf((float)sum, scale, bias);
+  asm("" : "+v"(v));
+  return v;
+}
+
 // 16 bytes a lane from memory into LDS at `to` + 16 lane, without passing through registers.
 __device__ __forceinline__ void to_lds(const int4v *from, int4v *to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
@@ -346,10 +354,10 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
 #pragma unroll
     for (int j = 0; j < FN; ++j)
       *reinterpret_cast<Four *>(turn + (lane & 15) * PITCH + (16 * j + 4 * (lane >> 4)) * sizeof(T)) =
-          Four{{static_cast<T>((float)acc[j][i][0] * (sm * t[j].x) + b[j].x),
-                static_cast<T>((float)acc[j][i][1] * (sm * t[j].y) + b[j].y),
-                static_cast<T>((float)acc[j][i][2] * (sm * t[j].z) + b[j].z),
-                static_cast<T>((float)acc[j][i][3] * (sm * t[j].w) + b[j].w)}};
+          Four{{static_cast<T>(scaled(acc[j][i][0], sm * t[j].x, b[j].x)),
+                static_cast<T>(scaled(acc[j][i][1], sm * t[j].y, b[j].y)),
+                static_cast<T>(scaled(acc[j][i][2], sm * t[j].z, b[j].z)),
+                static_cast<T>(scaled(acc[j][i][3], sm * t[j].w, b[j].w))}};
     asm volatile("" ::: "memory");   // other lanes read what this one wrote: a wave's LDS accesses keep their order
 #pragma unroll
     for (int r = 0; r < 16 * LANES; r += 64) {
@@ -470,8 +478,8 @@ __global__ __launch_bounds__(256 * C) void k_int8_few(const int4v *__restrict__ 
   for (int o = 1; o < 4; ++o) sum += sums[wave >> 2][o][part][lane];
   const float sm = kQuantise ? s_scale[m] : row_scale[m];
   const float4 t = *reinterpret_cast<const float4 *>(scale + c), b = *reinterpret_cast<const float4 *>(bias + c);
-  const float v[4] = {(float)sum[0] * (sm * t.x) + b.x, (float)sum[1] * (sm * t.y) + b.y,
-                      (float)sum[2] * (sm * t.z) + b.z, (float)sum[3] * (sm * t.w) + b.w};
+  const float v[4] = {scaled(sum[0], sm * t.x, b.x), scaled(sum[1], sm * t.y, b.y), scaled(sum[2], sm * t.z, b.z),
+                      scaled(sum[3], sm * t.w, b.w)};
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (c + r < n) y[m * ldy + c + r] = static_cast<T>(v[r]);

@@ -159,6 +159,19 @@ def test_top_of_odd_values(cols, dtype):
     _check_top(z, 30, 1.0, _mask(8, cols, 4, 0.5))
 
 
+@pytest.mark.parametrize("cols", [4168, 33000, 70000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_of_visible_columns_side_by_side(cols, dtype):
+    """All that a row shows lies in the columns of one wave: fewer than k, exactly k, and more, on one value and on many."""
+    z = _logits(6, cols, 9, dtype)
+    legal = torch.zeros(6, cols, dtype=torch.bool)
+    for r, n in enumerate([1, 140, 256, 257, 500, 250]):
+        legal[r, 16 * r: 16 * r + n] = True
+    z[2] = z[5] = 0.75
+    for k in (130, 256):
+        _check_top(z, k, 1.0, legal)
+
+
 def test_top_strides_streams_and_no_rows():
     from chessfly.distill import top_logits
     wide = _logits(9, 4300, 7)

@@ -172,6 +172,23 @@ def test_outputs_are_the_same_for_every_batch_around_them():
         assert torch.equal(lin(x[:rows]), whole[:rows]), rows
 
 
+def test_offsets_past_32_bits():
+    """Rows over 2^31 elements apart, and more outputs than that."""
+    from chessfly.int8 import Int8Linear, quantize_rows
+    w, t, b = _weight(17001, 70, 9)
+    lin = Int8Linear(w.to(DEV), t.to(DEV), b.to(DEV))
+    apart, x = 1_150_000_000, _x(3, 70, 3, torch.float16).to(DEV)
+    far = torch.empty(2 * apart + 70, dtype=torch.float16, device=DEV).as_strided((3, 70), (apart, 1))
+    far.copy_(x)
+    assert torch.equal(lin(far), lin(x))
+    assert all(torch.equal(a, b) for a, b in zip(quantize_rows(far), quantize_rows(x)))
+    del far
+    x = torch.randn(130_000, 70, device=DEV)
+    y = lin(x, torch.float16)
+    for part in (slice(0, 9), slice(126_300, 126_340), slice(129_900, 130_000)):
+        assert torch.equal(y[part], lin(x[part], torch.float16))
+
+
 def test_another_stream_and_a_graph():
     from chessfly.int8 import Int8Linear
     x = _x(64, 333, 8).to(DEV)
