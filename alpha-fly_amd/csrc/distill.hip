@@ -411,7 +411,7 @@ __global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top
     before += w < wave ? n : 0;
     count += n;
   }
-  if (fits && count <= most) {
+  if (__builtin_expect(fits && count <= most, 1)) {
     for (int i = tid & 63; i < mine; i += 64) {
       const float2 f = found[wave * kWaveCandidates + i];
       list[before + i] = candidate(f.x, __float_as_int(f.y));
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top
     part = {floor, sum};
     if (top == -INFINITY) {
       part = {-INFINITY, 0.0f};
-    } else if (tail != nullptr && !(sum > 1e-20f && fabsf(shift) < 1e37f)) {
+    } else if (__builtin_expect(tail != nullptr && !(sum > 1e-20f && fabsf(shift) < 1e37f), 0)) {
       // the lane's logits are so far below the bound that their sum would lose digits, or the bound is past what the scale
       // allows: against the lane's own largest
       float low = -INFINITY;
