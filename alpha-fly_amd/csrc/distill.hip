@@ -259,8 +259,8 @@ __device__ __forceinline__ int lanes_before(uint64_t lanes) {   // of the ballot
 
 // Where a bound leaves too many candidates (ties): the K-th key a byte at a time, its ties by column order, and the rest's
 // part of the tail.  The list then holds the row's K.  Reads the row again, a column at a time, for each pass.
-// Lanes with the first one's byte count together (rows of one value, 16,384 x 4,168 float16: 449 us, 1,168 with an atomic
-// for each lane and one thread searching the bins; 54 us without ties).
+// Lanes with the first one's byte count together (rows of one value, 16,384 x 4,168 float16: 456 us, 1,168 with an atomic
+// for each lane and one thread searching the bins; 50 us without ties).
 template <typename T>
 __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, uint32_t *hist, const T *z, const uint8_t *seen,
                                                  int cols, int k, float scale) {
@@ -737,8 +737,8 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
     by_type(type, [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      // Twice as many lanes as k (16,384 x 4,168 float16, k = 200: 241 us against 267 with as many; 4,000 x 20,000 80
-      // against 195).  A row too short to give half of them a piece is spread over 4 waves column by column.
+      // Twice as many lanes as k (16,384 x 4,168 float16, k = 200: 204 us against 214 with as many; 4,000 x 20,000 74
+      // against 181).  A row too short to give half of them a piece is spread over 4 waves column by column.
       const int least = (int)round_up(2 * k, 64), full = (int)(cols * (int64_t)sizeof(T) / 16);
       auto run = [&](auto kernel, int threads) {
         const int waves = threads / 64;
