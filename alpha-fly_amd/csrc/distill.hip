@@ -145,20 +145,25 @@ struct Spread {
 };
 
 // How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
-// threads cover a row with.  From 1,024 rows on (4 for each CU): 8, since what a wave does once per row weighs more than
-// the waves that are left idle (16,384 x 4,168 float16 with gradient: 61 us with 8, 82 with 2).  Past 512 threads 1,024
-// of them, as two workgroups of 16 waves fill a CU evenly (bfloat16 with gradient, 2,048 x 50,256: 95 us with 1,024
-// threads, 110 with 832; 4,096 x 32,768: 111 with 1,024, 118 with 512, 133 with 640); longer rows are read at every pass
-// (kept = 0).
+// threads cover a row with.  From 1,024 rows on (4 for each CU) at least `many`, since what a wave does once per row weighs
+// more than the waves that are left idle: 8 for the top logits (1,500 x 4,168 float32 12.1 us with 8, 14.7 with 4), 4 for
+// the distillation, whose 8 cost it registers (with gradient: 16,384 x 4,168 float16 57 us with 4, 63 with 8, 82 with 2;
+// float32 103, 113 with 8; 16,384 x 1,000 float32 28.7, 35.4 with 8).  Past 512 threads 1,024 of them, as two workgroups of
+// 16 waves fill a CU evenly (8 pieces: 2,048 x 50,256 95 us, with the 832 threads that it needs 110).  For many rows that is
+// where `many` pieces need them (distillation, 4 pieces on 1,024 threads against 8 on 512: 4,096 x 32,000 bfloat16 105 us
+// against 112 with gradient, 61 against 59 without; 4,096 x 12,000 float32 77 against 82), for few only where 8 do (256 x
+// 12,000 float32 with 4 13.0 us, with 8 11.4).  Longer rows are read at every pass (kept = 0).  Loss and gradient take the
+// same shape, so the loss has the same bits with the gradient and alone.
 struct RowShape {
   int kept, threads;
 };
-RowShape row_shape(int64_t rows, int64_t cols, size_t elem, int least) {
+RowShape row_shape(int64_t rows, int64_t cols, size_t elem, int least, int many) {
   const int64_t pieces = (cols * (int64_t)elem + 15) / 16;   // whole ones at most
   for (int kept : {1, 2, 4, 8}) {
     const int64_t threads = std::max<int64_t>(round_up((pieces + kept - 1) / kept, 64), least);
-    if (threads <= 512 && (kept == 8 || rows < 1024)) return {kept, (int)threads};
-    if (kept == 8 && threads <= 1024) return {kept, 1024};
+    const bool enough = kept >= many;
+    if (threads <= 512 && (enough || rows < 1024)) return {kept, (int)threads};
+    if (threads <= 1024 && (kept == 8 || (enough && rows >= 1024))) return {kept, 1024};
   }
   return {0, 1024};
 }
@@ -746,7 +751,7 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
                            as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature, values,
                            index, tail);
       };
-      const RowShape shape = row_shape(rows, cols, sizeof(T), least);
+      const RowShape shape = row_shape(rows, cols, sizeof(T), least, 8);
       const int holders = std::min(shape.threads / 64, std::max(1, (full + 63) / 64));
       if (k > 32 * holders && cols <= 1024) run(k_top<T, Spread<T, 4>, true>, 256);
       else if (k > 32 * holders && cols <= 4096) run(k_top<T, Spread<T, 16>, true>, 256);
@@ -774,7 +779,7 @@ extern "C" int fly_distill(const void *z, int32_t type, int64_t ldz, int64_t row
       const DistillArgs<T> a{static_cast<const T *>(z), ldz, cols, legal, ldl, values, index, tail, k, temperature,
                              1.0f / temperature, loss, static_cast<T *>(grad), ldg, row_scale, grad_scale};
       const size_t lds = (size_t)round_up(cols, 32) / 8;
-      by_shape(row_shape(rows, cols, sizeof(T), 64), [&](auto nv, auto res, int threads) {
+      by_shape(row_shape(rows, cols, sizeof(T), 64, 4), [&](auto nv, auto res, int threads) {
         constexpr auto kernel = &k_distill<T, decltype(nv)::value, decltype(res)::value>;
         if (lds > 60 * 1024)
           FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
