@@ -489,7 +489,7 @@ __device__ __forceinline__ float divergence(float logp, float p, float logq, flo
 
 // One workgroup per row.  The first waves hold the list and compute the row's scalars; the others wait for the factor of
 // their exponentials, so what does not depend on the columns is computed once and not by every wave.  Bound by the row's
-// bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 61 us, 4.5 TB/s of the 5.1 that a copy
+// bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 57 us, 4.8 TB/s of the 5.1 that a copy
 // reaches; 2,048 x 50,256 bfloat16 94 us, 4.4 TB/s; x 50,257, whose rows' pieces lie across the lines, 104 us), by a row's
 // chain of load, two reductions, list and store where there are few (256 x 4,168 float32 7.2 us).
 template <typename T, int NV, bool RES>
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
   if (!a.grad) return;
   T *gr = a.grad + r * a.ldg;
   // A row past the registers reads its logits again here: its gradients go around the caches, which so still hold them
-  // (2,048 x 70,000 bfloat16 140 us against 155).  Rows in registers gain nothing (16,384 x 4,168 float16 65 against 61).
+  // (2,048 x 70,000 bfloat16 140 us against 155).  Rows in registers gain nothing (16,384 x 4,168 float32 106 against 102).
   auto store = [&](int j, int i, const Piece<T> &g) {
     if (j < 0) store_last(gr, i, row.left, g);
     else store_whole<T, !RES>(gr, i, g);
