@@ -26,7 +26,7 @@ from . import _hip
 from .brain import ConnectomeRNN
 from .connectome import Connectome
 from .encoding import N_BASE, N_FEATURES, N_MOVES, move_squares
-from .int8 import Int8Linear, quantize_rows
+from .int8 import Int8Linear
 
 READOUT_SUPERCLASSES = ("descending_neuron",)   # plus every efferent neuron (model.py:23)
 
@@ -79,7 +79,8 @@ class FlyChessNet(nn.Module):
         self.light_cone_pruning = True
         # float32 reads the outputs out in float32 accuracy; int8 holds the policy and WDL maps in 8 bits with a scale
         # for each move and quantises each position's outputs (chessfly/int8.py): for a network that labels positions
-        # (chessfly/distill.py), whose kept logits need no more than that.  Evaluation only.
+        # (chessfly/distill.py), whose kept logits need no more than that.  Evaluation only, and for batches: the layers are
+        # calls of their own then, which a single position pays for.
         self.head_dtype = torch.float32
         if cfg.shuffled:
             conn = conn.shuffled()
@@ -155,7 +156,7 @@ class FlyChessNet(nn.Module):
 
     def _forward_int8_head(self, x: torch.Tensor, plan, dense, half: bool) -> tuple[torch.Tensor, torch.Tensor]:
         """Encoder and recurrence as in the fused forward (the drive in the state's dtype, as forward_io takes it), then
-        the maps in 8 bits on the normalised outputs, quantised once for both."""
+        the maps in 8 bits on the normalised outputs, which each quantises on its way (the same bits)."""
         lib, dev, batch = _hip.load(), x.device, x.shape[0]
         policy, value = self._int8_heads()
         if not batch:
@@ -169,8 +170,8 @@ class FlyChessNet(nn.Module):
         ws = _hip.workspace(lib.fly_forward_io_workspace(plan.handle, batch), dev)
         _hip.call("fly_forward_io", dev.index, plan.handle, u.data_ptr(), batch, batch, r.data_ptr(), batch, ws.data_ptr(),
                   ws.numel())
-        q, scale = quantize_rows(self.norm(r.T))
-        return policy(q, scale=scale), value(q, scale=scale)
+        out = self.norm(r.T).contiguous()
+        return policy(out), value(out)
 
     def _forward_layers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The forward as separate differentiable layers (chessfly/model.py:95-105): training, or any call
