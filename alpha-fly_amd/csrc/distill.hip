@@ -490,7 +490,7 @@ __device__ __forceinline__ float divergence(float logp, float p, float logq, flo
 // One workgroup per row.  The first waves hold the list and compute the row's scalars; the others wait for the factor of
 // their exponentials, so what does not depend on the columns is computed once and not by every wave.  Bound by the row's
 // bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 57 us, 4.8 TB/s of the 5.1 that a copy
-// reaches; 2,048 x 50,256 bfloat16 94 us, 4.4 TB/s; x 50,257, whose rows' pieces lie across the lines, 104 us), by a row's
+// reaches; 2,048 x 50,256 bfloat16 96 us, 4.3 TB/s; x 50,257, whose rows' pieces lie across the lines, 104 us), by a row's
 // chain of load, two reductions, list and store where there are few (256 x 4,168 float32 7.2 us).
 template <typename T, int NV, bool RES>
 __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const DistillArgs<T> a) {
@@ -543,7 +543,9 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
         if ((b >> e) & 1) erase<T>(p, e);
   };
   float kept[kKeep ? NV * N : 1];
-  float shift = 0.0f;   // of this thread's exponentials, in powers of two
+  float base = 0.0f;   // of this thread's exponentials
+  // The maximum comes off before the scale: fma(z, scale, -base * scale) keeps the rounding of its constant, which passes any
+  // exponent for logits of 1e10 (fills of hidden moves), and costs as much time.
   if constexpr (RES) {
     float top = -INFINITY, sum = 0.0f;
     row.each([&](int, int i, Raw16 &p) {
@@ -551,30 +553,12 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
 #pragma unroll
       for (int e = 0; e < N; ++e) top = fmaxf(top, element<T>(p, e));
     });
-    float base = base_of(top);
-    if (fabsf(base) * scale2 > 1e37f) {
-      // the product with the scale would pass the range: near the type's lowest value the differences are exactly 0 or
-      // far beyond any exponent, so they take the logits' place
-      row.each([&](int, int, Raw16 &p) {
-        Raw16 d;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) d.v[w] = 0;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const uint32_t b = to_bits(static_cast<T>(element<T>(p, e) - base));
-          if constexpr (N == 4) d.v[e] = b;
-          else d.v[e / 2] |= b << (16 * (e & 1));
-        }
-        p = d;
-      });
-      base = 0.0f;
-    }
-    shift = -base * scale2;
+    base = base_of(top);
     if (!kKeep) row.forget();
     row.each([&](int j, int, const Raw16 &p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const float x = exp2_of(fmaf(element<T>(p, e), scale2, shift));
+        const float x = exp2_of((element<T>(p, e) - base) * scale2);
         if (kKeep && j >= 0) kept[kKeep && j >= 0 ? j * N + e : 0] = x;
         sum += x;
       }
@@ -671,13 +655,13 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
   }
   if constexpr (RES) {
     if (!kKeep) row.forget();
-    const float f = factor * exp2_of((base_of(own_top) - s_base) * scale2);
+    const float f = factor * exp2_of((base - s_base) * scale2);
     row.each([&](int j, int i, const Raw16 &p) {
       Piece<T> g;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         if (kKeep && j >= 0) g.v[e] = kept[kKeep && j >= 0 ? j * N + e : 0] * f;
-        else g.v[e] = exp2_of(fmaf(element<T>(p, e), scale2, shift)) * f;
+        else g.v[e] = exp2_of((element<T>(p, e) - base) * scale2) * f;
       }
       store(j, i, g);
     });

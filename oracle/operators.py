@@ -5,7 +5,8 @@ TEST INFRASTRUCTURE ONLY (imported by tests/; never by the product).  No counter
   int8_linear  (sum q w) (s t) + b, and the bound of a float32 evaluation of it
   top          the k largest visible logits, ties to the lower column, and the rest's log-sum-exp
   distill      loss and gradient by the formulas, row by row
-  rounding     what a float32 evaluation of top and distill may be off in an exponent
+  rounding     what a float32 evaluation of top and distill may be off in an exponent, by the largest logit of all rows
+  row_rounding, tail_rounding   the same for each row by its own logits, where differences are taken before the scale
 """
 
 from __future__ import annotations
@@ -47,6 +48,14 @@ def _lse(v: np.ndarray) -> float:
     return float(m + np.log(np.exp(v - m).sum()))
 
 
+def _parts(v: np.ndarray, temperature: float) -> tuple[float, float]:
+    """The largest of v (0 where there is none but -inf), and log sum exp((v - it) / temperature)."""
+    if v.size == 0 or v.max() == -np.inf:
+        return 0.0, -np.inf
+    m = v.max()
+    return float(m), float(np.log(np.exp((v - m) / temperature).sum()))
+
+
 def top(z: np.ndarray, k: int, temperature: float, legal=None):
     rows, cols = z.shape
     z = np.asarray(z, dtype=np.float64)
@@ -84,26 +93,31 @@ def distill(z, values, index, tail, temperature: float, legal=None):
         if any(c >= cols for c in cols_of) or len(set(cols_of)) < len(cols_of):
             loss[r], grad[r] = np.nan, np.nan
             continue
-        zt = z[r] / T
-        if legal is not None:
-            zt = np.where(legal[r] != 0, zt, -np.inf)
+        # differences come before the scale: a float64 has no digits left for a logarithm next to logits of 1e12
+        zr = z[r] if legal is None else np.where(legal[r] != 0, z[r], -np.inf)
         rest = np.ones(cols, bool)
         rest[cols_of] = False
-        lse_rest = _lse(zt[rest])
-        at = -np.inf if tail is None or lse_rest == -np.inf else float(tail[r])
-        a = np.append(np.asarray(values[r], np.float64)[listed] / T, at)
-        student = np.append(zt[cols_of], lse_rest)
-        A, B = _lse(a), _lse(student)
-        if A == -np.inf or B == -np.inf:
+        rest_top, rest_log = _parts(zr[rest], T)
+        has_rest = rest_log != -np.inf
+        at = -np.inf if tail is None or not has_rest else float(tail[r])
+        v = np.asarray(values[r], np.float64)[listed]
+        if (v.size == 0 or v.max() == -np.inf) and at == -np.inf or np.all(zr == -np.inf):
             continue
-        logp, logq = a - A, student - B
+        m = zr.max()
+        ln_z = _parts(zr, T)[1]
+        logq = np.append((zr[cols_of] - m) / T - ln_z, (rest_top - m) / T + rest_log - ln_z if has_rest else -np.inf)
+        v_top, v_log = _parts(v, T)
+        x = v_top / T if v_log != -np.inf else -np.inf
+        ma = max(x, at)
+        ln_a = np.log(np.exp(x - ma + v_log) + np.exp(at - ma))
+        logp = np.append((v - v_top) / T + (x - ma) - ln_a, at - ma - ln_a)
         p, q = np.exp(logp), np.exp(logq)
         with np.errstate(invalid="ignore"):
             d = np.where(p > 0, logp - logq, 0.0)
         loss[r] = T * T * float(np.sum(np.where(p > 0, p * d, 0.0)))
         size[r] = T * T * (1.0 + float(np.sum(np.where(p > 0, p * np.abs(d), 0.0))))
-        if lse_rest != -np.inf:
-            share = np.exp(zt - lse_rest)
+        if has_rest:
+            share = np.exp((zr - rest_top) / T - rest_log)
             grad[r] = np.where(rest, T * share * (q[-1] - p[-1]), 0.0)
             parts[r] = np.where(rest, T * share * (q[-1] + p[-1]), 0.0)
         grad[r, cols_of] = T * (q[:-1] - p[:-1])
@@ -122,3 +136,50 @@ def rounding(z, values, temperature: float, threads: int = 64) -> float:
         big = max(big, float(np.abs(v).max()) / temperature if v.size else 0.0)
     terms = -(-np.asarray(z).shape[1] // threads)
     return (6 * big + terms + 24) * 2.0 ** -24
+
+
+MOST = 110.0        # exp of less than -MOST is 0 in float32: a difference past it adds no error
+LEAST = 2.0 ** -124  # four of float32's smallest normal numbers, below which an exponential may count as 0
+
+
+def _spread(v: np.ndarray, temperature: float) -> float:
+    v = np.asarray(v, dtype=np.float64)
+    v = v[np.isfinite(v)]
+    return min(float(v.max() - v.min()) / temperature, MOST) if v.size else 0.0
+
+
+def _terms(z, threads: int) -> int:
+    return -(-np.asarray(z).shape[1] // threads) + 24
+
+
+def row_rounding(z, values, tail, temperature: float, legal=None, threads: int = 64) -> np.ndarray:
+    """How far an exponent of distill may be off in each row.  Differences of logits come before the scale, so a row's error
+    does not depend on where its logits lie but on how far they spread: 2^-24 of a difference / T for it, the scale (its two
+    roundings) and the product, through up to three maxima (a thread's, a list's or the rest's, the row's), whose steps add
+    up to no more than the spread: 6 spreads, of the student and of the list.  The teacher's tail is scaled already: where it
+    is near the list's largest entry, that one is scaled too, two roundings of its size.  The sum and the functions as in
+    `rounding`."""
+    off = np.zeros(len(z))
+    for r in range(len(z)):
+        seen = z[r] if legal is None else np.asarray(z[r])[np.asarray(legal[r]) != 0]
+        size = 6 * (_spread(seen, temperature) + _spread(values[r], temperature))
+        v = np.asarray(values[r], np.float64)
+        v = v[np.isfinite(v)]
+        if tail is not None and np.isfinite(tail[r]) and v.size and abs(v.max() / temperature - tail[r]) < MOST + 10:
+            size += 2 * abs(v.max()) / temperature
+        off[r] = size
+    return (off + _terms(z, threads)) * 2.0 ** -24
+
+
+def tail_rounding(z, index, temperature: float, legal=None, threads: int = 64) -> np.ndarray:
+    """How far the tail of top may be off in each row: the spread of what is not listed, taken from a bound that lies at most
+    MOST / 2 above it, as above; and four roundings of its largest logit / T (the bound's scaling, 1 / T, its product, the
+    sum)."""
+    off = np.zeros(len(z))
+    for r in range(len(z)):
+        rest = np.ones(len(z[r]), bool) if legal is None else np.asarray(legal[r]) != 0
+        rest[[c for c in index[r] if c >= 0]] = False
+        v = np.asarray(z[r], np.float64)[rest]
+        v = v[np.isfinite(v)]
+        off[r] = 6 * (_spread(v, temperature) + MOST / 2) + 4 * (abs(v.max()) / temperature if v.size else 0.0)
+    return (off + _terms(z, threads)) * 2.0 ** -24

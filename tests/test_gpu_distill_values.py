@@ -1,0 +1,89 @@
+"""GPU tests of top logits and distillation where the logits' values are out of the ordinary, each row within its own bound:
+an extreme value in one row loosens no other (see oracle.operators.row_rounding and tail_rounding).
+
+Tolerances, of an exponent that is off by e: the loss moves by its size (sum p |log(p/q)| + 1) times two of them (p's and q's),
+doubled for the divergence's own terms; a gradient by its two parts times as much, plus its rounding to the logits' type.  What
+is below the smallest normal float32 may count as 0."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import operators as O
+from test_gpu_distill import DEV, FLOATS, INF, NAMES, _dev, _logits, _mask, _near, _np, _teacher
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_top(z, k, temperature=1.0, legal=None):
+    from chessfly.distill import top_logits
+    got = top_logits(_dev(z), k, temperature, _dev(legal))
+    with np.errstate(invalid="ignore"):
+        values, index, tail = O.top(_np(z), k, temperature, _np(legal))
+    assert np.array_equal(got.index.cpu().numpy(), index)
+    assert np.array_equal(got.values.double().cpu().numpy(), values, equal_nan=True)
+    _near(got.tail, tail, O.tail_rounding(_np(z), index, temperature, _np(legal)))
+
+
+def _check_distill(z, teacher, temperature=1.0, legal=None):
+    """The one-pass call, the loss alone, and autograd with a factor of its own for each row.  Returns the gradient."""
+    from chessfly.distill import TopLogits, distill_loss, distill_loss_and_grad
+    td, zd = TopLogits(*map(_dev, teacher)), _dev(z)
+    kw = dict(temperature=temperature, legal=_dev(legal))
+    loss, grad = distill_loss_and_grad(zd, td, **kw)
+    with np.errstate(invalid="ignore", over="ignore"):
+        ref, ref_grad, size, parts = O.distill(_np(z), *map(_np, teacher), temperature, _np(legal))
+    off = O.row_rounding(_np(z), _np(teacher[0]), _np(teacher[2]), temperature, _np(legal))
+    unit, tiny = O.UNIT[NAMES[z.dtype]], O.TINY[NAMES[z.dtype]]
+
+    def check_grad(got, w):
+        _near(got, ref_grad * w, (4 * off[:, None] + 8 * 2.0 ** -24) * np.abs(parts * w) + 1.01 * unit * np.abs(ref_grad * w)
+              + tiny + O.LEAST * temperature * np.abs(w))
+
+    _near(loss, ref, 4 * off * size)
+    check_grad(grad, np.ones((len(z), 1)))
+    alone = distill_loss(zd, td, reduction="none", **kw)
+    assert torch.equal(torch.nan_to_num(alone, 7.0), torch.nan_to_num(loss, 7.0))
+    leaf = zd.detach().clone().requires_grad_(True)
+    up = torch.linspace(0.25, 2.0, len(z))
+    distill_loss(leaf, td, reduction="none", **kw).backward(_dev(up))
+    check_grad(leaf.grad, _np(up)[:, None])
+    return grad
+
+
+# the fills that a program puts on moves that are not legal, and how far its logits spread with them
+FILLS = [(torch.float32, f) for f in (-1e5, -1e9, -1e10, -1e12, -1e20, -1e30, -1e32, -3.4028234663852886e38)]
+FILLS += [(torch.bfloat16, f) for f in (-1e9, -1e10, -1e12, -1e20, -1e30, -1e32, -3.3895313892515355e38)]
+FILLS += [(torch.float16, f) for f in (-3e4, -65504.0)]
+
+
+@pytest.mark.parametrize("cols", [300, 4168, 16390, 33000, 70000])
+@pytest.mark.parametrize("dtype,fill", FILLS)
+def test_illegal_moves_filled_with_a_large_negative_number(cols, dtype, fill):
+    """No mask: the fill takes its place.  The list holds some of the 30 legal moves, all of them, and fills too."""
+    g = torch.Generator().manual_seed(cols)
+    z, t = _logits(5, cols, 1), _logits(5, cols, 2)
+    for row in (0, 1, 2):
+        hidden = torch.ones(cols, dtype=torch.bool)
+        hidden[torch.randperm(cols, generator=g)[:30]] = False
+        z[row, hidden] = t[row, hidden] = fill
+    z[1] = fill                                             # nothing but fills
+    z[3] = (z[3] * abs(fill) / 64).clamp(fill / 8, -fill / 8)   # logits of that size themselves
+    z, t = z.to(dtype), t.to(dtype).float()
+    f = lambda a: torch.from_numpy(a.astype(np.float32))
+    for k, temperature in ((8, 1.0), (30, 1.0), (40, 1.0)) + (((8, 2.0), (30, 2.0)) if fill > -1e35 else ()):
+        values, index, tail = O.top(_np(t), k, temperature)
+        teacher = f(values), torch.from_numpy(index), f(tail)
+        _check_distill(z, teacher, temperature)
+        _check_distill(z, (*teacher[:2], None), temperature)
+        _check_top(z, k, temperature)
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 1e-6])
+def test_a_small_temperature_is_a_large_logit(temperature):
+    for dtype in FLOATS:
+        z = _logits(4, 4168, 3, dtype)
+        _check_distill(z, _teacher(4, 4168, 8, 5, temperature, tail=False), temperature)
+        _check_top(z, 8, temperature)
