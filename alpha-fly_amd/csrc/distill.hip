@@ -655,7 +655,9 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
   }
   if constexpr (RES) {
     if (!kKeep) row.forget();
-    const float f = factor * exp2_of((base - s_base) * scale2);
+    // A thread that holds none of the rest has exponentials of 0, and no base of its own to compare with the row's: its
+    // gradients are 0, but the row's NaN where the factor is one.
+    const float f = factor * (own_top == -INFINITY ? 0.0f : exp2_of((base - s_base) * scale2));
     row.each([&](int j, int i, const Raw16 &p) {
       Piece<T> g;
 #pragma unroll

@@ -87,3 +87,20 @@ def test_a_small_temperature_is_a_large_logit(temperature):
         z = _logits(4, 4168, 3, dtype)
         _check_distill(z, _teacher(4, 4168, 8, 5, temperature, tail=False), temperature)
         _check_top(z, 8, temperature)
+
+
+# register rows of 1, 2, 4 and 8 pieces a thread, and rows past them
+@pytest.mark.parametrize("rows,cols", [(4, 300), (4, 4168), (4, 9000), (4, 20000), (4, 33000), (2, 70000), (1030, 1200)])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shift,temperature", [(-100.0, 1.0), (-1000.0, 1.0), (0.0, 0.02), (-60.0, 0.5), (1000.0, 1.0)])
+def test_threads_that_see_nothing_of_a_row_that_lies_low(rows, cols, dtype, shift, temperature):
+    """About 30 visible moves: most threads hold none.  The softmax does not see a constant added to all logits."""
+    z = (_logits(rows, cols, 1) - 10 * (shift == 0) + shift).to(dtype)
+    legal = _mask(rows, cols, 7, 30 / cols)
+    legal[rows - 1, :20] = True
+    hidden = torch.where(legal, z, torch.tensor(-INF, dtype=dtype))     # the same without a mask
+    for k in (8, 64):
+        teacher = _teacher(rows, cols, k, 5, temperature, legal)
+        grad = _check_distill(z, teacher, temperature, legal)
+        assert bool((grad[~legal.to(DEV)] == 0).all())
+        assert torch.equal(_check_distill(hidden, teacher, temperature), grad)
