@@ -708,8 +708,8 @@ void check_logits(const void *z, int64_t ldz, int64_t rows, int64_t cols, const 
                   float temperature) {
   FLY_REQUIRE(rows >= 0 && rows < INT32_MAX && cols >= 1 && cols <= kMostColumns, "rows or columns out of range");
   FLY_REQUIRE(k >= 1 && k <= kMostListed, "k must lie in 1..256");
-  FLY_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature),
-              "the temperature must be positive and finite");
+  FLY_REQUIRE(temperature > 0.0f && std::isfinite(temperature) && std::isfinite(1.0f / temperature * kLog2e),
+              "the temperature must be positive and finite, and log2(e) / temperature too");
   FLY_REQUIRE(!rows || (z && ldz >= cols), "logits are null or their rows overlap");
   FLY_REQUIRE(!legal || ldl >= cols, "the mask's rows overlap");
 }

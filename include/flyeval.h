@@ -487,7 +487,7 @@ int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int
 /* ---- distillation from a teacher's top logits ---------------------------------------------------- */
 /* No counterpart in the reference.  Logits z (rows, ldz) are FLY_F32, FLY_F16 or FLY_BF16 over cols columns (1 to 2^20); legal
  * (rows, ldl) bytes, NULL or 0 for columns that do not exist for the row.  Columns at -inf count as not existing too.
- * k lies in 1..256, the temperature is positive.
+ * k lies in 1..256, the temperature is positive and finite, and so is log2(e) / temperature in float32 (from 4.3e-39 on).
  *
  * fly_top_logits: values and index (rows, k): the k largest logits in falling order, the lower column first among
  * equals (NaN above all), padded with -inf and -1; tail (rows) or NULL: log sum exp(z / temperature) over the columns
