@@ -594,7 +594,8 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
     const float logqt = has_rest ? (rest_top - mz) * a.inv_t + ln_of(part[0].sum) - ln_z : -INFINITY;
     // the teacher's, its tail a scaled number already: log p = (v - mv) / T + (x - ma) - ln_a
     const float at = a.tail && has_rest ? a.tail[r] : -INFINITY;   // no rest to put it on: the list alone
-    const float mv = base_of(part[1].top), x = part[1].empty() ? -kMostFloat : fmaxf(mv * a.inv_t, -kMostFloat);
+    const float mv = base_of(part[1].top);
+    const float x = part[1].empty() ? -kMostFloat : fminf(fmaxf(mv * a.inv_t, -kMostFloat), kMostFloat);
     const float ma = fmaxf(x, at);
     const float ln_a = ln_of(part[1].sum * exp_of(x - ma) + exp_of(at - ma)), logpt = at - ma - ln_a;
     const bool some = !(part[1].empty() && at == -INFINITY) && !(part[0].empty() && part[2].empty());
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
       s_nothing = !some;
       s_factor = bad ? nan : has_rest ? scale * (qt - pt) / part[0].sum : 0.0f;
       s_loss = some ? divergence(logpt, pt, logqt, qt) : 0.0f;   // the rest's share
-      if (few == 1 && a.loss) a.loss[r] = bad ? nan : a.t * a.t * (l + s_loss);
+      if (few == 1 && a.loss) a.loss[r] = bad ? nan : a.t * (a.t * (l + s_loss));
     }
   }
   __syncthreads();
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const Distill
       n += share_loss[2 * w + 1];
     }
     bad = n != 0.0f;
-    if (tid == 0 && a.loss) a.loss[r] = bad ? nan : a.t * a.t * (l + s_loss);
+    if (tid == 0 && a.loss) a.loss[r] = bad ? nan : a.t * (a.t * (l + s_loss));
     if (bad) factor = nan;
   }
   if (!a.grad) return;

@@ -495,7 +495,8 @@ int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int
  *
  * fly_distill: from values, index (rows, k) and tail (rows; NULL: the teacher is its list alone) the loss (rows) and its
  * gradient by z, either NULL: temperature^2 times the Kullback-Leibler divergence from the teacher's softmax to the
- * student's at the temperature, over the listed columns and one class for all others.
+ * student's at the temperature, over the listed columns and one class for all others.  Sums are float32, so a loss
+ * carries about 1e-7 temperature^2.
  * grad (rows, ldg) of z's type = grad_scale * row_scale[r] (NULL: 1) * dloss[r]/dz, 0 on columns that do not exist.
  * Entries with index -1 (any negative), or on a column that does not exist by `legal`, are left out; so is the tail
  * where the student has no column outside the list.  A row with no entry left, or whose student has no column, gives 0.

@@ -39,8 +39,12 @@ def _check_distill(z, teacher, temperature=1.0, legal=None):
     unit, tiny = O.UNIT[NAMES[z.dtype]], O.TINY[NAMES[z.dtype]]
 
     def check_grad(got, w):
-        _near(got, ref_grad * w, (4 * off[:, None] + 8 * 2.0 ** -24) * np.abs(parts * w) + 1.01 * unit * np.abs(ref_grad * w)
-              + tiny + O.LEAST * temperature * np.abs(w))
+        want = ref_grad * w
+        tol = ((4 * off[:, None] + 8 * 2.0 ** -24) * np.abs(parts * w) + 1.01 * unit * np.abs(want) + tiny
+               + O.LEAST * temperature * np.abs(w))
+        past = np.isfinite(want) & (np.abs(want) + tol > torch.finfo(z.dtype).max)     # may round to an infinity
+        assert not bool(torch.isnan(got)[torch.from_numpy(past).to(DEV)].any())
+        _near(torch.where(torch.from_numpy(past).to(DEV), 0.0, got.double()), np.where(past, 0.0, want), tol)
 
     _near(loss, ref, 4 * off * size)
     check_grad(grad, np.ones((len(z), 1)))
@@ -104,3 +108,16 @@ def test_threads_that_see_nothing_of_a_row_that_lies_low(rows, cols, dtype, shif
         grad = _check_distill(z, teacher, temperature, legal)
         assert bool((grad[~legal.to(DEV)] == 0).all())
         assert torch.equal(_check_distill(hidden, teacher, temperature), grad)
+
+
+@pytest.mark.parametrize("temperature", [1e-20, 1e-36, 1e20])
+def test_temperatures_whose_square_leaves_the_range(temperature):
+    for dtype in FLOATS:
+        z = _logits(4, 4168, 3, dtype)
+        _check_distill(z, _teacher(4, 4168, 8, 5, temperature, tail=temperature > 1), temperature)
+        _check_top(z, 8, temperature)
+
+
+def test_a_teacher_whose_scaled_logits_leave_the_range():
+    z, (values, index, _) = _logits(4, 4168, 3, scale=0.3), _teacher(4, 4168, 8, 5, 1.0)
+    _check_distill(z, (values / 10 + 10, index, None), 2e-38)
