@@ -266,6 +266,14 @@ inline unsigned blocks_for(int64_t work, int per_block) {
   return static_cast<unsigned>((work + per_block - 1) / per_block);
 }
 
+// f(first row, rows) for slices of `rows` whose launches stay below 2^31 threads (past 2^32 a grid wraps without an error), at
+// `threads` for each row; slices start at multiples of 2^16 rows.
+template <typename F>
+void in_slices(int64_t rows, int64_t threads, F &&f) {
+  const int64_t most = std::max<int64_t>((((int64_t)1 << 31) / threads) >> 16, 1) << 16;
+  for (int64_t first = 0; first < rows; first += most) f(first, std::min(most, rows - first));
+}
+
 inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 inline bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }

@@ -734,9 +734,12 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
       const int least = (int)round_up(2 * k, 64), full = (int)(cols * (int64_t)sizeof(T) / 16);
       auto run = [&](auto kernel, int threads) {
         const int waves = threads / 64;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 8 * (size_t)(top_list(waves) + waves * kWaveCandidates),
-                           as_stream(stream), static_cast<const T *>(z), ldz, cols, legal, ldl, k, 1.0f / temperature, values,
-                           index, tail);
+        in_slices(rows, threads, [&](int64_t r, int64_t n) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 8 * (size_t)(top_list(waves) + waves * kWaveCandidates),
+                             as_stream(stream), static_cast<const T *>(z) + r * ldz, ldz, cols, legal ? legal + r * ldl : nullptr,
+                             ldl, k, 1.0f / temperature, values + r * k, index + r * k, tail ? tail + r : nullptr);
+          check_launch("top logits");
+        });
       };
       const RowShape shape = row_shape(rows, cols, sizeof(T), least, 8);
       const int holders = std::min(shape.threads / 64, std::max(1, (full + 63) / 64));
@@ -746,7 +749,6 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
         by_shape(shape, [&](auto nv, auto res, int threads) {
           run(k_top<T, Row<T, decltype(nv)::value, decltype(res)::value>, false>, threads);
         });
-      check_launch("top logits");
     });
   });
 }
@@ -763,17 +765,21 @@ extern "C" int fly_distill(const void *z, int32_t type, int64_t ldz, int64_t row
     by_type(type, [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      const DistillArgs<T> a{static_cast<const T *>(z), ldz, cols, legal, ldl, values, index, tail, k, temperature,
-                             1.0f / temperature, loss, static_cast<T *>(grad), ldg, row_scale, grad_scale};
       const size_t lds = (size_t)round_up(cols, 32) / 8;
       by_shape(row_shape(rows, cols, sizeof(T), 64, 4), [&](auto nv, auto res, int threads) {
         constexpr auto kernel = &k_distill<T, decltype(nv)::value, decltype(res)::value>;
         if (lds > 60 * 1024)
           FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)lds));
-        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), lds, as_stream(stream), a);
+        in_slices(rows, threads, [&](int64_t r, int64_t n) {
+          const DistillArgs<T> a{static_cast<const T *>(z) + r * ldz, ldz, cols, legal ? legal + r * ldl : nullptr, ldl,
+                                 values + r * k, index + r * k, tail ? tail + r : nullptr, k, temperature, 1.0f / temperature,
+                                 loss ? loss + r : nullptr, grad ? static_cast<T *>(grad) + r * ldg : nullptr, ldg,
+                                 row_scale ? row_scale + r : nullptr, grad_scale};
+          hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), lds, as_stream(stream), a);
+          check_launch("distillation");
+        });
       });
-      check_launch("distillation");
     });
   });
 }

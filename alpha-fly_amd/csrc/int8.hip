@@ -582,9 +582,12 @@ extern "C" int fly_quantize_rows(const void *x, int32_t x_type, int64_t ldx, int
     by_float(x_type, "x must be float32, float16 or bfloat16", [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      hipLaunchKernelGGL((k_quantize<T, false>), dim3(blocks_for(rows, 4)), dim3(256), 0, as_stream(stream),
-                         static_cast<const T *>(x), ldx, rows, cols, (int64_t)0, q, ldq, scale);
-      check_launch("quantised rows");
+      in_slices(rows, 64, [&](int64_t r, int64_t n) {
+        hipLaunchKernelGGL((k_quantize<T, false>), dim3(blocks_for(n, 4)), dim3(256), 0, as_stream(stream),
+                           cols ? static_cast<const T *>(x) + r * ldx : nullptr, ldx, n, cols, (int64_t)0,
+                           cols ? q + r * ldq : nullptr, ldq, scale + r);
+        check_launch("quantised rows");
+      });
     });
   });
 }
