@@ -27,6 +27,8 @@ namespace {
 
 typedef int int4v __attribute__((ext_vector_type(4)));
 constexpr int64_t kMostK = 1 << 17;   // sums below 2^31
+// A launch holds less than 2^32 threads: 64 for each block of an operand that is laid out, 256 for 16 channels of few rows.
+constexpr int64_t kMostBlocks = (int64_t)1 << 26, kMostChannels = (int64_t)1 << 28;
 constexpr int kFewBlocks = 12;   // blocks of k that a wave of k_int8_few holds
 
 // Where 16-byte piece c (k 16 c .. + 15) of row r lies among the blocks.
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restr
 template <typename T, int WN, int WM, int FN, int FM, int S>
 void int8_gemm(const fly_int8 &p, const int4v *q, const float *row_scale, int64_t rows, T *y, int64_t ldy, hipStream_t st) {
   const int mb = (int)((rows + 15) / 16), mt = (mb + WM * FM - 1) / (WM * FM), nt = (int)((p.nb + WN * FN - 1) / (WN * FN));
-  FLY_REQUIRE((int64_t)mt * nt < INT32_MAX / 16, "product too large");
+  FLY_REQUIRE((int64_t)mt * nt < (int64_t)1 << 32 >> 9, "product too large");   // at up to 512 threads
   hipLaunchKernelGGL((k_int8_gemm<T, WN, WM, FN, FM, S>), dim3(mt * nt), dim3(64 * WN * WM), 0, st,
                      reinterpret_cast<const int4v *>(p.w()), q, row_scale, p.scale(), p.bias(), (int)rows, (int)p.n,
                      (int)p.nb, mb, (int)p.kb, mt * nt, mt, nt, y, ldy);
@@ -497,7 +499,7 @@ void by_float(int32_t type, const char *what, F &&f) {
 
 void pack(const int8_t *src, int64_t ld, int64_t rows, int64_t k, int64_t kb, void *out, hipStream_t st) {
   const int64_t blocks = (rows + 15) / 16 * kb;
-  FLY_REQUIRE(blocks < INT32_MAX, "operand too large");
+  FLY_REQUIRE(blocks < kMostBlocks, "operand too large");
   hipLaunchKernelGGL(k_int8_pack, dim3(blocks_for(blocks, 4)), dim3(256), 0, st, src, ld, rows, k, (uint32_t)kb,
                      (uint32_t)blocks, static_cast<int4v *>(out));
   check_launch("8-bit blocks");
@@ -597,7 +599,8 @@ extern "C" int fly_int8_create(const int8_t *w, int64_t ldw, const float *scale,
   return guard([&] {
     FLY_REQUIRE(out != nullptr, "out is null");
     *out = nullptr;
-    FLY_REQUIRE(n >= 1 && k >= 1 && k < kMostK && n < (int64_t)INT32_MAX && ldw >= k, "bad size");
+    FLY_REQUIRE(n >= 1 && k >= 1 && k < kMostK && n < kMostChannels && ldw >= k, "bad size");
+    FLY_REQUIRE((n + 15) / 16 * ((k + 63) / 64) < kMostBlocks, "bad size: the weight is too large");
     FLY_REQUIRE(w && scale, "null pointer");
     hipStream_t st = as_stream(stream);
     auto p = std::make_unique<fly_int8>();

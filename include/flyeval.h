@@ -469,15 +469,16 @@ int fly_train_step_backward(int64_t rows, int64_t batch, const float *g_dev, int
 int fly_quantize_rows(const void *x_dev, int32_t x_type, int64_t ldx, int64_t rows, int64_t cols, int8_t *q_dev,
                       int64_t ldq, float *scale_dev, void *stream);
 
-/* A weight in 8 bits, laid out once for the matrix cores: w (n, ldw) int8 over k columns (k below 2^17), scale (n), bias
- * (n) or NULL.  The plan copies what it needs. */
+/* A weight in 8 bits, laid out once for the matrix cores: w (n, ldw) int8 over k columns (k below 2^17, n below 2^28, and n k,
+ * rounded up to 16 and 64, below 2^36), scale (n), bias (n) or NULL.  The plan copies what it needs. */
 typedef struct fly_int8 fly_int8;
 int fly_int8_create(const int8_t *w_dev, int64_t ldw, const float *scale_dev, const float *bias_dev, int64_t n,
                     int64_t k, void *stream, fly_int8 **out);
 int fly_int8_destroy(fly_int8 *plan);
 /* y (rows, ldy) of y_type = (sum_k q[m, k] w[n, k]) (s[m] scale[n]) + bias[n]: integer sums exact, scaled in float32.
  * x (rows, ldx) float32, float16 or bfloat16 is quantised by rows as fly_quantize_rows does (x_scale NULL); FLY_I8
- * rows are taken as they are, with x_scale (rows).  rows below 2^24.  y must not overlap x.  The workspace, 256-byte
+ * rows are taken as they are, with x_scale (rows).  rows below 2^24, and of FLY_I8 rows k, rounded up as n k is, below 2^36.
+ * y must not overlap x.  The workspace, 256-byte
  * aligned, may be NULL where the query says 0 (few rows). */
 size_t fly_int8_workspace(const fly_int8 *plan, int32_t x_type, int64_t rows);
 int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int64_t ldx, const float *x_scale_dev,
