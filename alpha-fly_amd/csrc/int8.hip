@@ -406,7 +406,10 @@ __global__ __launch_bounds__(256 * C) void k_int8_few(const int4v *__restrict__ 
   extern __shared__ int4v blocks[];   // the quantised rows, R x kb blocks
   __shared__ int4v sums[C][4][R][64];
   __shared__ float s_scale[16 * R];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave & 3, cb = blockIdx.x * C + (wave >> 2);
+  // one number for the wave: its loads and products stand behind scalar branches.  The matrix cores do not look at exec, so a
+  // product behind a mask is skipped only where the compiler happens to keep a branch over it.
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = wave & 3, cb = blockIdx.x * C + (wave >> 2);
   const int4v *wb = w + (int64_t)min(cb, nb - 1) * kb * 64 + lane;
   int4v fw[kFewBlocks];
   auto fetch = [&](int b0) {
