@@ -266,6 +266,14 @@ inline unsigned blocks_for(int64_t work, int per_block) {
   return static_cast<unsigned>((work + per_block - 1) / per_block);
 }
 
+// Lets `kernel` have `most` bytes of dynamic LDS.  The limit belongs to the function and not to a launch: with each call's own
+// size here, a small call would take it back between another thread's large call and that one's launch.  So `most` is the
+// most that the kernel can take, whatever this call needs.
+template <typename K>
+void allow_lds(K kernel, int64_t most) {
+  FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+}
+
 // f(first row, rows) for slices of `rows` whose launches stay below 2^31 threads (past 2^32 a grid wraps without an error), at
 // `threads` for each row; slices start at multiples of 2^16 rows.
 template <typename F>

@@ -768,9 +768,7 @@ extern "C" int fly_distill(const void *z, int32_t type, int64_t ldz, int64_t row
       const size_t lds = (size_t)round_up(cols, 32) / 8;
       by_shape(row_shape(rows, cols, sizeof(T), 64, 4), [&](auto nv, auto res, int threads) {
         constexpr auto kernel = &k_distill<T, decltype(nv)::value, decltype(res)::value>;
-        if (lds > 60 * 1024)
-          FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)lds));
+        if (lds > 60 * 1024) allow_lds(kernel, kMostColumns / 8);
         in_slices(rows, threads, [&](int64_t r, int64_t n) {
           const DistillArgs<T> a{static_cast<const T *>(z) + r * ldz, ldz, cols, legal ? legal + r * ldl : nullptr, ldl,
                                  values + r * k, index + r * k, tail ? tail + r : nullptr, k, temperature, 1.0f / temperature,

@@ -30,6 +30,7 @@ constexpr int64_t kMostK = 1 << 17;   // sums below 2^31
 // A launch holds less than 2^32 threads: 64 for each block of an operand that is laid out, 256 for 16 channels of few rows.
 constexpr int64_t kMostBlocks = (int64_t)1 << 26, kMostChannels = (int64_t)1 << 28;
 constexpr int kFewBlocks = 12;   // blocks of k that a wave of k_int8_few holds
+constexpr int kFewSpan = 48;     // and that a row has at most where the product quantises it
 
 // Where 16-byte piece c (k 16 c .. + 15) of row r lies among the blocks.
 __device__ __forceinline__ int64_t block_piece(int64_t r, int64_t c, int64_t kb) {
@@ -538,7 +539,7 @@ size_t int8_ws(const fly_int8 &p, int64_t rows) {
 // rows 10.5 against 11.5, 32 rows 13.8 against 13.2; the second launch costs the host another 4.  17,937 channels over 838:
 // 1 row 12.8 against 9.9.
 bool quantises_few(const fly_int8 &p, int32_t x_type, int64_t rows) {
-  return x_type != FLY_I8 && rows <= 32 && p.nb <= 512 && p.kb <= 48;
+  return x_type != FLY_I8 && rows <= 32 && p.nb <= 512 && p.kb <= kFewSpan;
 }
 
 template <typename X, typename T, int C, int R>
@@ -546,8 +547,7 @@ void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_sc
               hipStream_t st) {
   const size_t lds = std::is_void_v<X> ? 0 : (size_t)R * p.kb * 1024;
   constexpr auto kernel = &k_int8_few<X, T, C, R>;
-  if (lds > 48 * 1024)
-    FLY_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  if (lds > 32 * 1024) allow_lds(kernel, R * kFewSpan * 1024);
   hipLaunchKernelGGL(kernel, dim3(blocks_for(p.nb, C)), dim3(256 * C), lds, st, reinterpret_cast<const int4v *>(p.w()), x,
                      ldx, row_scale, p.scale(), p.bias(), (int)rows, (int)p.n, (int)p.k, (int)p.nb, (int)p.kb, y, ldy);
   check_launch("8-bit product of few rows");
