@@ -10,6 +10,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libflyeval.so")
 
@@ -187,6 +188,36 @@ def row_major(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     if (cols <= 1 or step == 1) and (rows <= 1 or ld >= cols):
         return t, ld if rows > 1 else cols or 1
     return t.contiguous(), cols or 1
+
+
+def tracked(t: torch.Tensor) -> bool:
+    """Whether autograd, backward or forward mode, follows what is computed from t."""
+    if t.requires_grad and torch.is_grad_enabled():
+        return True
+    # unpack_dual alone takes 0.3 us; the level, where this torch has it, says that no tensor is dual
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+class _NoBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, run, *tensors):
+        ctx.what = what
+        out = run()
+        ctx.mark_non_differentiable(*(t for t in (out if isinstance(out, tuple) else (out,))
+                                      if t is not None and not t.is_floating_point()))
+        return out
+
+    @staticmethod
+    def backward(ctx, *up):
+        raise RuntimeError(f"{ctx.what} has no backward pass: detach its inputs or results")
+
+
+def undifferentiated(what: str, run, *tensors):
+    """run(), an operator without a derivative, on tensors of which autograd tracks one: the results are the same, and a backward
+    pass that would go through them raises, as torch's own operators without a derivative do, instead of finding nothing."""
+    if any(t is not None and tracked(t) and not t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+    return _NoBackward.apply(what, run, *tensors)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

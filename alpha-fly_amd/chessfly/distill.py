@@ -54,7 +54,10 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal: to
                tail: bool = True) -> TopLogits:
     """The k (1 to 256) largest logits of each row over the legal columns, the lower column first among equals, and the
     log-sum-exp of the others.  Rows with fewer legal columns (a column at -inf is none) end in values -inf and index -1;
-    a tail of nothing is -inf."""
+    a tail of nothing is -inf.  Not differentiable: a backward pass through the values or the tail raises."""
+    if _hip.tracked(logits):
+        return TopLogits(*_hip.undifferentiated(
+            "top_logits", lambda: tuple(top_logits(logits, k, temperature, legal, tail)), logits))
     logits, ld = _logits(logits, "top_logits")
     legal, ld_legal = _legal(legal, logits, "top_logits")
     rows, cols = logits.shape
@@ -98,7 +101,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher: TopLogits, temperature:
                           legal: torch.Tensor | None = None, grad_scale: float = 1.0,
                           row_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The loss of each row (float32) and, in the same pass, grad_scale * row_scale * dloss/dlogits in the logits' type
-    (grad_scale = 1 / rows: the gradient of the mean).  For training loops: `logits.backward(grad)`."""
+    (grad_scale = 1 / rows: the gradient of the mean).  For training loops: `logits.backward(grad)`; autograd does not follow
+    the two results themselves."""
     what = "distill_loss_and_grad"
     logits, ld = _logits(logits, what)
     legal, ld_legal = _legal(legal, logits, what)
@@ -139,7 +143,7 @@ class _DistillLoss(torch.autograd.Function):
 
 def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 1.0,
                  legal: torch.Tensor | None = None, reduction: str = "mean") -> torch.Tensor:
-    """The student's loss against a teacher's list, differentiable by `logits` (the teacher's tensors get no gradient).
+    """The student's loss against a teacher's list, differentiable once by `logits` (the teacher's tensors get no gradient).
     reduction: "mean" or "sum" over rows, or "none" (rows) float32.
 
     A row without a listed legal move (index -1, or a move that `legal` hides), or whose student sees no move, has loss
@@ -150,7 +154,7 @@ def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 
     logits, ld = _logits(logits, "distill_loss")
     legal, ld_legal = _legal(legal, logits, "distill_loss")
     teacher = _teacher(teacher, logits, "distill_loss")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _hip.tracked(logits):      # in forward mode torch says that there is no such derivative
         loss = _DistillLoss.apply(logits, ld, *(t.detach() if t is not None else None for t in teacher), temperature, legal,
                                   ld_legal)
     else:

@@ -26,7 +26,10 @@ def _rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """x (rows, columns) float32, float16 or bfloat16 -> int8 values (rows, columns) and float32 scales (rows)."""
+    """x (rows, columns) float32, float16 or bfloat16 -> int8 values (rows, columns) and float32 scales (rows).  Not
+    differentiable: a backward pass through the scales raises."""
+    if _hip.tracked(x):
+        return _hip.undifferentiated("quantize_rows", lambda: quantize_rows(x), x)
     x, ld = _rows(x, "quantize_rows")
     if x.dtype not in FLOATS:
         raise RuntimeError(f"quantize_rows: x must be float32, float16 or bfloat16, got {x.dtype}")
@@ -40,7 +43,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 class Int8Linear:
     """y = x W^T + b with W (channels, k) in 8 bits.  The weight is laid out for the matrix cores once, here; the object
-    keeps no reference to the tensors.  Calls run on the current stream with scratch from torch's allocator."""
+    keeps no reference to the tensors: they are constants to autograd.  Calls run on the current stream with scratch from
+    torch's allocator."""
 
     def __init__(self, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None):
         weight, ld = _rows(weight, "Int8Linear")
@@ -69,7 +73,10 @@ class Int8Linear:
 
     def __call__(self, x: torch.Tensor, out_dtype: torch.dtype = torch.float32,
                  scale: torch.Tensor | None = None) -> torch.Tensor:
-        """x (rows, k) float32, float16 or bfloat16; or int8 with the rows' scales.  Returns (rows, channels)."""
+        """x (rows, k) float32, float16 or bfloat16; or int8 with the rows' scales.  Returns (rows, channels).  Not
+        differentiable: a backward pass through the outputs raises."""
+        if _hip.tracked(x) or (scale is not None and _hip.tracked(scale)):
+            return _hip.undifferentiated("Int8Linear", lambda: self(x, out_dtype, scale), x, scale)
         x, ld = _rows(x, "Int8Linear")
         rows, k = x.shape
         dev = x.device
