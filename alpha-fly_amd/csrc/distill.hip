@@ -11,6 +11,7 @@
 //              dL/dz_j = T (q_j - p_j) on S,  T exp(z_j / T - lse_rest) (q_t - p_t) outside.
 //            q_t is summed over the rest itself, never as 1 - sum q.
 // Rows, maxima and sums are float32 whatever the logits' type; gradients round once, on their store.
+#include "row_rules.hpp"
 #include "rows.hpp"
 
 namespace fly {
@@ -98,8 +99,6 @@ struct Row {
       for (int e = 0; e < N; ++e) f(element<T>(p, e), i * N + e);
     });
   }
-  // waves that hold whole pieces
-  __device__ __forceinline__ int holders() const { return min((int)blockDim.x >> 6, max(1, (full + 63) >> 6)); }
   // f(j, piece number, piece) for this thread's pieces, columns that do not exist at -inf; j = -1 for the last one where it
   // is not whole (a constant after inlining)
   template <typename F>
@@ -140,33 +139,8 @@ struct Spread {
   }
   template <typename F>
   __device__ __forceinline__ void values_wave(F &&f) { values(f); }
-  __device__ __forceinline__ int holders() const { return min((int)blockDim.x >> 6, (cols + 63) >> 6); }
   __device__ __forceinline__ void forget() {}
 };
-
-// How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
-// threads cover a row with.  From 1,024 rows on (4 for each CU) at least `many`, since what a wave does once per row weighs
-// more than the waves that are left idle: 8 for the top logits (1,500 x 4,168 float32 12.1 us with 8, 14.7 with 4), 4 for
-// the distillation, whose 8 cost it registers (with gradient: 16,384 x 4,168 float16 57 us with 4, 63 with 8, 82 with 2;
-// float32 103, 113 with 8; 16,384 x 1,000 float32 28.7, 35.4 with 8).  Past 512 threads 1,024 of them, as two workgroups of
-// 16 waves fill a CU evenly (8 pieces: 2,048 x 50,256 95 us, with the 832 threads that it needs 110).  For many rows that is
-// where `many` pieces need them (distillation, 4 pieces on 1,024 threads against 8 on 512: 4,096 x 32,000 bfloat16 105 us
-// against 112 with gradient, 61 against 59 without; 4,096 x 12,000 float32 77 against 82), for few only where 8 do (256 x
-// 12,000 float32 with 4 13.0 us, with 8 11.4).  Longer rows are read at every pass (kept = 0).  Loss and gradient take the
-// same shape, so the loss has the same bits with the gradient and alone.
-struct RowShape {
-  int kept, threads;
-};
-RowShape row_shape(int64_t rows, int64_t cols, size_t elem, int least, int many) {
-  const int64_t pieces = (cols * (int64_t)elem + 15) / 16;   // whole ones at most
-  for (int kept : {1, 2, 4, 8}) {
-    const int64_t threads = std::max<int64_t>(round_up((pieces + kept - 1) / kept, 64), least);
-    const bool enough = kept >= many;
-    if (threads <= 512 && (enough || rows < 1024)) return {kept, (int)threads};
-    if (threads <= 1024 && (kept == 8 || (enough && rows >= 1024))) return {kept, 1024};
-  }
-  return {0, 1024};
-}
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kMostFloat = 3.4028234663852886e38f;
 
@@ -186,7 +160,7 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
-constexpr int kMostCandidates = 1024, kWaveCandidates = 128;
+constexpr int kMostCandidates = 1024;
 
 // What a workgroup of k_top keeps in LDS besides these, 128 entries for each wave (at most 1,024 in the first): the joined
 // list, and the waves' own lists, whose place a histogram and the candidates that are not listed (`spare`, by rank) take
@@ -342,16 +316,16 @@ __device__ __forceinline__ PartSum top_by_digits(TopShared &s, uint64_t *list, u
 
 // One workgroup per row.  A bound from below: with W waves and c = ceil(K / W), the least over the waves of a logit that each
 // has c at or above has at least K at or above it.  A wave takes the c-th largest of its lanes' largest (it holds the row
-// interleaved, so few more than c logits pass it), or of all its logits (EXACT) where c is most of the lanes.  What passes
-// is packed by ballots, without atomics, into the wave's list in LDS, and the lists are joined and ranked.  NaN passes
-// every bound.  Lists that would not fit (ties) are left to top_by_digits.
+// interleaved, so few more than c logits pass it), or of all its logits (EXACT) where c is most of the lanes; a last wave
+// of few lanes does not count (top_shape).  What passes is packed by ballots, without atomics, into the wave's list in LDS,
+// and the lists are joined and ranked.  NaN passes every bound.  Lists that would not fit (ties) are left to top_by_digits.
 // Bound by the row's bytes where k is small (4,096 x 32,000 bfloat16: k = 8 59 us, k = 64 64 us, 51 us at the rate of a copy),
 // by the instructions per candidate where it is not (k = 256 91 us).
 template <typename T, typename R, bool EXACT>
 __global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top(const T *__restrict__ z, int64_t ldz,
                                               int64_t cols,
-                                              const uint8_t *__restrict__ legal, int64_t ldl, int k, float inv_t,
-                                              float *__restrict__ values, int32_t *__restrict__ index,
+                                              const uint8_t *__restrict__ legal, int64_t ldl, int k, int holders,
+                                              float inv_t, float *__restrict__ values, int32_t *__restrict__ index,
                                               float *__restrict__ tail) {
   __shared__ TopShared s;
   extern __shared__ uint64_t lists[];
@@ -361,7 +335,7 @@ __global__ __launch_bounds__(1024, sizeof(R) > 128 && !EXACT ? 8 : 4) void k_top
   const T *zr = z + r * ldz;
   const uint8_t *seen = legal ? legal + r * ldl : nullptr;
   R row(zr, seen, (int)cols);
-  const int holders = row.holders(), c = (k + holders - 1) / holders, most = top_list(waves);
+  const int c = (k + holders - 1) / holders, most = top_list(waves);
   uint64_t *list = lists;
   float2 *found = reinterpret_cast<float2 *>(lists + most);
   float top = -INFINITY;   // NaN where the lane has one
@@ -729,24 +703,21 @@ extern "C" int fly_top_logits(const void *z, int32_t type, int64_t ldz, int64_t 
     by_type(type, [&](auto t) {
       using T = decltype(t);
       if (!rows) return;
-      // Twice as many lanes as k (16,384 x 4,168 float16, k = 200: 204 us against 214 with as many; 4,000 x 20,000 74
-      // against 181).  A row too short to give half of them a piece is spread over 4 waves column by column.
-      const int least = (int)round_up(2 * k, 64), full = (int)(cols * (int64_t)sizeof(T) / 16);
+      const TopShape shape = top_shape(rows, cols, sizeof(T), k);
       auto run = [&](auto kernel, int threads) {
         const int waves = threads / 64;
         in_slices(rows, threads, [&](int64_t r, int64_t n) {
           hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(threads), 8 * (size_t)(top_list(waves) + waves * kWaveCandidates),
                              as_stream(stream), static_cast<const T *>(z) + r * ldz, ldz, cols, legal ? legal + r * ldl : nullptr,
-                             ldl, k, 1.0f / temperature, values + r * k, index + r * k, tail ? tail + r : nullptr);
+                             ldl, k, shape.holders, 1.0f / temperature, values + r * k, index + r * k,
+                             tail ? tail + r : nullptr);
           check_launch("top logits");
         });
       };
-      const RowShape shape = row_shape(rows, cols, sizeof(T), least, 8);
-      const int holders = std::min(shape.threads / 64, std::max(1, (full + 63) / 64));
-      if (k > 32 * holders && cols <= 1024) run(k_top<T, Spread<T, 4>, true>, 256);
-      else if (k > 32 * holders && cols <= 4096) run(k_top<T, Spread<T, 16>, true>, 256);
+      if (shape.spread == 4) run(k_top<T, Spread<T, 4>, true>, 256);
+      else if (shape.spread == 16) run(k_top<T, Spread<T, 16>, true>, 256);
       else
-        by_shape(shape, [&](auto nv, auto res, int threads) {
+        by_shape(shape.row, [&](auto nv, auto res, int threads) {
           run(k_top<T, Row<T, decltype(nv)::value, decltype(res)::value>, false>, threads);
         });
     });
