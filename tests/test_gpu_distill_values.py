@@ -121,3 +121,70 @@ def test_temperatures_whose_square_leaves_the_range(temperature):
 def test_a_teacher_whose_scaled_logits_leave_the_range():
     z, (values, index, _) = _logits(4, 4168, 3, scale=0.3), _teacher(4, 4168, 8, 5, 1.0)
     _check_distill(z, (values / 10 + 10, index, None), 2e-38)
+
+
+LENGTHS = [37, 300, 4168, 16390, 33000, 70000]
+
+
+@pytest.mark.parametrize("cols", LENGTHS)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_top_of_odd_values_row_by_row(cols, dtype):
+    low = torch.finfo(dtype).min
+    z = _logits(10, cols, 3, dtype)
+    z[0] = -INF
+    z[1] = low
+    z[2, ::3] = low
+    z[3, ::2] = -INF
+    z[4, 5] = INF
+    z[5, [2, 9]] = float("nan")
+    z[6] = -INF
+    z[6, 11] = 2.0
+    z[7] = torch.finfo(dtype).tiny
+    z[7, 3] = -torch.finfo(dtype).tiny
+    z[8] = -low
+    z[9, 1::2] -= 1000
+    for k, legal in ((1, None), (4, None), (30, _mask(10, cols, 4, 0.5)), (256, None)):
+        _check_top(z, k, 1.0, legal)
+        _check_top(z, k, 3.0, legal)
+
+
+@pytest.mark.parametrize("cols", LENGTHS)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_distill_odd_values_row_by_row(cols, dtype):
+    low = torch.finfo(dtype).min
+    values, index, tail = _teacher(16, cols, 6, 3, 1.0)
+    z = _logits(16, cols, 4, dtype)
+    z[0] = -INF                                  # the student sees nothing
+    z[1] = low
+    z[2, ::3] = low
+    z[3] = -INF
+    z[3, index[3, 0].item()] = 1.0               # nothing but one listed move
+    z[4, index[4, 1].item()] = -INF              # the teacher's move is impossible: infinite loss, finite gradient
+    z[5, (index[5, 0].item() + 1) % cols] = float("nan")
+    index[6] = -1                                # nothing listed: the tail alone
+    index[7, 1:] = -1
+    index[8, 0], index[8, 2] = -1, -5
+    values[9, 3:] = -INF                         # listed, of no probability
+    tail[10] = -INF
+    z[11] += 40.0
+    z[12], z[13] = -low, 0.0
+    values[14] = torch.finfo(torch.float32).min  # the teacher lists what it masks
+    values[15, 2:] = torch.finfo(torch.float32).min
+    _check_distill(z, (values, index, tail))
+    _check_distill(z, (values, index, None), 2.0)
+    _check_distill(z, (values, index, tail), 1.0, _mask(16, cols, 3, 0.5))
+
+
+def test_each_row_is_scaled_by_its_own_upstream_gradient():
+    """Bit for bit the gradient that a factor for each row gives, and not the first row's factor."""
+    from chessfly.distill import TopLogits, distill_loss, distill_loss_and_grad
+    z, up = _logits(9, 700, 3).to(DEV), torch.linspace(-1.5, 2.0, 9).to(DEV)
+    teacher = TopLogits(*map(_dev, _teacher(9, 700, 12, 5, 1.0)))
+    leaf = z.clone().requires_grad_(True)
+    distill_loss(leaf, teacher, reduction="none").backward(up)
+    assert torch.equal(leaf.grad, distill_loss_and_grad(z, teacher, row_scale=up)[1])
+    one = torch.zeros(9, device=DEV)
+    one[4] = 1.0
+    leaf.grad = None
+    distill_loss(leaf, teacher, reduction="none").backward(one)
+    assert bool((leaf.grad[torch.arange(9, device=DEV) != 4] == 0).all()) and bool((leaf.grad[4] != 0).any())
