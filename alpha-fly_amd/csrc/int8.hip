@@ -225,10 +225,11 @@ __device__ __forceinline__ void int8_tile(int tiles, int mt, int nt, int &m, int
 template <int N>
 using Stages = std::integral_constant<int, N>;
 
-// WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.  Large
-// products are bound by the matrix cores at the clock that random operands leave them: 16,384 rows of 2,333 into 4,168 run
-// at 1.79e15 operations a second, 178 us, and the main loop alone on a long k at 2.83e15 (3.52e15 with constant operands).
-// Small ones are bound by the tiles' chain of loads, products and stores: 1,120 rows 20 us, where the bytes take 7.6.
+// WN x WM waves, each FN x FM blocks of channels x tokens; S stages of one block of k in LDS, loaded S - 1 ahead.  16,384 rows
+// of 2,333 into 4,168 run at 1.79e15 operations a second, 178 us.  The main loop alone on a long k reaches 2.83e15 with random
+// operands, by the matrix cores' clock (3.52e15 with constant ones): 113 of the 178 us.  The other 65 are the tiles' filling,
+// emptying and stores, which only the CU's second workgroup covers.  Small products are bound by that chain alone: 1,120
+// rows 20 us, where the bytes take 7.6.
 template <typename T, int WN, int WM, int FN, int FM, int S>
 __global__ __launch_bounds__(64 * WN * WM) void k_int8_gemm(const int4v *__restrict__ w, const int4v *__restrict__ q,
                                                             const float *__restrict__ row_scale,
@@ -394,9 +395,9 @@ void int8_gemm(const fly_int8 &p, const int4v *q, const float *row_scale, int64_
 // Few rows, R blocks of 16 of them: a workgroup has C blocks of 16 channels, 4 waves for each, and a wave every fourth block
 // of k, whose weights go straight from memory to the matrix cores; the waves' integer sums meet in LDS.  The work is the
 // weights' way here, so their loads go first.  X = void: the rows come quantised from the workspace.  Else every workgroup
-// quantises them for itself, a wave per row, while its weights are on their way: one launch, and no workspace.  C = 1 up to 8
-// rows, 261 workgroups for 4,168 channels (8 rows of 2,333 8.4 us, C = 4 9.0); C = 4 past that, whose 16 waves share the rows
-// (16 rows 10.5 us against 11.9).
+// quantises them for itself, a wave per row, while its weights are on their way: one launch, and no workspace.  C = 1 up to 4
+// rows, one for each wave, 261 workgroups for 4,168 channels (1 row of 2,333 4.9 us, C = 4 5.2; 4 rows of 3,000 into 500 4.9
+// against 5.3); C = 4 past that, whose 16 waves share the rows (8 rows of 2,333 6.0 us against 7.1, 16 rows 7.7 against 10.3).
 template <typename X, typename T, int C, int R>
 __global__ __launch_bounds__(256 * C) void k_int8_few(const int4v *__restrict__ w, const void *__restrict__ in, int64_t ldx,
                                                       const float *__restrict__ row_scale,
@@ -535,9 +536,9 @@ size_t int8_ws(const fly_int8 &p, int64_t rows) {
 
 // Whether a call quantises its rows in the product itself (k_int8_few): up to 32 rows of at most 3,072 columns (a wave's
 // registers; 96 KB of blocks) into at most 8,192 channels, over which every workgroup repeats the work.  Measured, us of the
-// kernels against the two of the other path: 4,168 channels over 2,333: 1 row 6.0 against 9.5, 8 rows 8.4 against 10, 16
-// rows 10.5 against 11.5, 32 rows 13.8 against 13.2; the second launch costs the host another 4.  17,937 channels over 838:
-// 1 row 12.8 against 9.9.
+// kernels in a graph against the two of the other path: 4,168 channels over 2,333: 1 row 4.9 against 8.6, 8 rows 6.0 against
+// 8.9, 16 rows 7.7 against 9.6, 32 rows 10.6 against 12.3; the second launch costs the host another 4.  17,937 channels over
+// 838: 1 row 7.1 against 5.9, 16 rows 11.3 against 7.0; 12,000 channels 1 row 4.5 against 5.9, 32 rows 8.8 against 8.1.
 bool quantises_few(const fly_int8 &p, int32_t x_type, int64_t rows) {
   return x_type != FLY_I8 && rows <= 32 && p.nb <= 512 && p.kb <= kFewSpan;
 }
@@ -648,7 +649,7 @@ extern "C" int fly_int8_linear(const fly_int8 *p, const void *x, int32_t x_type,
         by_float(x_type, "", [&](auto xt) {
           using X = decltype(xt);
           T *out = static_cast<T *>(y);
-          if (rows <= 8) int8_few<X, T, 1, 1>(*p, x, ldx, nullptr, rows, out, ldy, st);
+          if (rows <= 4) int8_few<X, T, 1, 1>(*p, x, ldx, nullptr, rows, out, ldy, st);
           else if (rows <= 16) int8_few<X, T, 4, 1>(*p, x, ldx, nullptr, rows, out, ldy, st);
           else int8_few<X, T, 4, 2>(*p, x, ldx, nullptr, rows, out, ldy, st);
         });
