@@ -492,7 +492,7 @@ int fly_int8_linear(const fly_int8 *plan, const void *x_dev, int32_t x_type, int
  *
  * fly_top_logits: values and index (rows, k): the k largest logits in falling order, the lower column first among
  * equals (NaN above all), padded with -inf and -1; tail (rows) or NULL: log sum exp(z / temperature) over the columns
- * not listed, -inf when there are none.
+ * not listed, -inf when there are none (NaN where +inf or NaN is not listed, so only in a row of more than k of them).
  *
  * fly_distill: from values, index (rows, k) and tail (rows; NULL: the teacher is its list alone) the loss (rows) and its
  * gradient by z, either NULL: temperature^2 times the Kullback-Leibler divergence from the teacher's softmax to the
