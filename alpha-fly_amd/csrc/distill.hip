@@ -463,8 +463,8 @@ __device__ __forceinline__ float divergence(float logp, float p, float logq, flo
 
 // One workgroup per row.  The first waves hold the list and compute the row's scalars; the others wait for the factor of
 // their exponentials, so what does not depend on the columns is computed once and not by every wave.  Bound by the row's
-// bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 57 us, 4.8 TB/s of the 5.1 that a copy
-// reaches; 2,048 x 50,256 bfloat16 96 us, 4.3 TB/s; x 50,257, whose rows' pieces lie across the lines, 104 us), by a row's
+// bytes in and out where there are rows to fill the chip (16,384 x 4,168 float16 58 us, 4.7 TB/s of the 5.1 that a copy
+// reaches; 2,048 x 50,256 bfloat16 96 us, 4.3 TB/s; x 50,257, whose rows' pieces lie across the lines, 105 us), by a row's
 // chain of load, two reductions, list and store where there are few (256 x 4,168 float32 7.2 us).
 template <typename T, int NV, bool RES>
 __global__ __launch_bounds__(1024, NV == 8 ? 8 : 4) void k_distill(const DistillArgs<T> a) {

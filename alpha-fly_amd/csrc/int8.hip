@@ -555,7 +555,7 @@ void int8_few(const fly_int8 &p, const void *x, int64_t ldx, const float *row_sc
 }
 
 // The product of rows in blocks.  Measured, us of the product (2,333 into 4,168 where nothing else is said):
-// * up to 16 rows, a workgroup for each 16 channels (k_int8_few): 16 rows 5.9;
+// * up to 16 rows, a workgroup for each 16 channels (k_int8_few): 16 rows 5.2;
 // * tiles of 64 x 64 while there are at most 512 of them: 384 rows 12.0 against 13.5 (128 x 128), 1,120 rows of 200 into 500
 //   4.2 against 5.4; but 512 rows 14.7 against 13.5;
 // * 128 x 128 while there are at most 256, one for each CU: 600 rows 14.0 against 17.6 (192 x 128); but 900 rows 20.2 against

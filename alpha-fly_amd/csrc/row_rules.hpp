@@ -12,11 +12,11 @@ namespace fly {
 // How many pieces a thread keeps and how many threads a row gets.  Few rows: the fewest of {1, 2, 4, 8} pieces that 512
 // threads cover a row with.  From 1,024 rows on (4 for each CU) at least `many`, since what a wave does once per row weighs
 // more than the waves that are left idle: 8 for the top logits (1,500 x 4,168 float32 12.1 us with 8, 14.7 with 4), 4 for
-// the distillation, whose 8 cost it registers (with gradient: 16,384 x 4,168 float16 57 us with 4, 63 with 8, 82 with 2;
-// float32 103, 113 with 8; 16,384 x 1,000 float32 28.7, 35.4 with 8).  Past 512 threads 1,024 of them, as two workgroups of
-// 16 waves fill a CU evenly (8 pieces: 2,048 x 50,256 95 us, with the 832 threads that it needs 110).  For many rows that is
-// where `many` pieces need them (distillation, 4 pieces on 1,024 threads against 8 on 512: 4,096 x 32,000 bfloat16 105 us
-// against 112 with gradient, 61 against 59 without; 4,096 x 12,000 float32 77 against 82), for few only where 8 do (256 x
+// the distillation, whose 8 cost it registers (with gradient: 16,384 x 4,168 float16 57 us with 4, 64 with 8, 77 with 2;
+// float32 100, 112 with 8; 16,384 x 1,000 float32 26.6, 30.6 with 8).  Past 512 threads 1,024 of them, as two workgroups of
+// 16 waves fill a CU evenly (8 pieces: 2,048 x 50,256 95 us, with the 832 threads that it needs 111).  For many rows that is
+// where `many` pieces need them (distillation, 4 pieces on 1,024 threads against 8 on 512: 4,096 x 32,000 bfloat16 102 us
+// against 110 with gradient, but 58 against 47 without; 4,096 x 12,000 float32 76 against 82), for few only where 8 do (256 x
 // 12,000 float32 with 4 13.0 us, with 8 11.4).  Longer rows are read at every pass (kept = 0).  Loss and gradient take the
 // same shape, so the loss has the same bits with the gradient and alone.
 struct RowShape {
