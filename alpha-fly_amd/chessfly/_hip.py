@@ -107,6 +107,11 @@ SIGNATURES = {
     "fly_int8_linear": (_i32, [_p, _p, _i32, _i64, _p, _i64, _p, _i32, _i64, _p, _sz, _p]),
     "fly_top_logits": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _f32, _p, _p, _p, _p]),
     "fly_distill": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i32, _f32, _p, _p, _i64, _p, _f32, _p]),
+    "fly_readout_loss_workspace": (_sz, [_i32, _i64, _i64, _i64, _i32]),
+    "fly_readout_loss": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _p, _i64, _p, _i32, _p, _i32, _p, _p,
+                                _f32, _p, _i64, _p, _i64, _p, _p, _sz, _p]),
+    "fly_clip_workspace": (_sz, [_p, _p, _i64]),
+    "fly_clip_gradients": (_i32, [_p, _p, _p, _i64, _i32, _f32, _p, _p, _sz, _p]),
     "fly_profile_enable": (_i32, [_i32]),
     "fly_profile_read": (_i32, [_p, _p]),
     "fly_profile_launches": (_i64, [_p, _p, _i64]),
@@ -218,6 +223,34 @@ def undifferentiated(what: str, run, *tensors):
     if any(t is not None and tracked(t) and not t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative")
     return _NoBackward.apply(what, run, *tensors)
+
+
+_STREAM, _PROBE = "chessfly.stream", "chessfly.probe"
+
+
+def held_leaves(what: str, *tensors) -> list:
+    """The autograd nodes that collect the gradients of the leaves among the tensors, to be kept until an operator has taken
+    them.  A leaf has one such node while any graph of it lives, and the backward pass waits for the stream that was current when
+    it was made.  In a captured backward pass a wait for a stream outside the capture ends the process, so a leaf whose node an
+    eager call has made, and whose graph still lives, is refused while its stream is captured."""
+    nodes = []
+    for t in tensors:
+        if t is None or not (t.requires_grad and t.is_leaf):
+            continue
+        node = torch.autograd.graph.get_gradient_edge(t).node
+        here, made = _raw_stream(t.device.index), node.metadata.get(_STREAM)
+        if made is None:
+            # whether it was there before: a new one goes with its last reference
+            node.metadata[_PROBE] = True
+            del node
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            if node.metadata.pop(_PROBE, None) is None:
+                node.metadata[_STREAM] = here
+        elif made != here and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what}: a graph of a leaf made outside this capture is still alive: drop its results before "
+                               "capturing, or capture on its stream")
+        nodes.append(node)
+    return nodes
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

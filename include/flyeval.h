@@ -75,7 +75,7 @@ enum fly_mode {
 };
 
 /* Element types of the entry points that take more than one. */
-enum fly_type { FLY_F32 = 0, FLY_F16 = 1, FLY_BF16 = 2, FLY_I8 = 3 };
+enum fly_type { FLY_F32 = 0, FLY_F16 = 1, FLY_BF16 = 2, FLY_I8 = 3, FLY_I32 = 4, FLY_I64 = 5 };
 
 typedef struct fly_cone fly_cone;
 typedef struct fly_plan fly_plan;
@@ -509,6 +509,38 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
                 int64_t ldl, const float *values_dev, const int32_t *index_dev, const float *tail_dev, int32_t k,
                 float temperature, float *loss_dev, void *grad_dev, int64_t ldg, const float *row_scale_dev,
                 float grad_scale, void *stream);
+
+/* ---- a read-out's softmax cross entropy, and its gradients ---------------------------------------- */
+/* No counterpart in the reference, whose training takes torch's softmax over kept logits.  Logits z = x w^T + bias of x (rows,
+ * ldx) and w (v, ldw), both of `type` over d columns (d 1 to 2^16, v 1 to 2^20), bias of bias_type (v) or NULL; legal (rows, ldl)
+ * bytes, NULL or 0 for columns that do not exist for the row.  Targets: index (rows, k) FLY_I32 or FLY_I64 with weight (rows, k)
+ * float32, NULL for 1; k 1 to 1024.  A negative index, a weight of 0 and a column that does not exist are left out; those of a
+ * column listed twice add up; an index at or past v makes the row NaN.  With a over the entries that are left:
+ *   loss[r] = sum_j a_rj (log sum exp z_r - z_r,t_rj), 0 of a row with none;  any of loss, gx, gw, gb may be NULL
+ *   gx (rows, ldgx), gw (v, ldgw) of `type` and gb (v) of bias_type: grad_scale times the gradient of sum_r row_scale[r] loss[r]
+ *   (row_scale NULL: 1) by x, w and bias; of no rows they are 0.
+ * Sums are float32; float32 operands are multiplied as two float16 each, 22 bits.  The workspace, 256-byte aligned, holds both
+ * operands laid out and logits of as many rows as fit 2 GiB; it depends on `wanted`, the gradients that are not NULL.  The
+ * outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums, but for rows of
+ * x without a target, which count as zeros whatever they hold. */
+enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };
+size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t wanted);
+int fly_readout_loss(const void *x_dev, int32_t type, int64_t ldx, int64_t rows, int64_t d, const void *w_dev, int64_t ldw,
+                     int64_t v, const void *bias_dev, int32_t bias_type, const uint8_t *legal_dev, int64_t ldl,
+                     const void *index_dev, int32_t index_type, const float *weight_dev, int32_t k, float *loss_dev,
+                     const float *row_scale_dev, float grad_scale, void *gx_dev, int64_t ldgx, void *gw_dev, int64_t ldgw,
+                     void *gb_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* ---- the norm of many gradients, and clipping by it ---------------------------------------------- */
+/* grads, sizes (elements) and types (FLY_F32, FLY_F16 or FLY_BF16) are host arrays of n; the gradients are contiguous device
+ * memory at their elements' alignment.  norm (device, one float) = sqrt(sum of squares) or max |g| over all of them, summed in
+ * float64; 0 of none.  limit >= 0: the gradients are then scaled in place by limit / (norm + 1e-6) where that is below 1 (NaN
+ * where the norm is NaN), each product rounded once; else they stay as they are and must not overlap then.  limit < 0: the norm
+ * alone.  The workspace is 8-byte aligned; results depend on sizes and values alone, not on scheduling. */
+enum fly_norm { FLY_NORM_MAX = 0, FLY_NORM_2 = 2 };
+size_t fly_clip_workspace(const int64_t *sizes, const int32_t *types, int64_t n);
+int fly_clip_gradients(void *const *grads, const int64_t *sizes, const int32_t *types, int64_t n, int32_t norm_kind,
+                       float limit, float *norm_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 
 /* ---- measurement ------------------------------------------------------------------------------- */
 
