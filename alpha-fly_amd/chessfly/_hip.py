@@ -107,7 +107,7 @@ SIGNATURES = {
     "fly_int8_linear": (_i32, [_p, _p, _i32, _i64, _p, _i64, _p, _i32, _i64, _p, _sz, _p]),
     "fly_top_logits": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i32, _f32, _p, _p, _p, _p]),
     "fly_distill": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i32, _f32, _p, _p, _i64, _p, _f32, _p]),
-    "fly_readout_loss_workspace": (_sz, [_i32, _i64, _i64, _i64, _i32]),
+    "fly_readout_loss_workspace": (_sz, [_i32, _i64, _i64, _i64, _i32, _i32]),
     "fly_readout_loss": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _p, _i64, _p, _i32, _p, _i32, _p, _p,
                                 _f32, _p, _i64, _p, _i64, _p, _p, _sz, _p]),
     "fly_clip_workspace": (_sz, [_p, _p, _i64]),

@@ -93,11 +93,12 @@ def _run(c: _Call, loss, row_scale, grad_scale: float, want: tuple[bool, bool, b
     gw = torch.empty(cols, d, dtype=c.x.dtype, device=dev) if want[1] else None
     gb = torch.empty(cols, dtype=c.bias.dtype, device=dev) if want[2] else None
     kind, wanted = FLOATS[c.x.dtype], want[0] + 2 * want[1] + 4 * want[2]
-    need = _hip.load().fly_readout_loss_workspace(kind, rows, d, cols, wanted)
+    k = c.share.shape[1] if c.share is not None else 1
+    need = _hip.load().fly_readout_loss_workspace(kind, rows, d, cols, k, wanted)
     ws = _hip.workspace(need, dev)
     _hip.call("fly_readout_loss", dev.index, c.x.data_ptr(), kind, c.ldx, rows, d, c.weight.data_ptr(), c.ldw, cols,
               _hip.ptr(c.bias), FLOATS[c.bias.dtype] if c.bias is not None else 0, _hip.ptr(c.legal), c.ldl,
-              c.index.data_ptr(), INDEX[c.index.dtype], _hip.ptr(c.share), c.share.shape[1] if c.share is not None else 1,
+              c.index.data_ptr(), INDEX[c.index.dtype], _hip.ptr(c.share), k,
               _hip.ptr(loss), _hip.ptr(row_scale), grad_scale, _hip.ptr(gx), d, _hip.ptr(gw), d, _hip.ptr(gb), ws.data_ptr(),
               need)
     return ReadoutGrads(gx, gw, gb)

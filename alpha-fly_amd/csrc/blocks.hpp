@@ -83,30 +83,47 @@ using Ahead = std::integral_constant<int, N>;
 struct Blocks {
   const int4v *a, *b;
   int na, mb, kb;       // blocks of n, of m and of k
+  int splits;           // parts of k, each a job of its own
   int tiles, mt, nt;    // filled in at the launch
 };
 
+// The products of one launch, side by side: what one of them leaves idle at its end, the next one takes.
+template <typename EP, int COUNT>
+struct Products {
+  Blocks of[COUNT];
+  EP ep[COUNT];
+};
+
 // WN x WM waves, each FN x FM blocks of n x m; S stages of one block of k in LDS, loaded S - 1 ahead.  `ep` takes each wave's
-// sums: ep.tile<FN, FM>(acc, m0, n0, lane, part) with a wave's m0 and n0 in rows, its column part, and 16 rows x 16 FN
-// floats of LDS of its own to turn them over in.
-template <typename H, int P, int WN, int WM, int FN, int FM, int S, typename EP>
-__global__ __launch_bounds__(64 * WN * WM) void k_blocks(const Blocks o, const EP ep) {
+// sums: ep.tile<FN, FM>(acc, m0, n0, lane, part, split, turn) with a wave's m0 and n0 in rows, its column part, its part of k, and
+// 16 rows x 16 FN floats of LDS of its own to turn them over in.
+template <typename H, int P, int WN, int WM, int FN, int FM, int S, typename EP, int COUNT>
+__global__ __launch_bounds__(64 * WN * WM) void k_blocks(const Products<EP, COUNT> products) {
   constexpr int WAVES = WN * WM, BN = WN * FN, BM = WM * FM, ALL = (BN + BM) * P;
   constexpr int LOADS = (ALL + WAVES - 1) / WAVES;
   constexpr int FEWER = (WAVES - ALL % WAVES) % WAVES;   // waves with one load less
   constexpr int READS = (FN + FM) * P < 15 ? (FN + FM) * P : 15;
   __shared__ __attribute__((aligned(16))) int4v lds[S][ALL][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int index = blockIdx.x, which = 0;
+  if constexpr (COUNT > 1)
+    while (index >= products.of[which].tiles * products.of[which].splits) {
+      index -= products.of[which].tiles * products.of[which].splits;
+      ++which;
+    }
+  const Blocks &o = products.of[which];
+  const int split = index / o.tiles, k0 = (int)((int64_t)o.kb * split / o.splits);
   int tm, tn;
-  block_tile(blockIdx.x, o.tiles, o.mt, o.nt, tm, tn);
-  const int n0 = tn * BN, m0 = tm * BM, wn = wave % WN, wm = wave / WN, kb = o.kb;
+  block_tile(index - split * o.tiles, o.tiles, o.mt, o.nt, tm, tn);
+  const int n0 = tn * BN, m0 = tm * BM, wn = wave % WN, wm = wave / WN;
+  const int kb = (int)((int64_t)o.kb * (split + 1) / o.splits) - k0;
   const int4v *src[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     // blocks past the operands' ends load their last one, whose products go nowhere
     const int at = min(wave + i * WAVES, ALL - 1), b = at / P;
-    src[i] = (b < BN ? o.a + (int64_t)min(n0 + b, o.na - 1) * kb * P * 64
-                     : o.b + (int64_t)min(m0 + b - BN, o.mb - 1) * kb * P * 64) + (at % P) * 64 + lane;
+    src[i] = (b < BN ? o.a + ((int64_t)min(n0 + b, o.na - 1) * o.kb + k0) * P * 64
+                     : o.b + ((int64_t)min(m0 + b - BN, o.mb - 1) * o.kb + k0) * P * 64) + (at % P) * 64 + lane;
   }
   const bool fewer = FEWER > 0 && wave >= WAVES - FEWER;
   auto load = [&](int s) {
@@ -215,7 +232,7 @@ __global__ __launch_bounds__(64 * WN * WM) void k_blocks(const Blocks o, const E
       sum[j][i] = acc[j][i][0];
       if constexpr (P == 2) sum[j][i] += acc[j][i][1] * kLow;
     }
-  ep.template tile<FN, FM>(sum, 16 * (m0 + wm * FM), 16 * (n0 + wn * FN), lane, tn * WN + wn,
+  products.ep[which].template tile<FN, FM>(sum, 16 * (m0 + wm * FM), 16 * (n0 + wn * FN), lane, tn * WN + wn, split,
                            reinterpret_cast<float *>(lds) + wave * TURN);
 }
 
@@ -236,13 +253,17 @@ __device__ __forceinline__ void turn_over(const float4v (&v)[FN], float *turn, i
   asm volatile("" ::: "memory");
 }
 
-template <typename H, int P, int WN, int WM, int FN, int FM, int S, typename EP>
-void launch_blocks(Blocks o, const EP &ep, hipStream_t st) {
-  o.mt = (o.mb + WM * FM - 1) / (WM * FM);
-  o.nt = (o.na + WN * FN - 1) / (WN * FN);
-  FLY_REQUIRE((int64_t)o.mt * o.nt < (int64_t)1 << 32 >> 9, "product too large");   // at up to 512 threads
-  o.tiles = o.mt * o.nt;
-  hipLaunchKernelGGL((k_blocks<H, P, WN, WM, FN, FM, S, EP>), dim3(o.tiles), dim3(64 * WN * WM), 0, st, o, ep);
+template <typename H, int P, int WN, int WM, int FN, int FM, int S, typename EP, int COUNT>
+void launch_blocks(Products<EP, COUNT> p, hipStream_t st) {
+  int64_t all = 0;
+  for (Blocks &o : p.of) {
+    o.mt = (o.mb + WM * FM - 1) / (WM * FM);
+    o.nt = (o.na + WN * FN - 1) / (WN * FN);
+    o.tiles = o.mt * o.nt;
+    all += (int64_t)o.mt * o.nt * o.splits;
+  }
+  FLY_REQUIRE(all < (int64_t)1 << 32 >> 10, "product too large");   // at up to 1,024 threads
+  hipLaunchKernelGGL((k_blocks<H, P, WN, WM, FN, FM, S, EP, COUNT>), dim3((unsigned)all), dim3(64 * WN * WM), 0, st, p);
   check_launch("product of blocks");
 }
 

@@ -22,12 +22,13 @@ constexpr int64_t kPieceRows = (int64_t)1 << 19;    // a piece at most: tiles of
 struct Maxima {
   uint32_t weight, row;
 };
+// Raises *to to a finite v.  A look first: thousands of rows' factors are alike, and as many atomics on one address took 12 ns
+// each.
 __device__ __forceinline__ void raise(uint32_t *to, float v) {
-  if (v > 0.0f && v <= 3.4028234663852886e38f) atomicMax(to, __float_as_uint(v));
+  if (v > 0.0f && v <= 3.4028234663852886e38f &&
+      __float_as_uint(v) > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+    atomicMax(to, __float_as_uint(v));
 }
-
-__global__ void k_clear(Maxima *m) { *m = Maxima{0u, 0u}; }
-__global__ void k_clear_row(Maxima *m) { m->row = 0u; }
 
 // ---- targets ---------------------------------------------------------------------------------------------------------
 
@@ -52,6 +53,58 @@ __device__ __forceinline__ int target_of(const Targets &t, int64_t row, int j, f
   return t.legal && !t.legal[row * t.ldl + c] ? -1 : (int)c;
 }
 
+// A row's targets as the later kernels take them: each column once (-1: none) with its weights added up, and over the row the sum
+// of the weights and of their sizes.
+struct List {
+  int *column;      // (row, k)
+  float *weight;
+  float *logit;     // filled in by the product
+  float2 *sums;     // (row)
+  int k;
+};
+
+// By a wave; whether any target counts.
+__device__ __forceinline__ bool list_row(const Targets &t, const List &l, int64_t row, int lane) {
+  float share = 0.0f, whole = 0.0f;
+  bool some = false;
+  for (int first = 0; first < t.k; first += 64) {
+    const int j = first + lane;
+    float a = 0.0f;
+    int c = j < t.k ? target_of(t, row, j, a) : -1;
+    some |= c != -1;
+    if (c == -2) share = whole = __builtin_nanf("");
+    if (c < 0) a = 0.0f;
+    share += a;
+    whole += fabsf(a);
+    float sum = a;
+    bool again = c < 0;
+    if (t.k > 1)
+      for (int other = 0; other < t.k; other += 64) {
+        float b = a;
+        int d = c;
+        if (other != first) {
+          d = other + lane < t.k ? target_of(t, row, other + lane, b) : -1;
+          if (d < 0) b = 0.0f;
+        }
+        const int n = min(64, t.k - other);
+        for (int i = 0; i < n; ++i) {
+          const int di = __builtin_amdgcn_readlane(d, i);
+          const float bi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(b), i));
+          again |= di == c && other + i < j;
+          if (di == c && other + i > j) sum += bi;
+        }
+      }
+    if (j < t.k) {
+      l.column[row * t.k + j] = again ? -1 : c;
+      l.weight[row * t.k + j] = sum;
+    }
+  }
+  share = wave_sum(share);
+  whole = wave_sum(whole);
+  if (lane == 0) l.sums[row] = make_float2(share, whole);
+  return __ballot(some) != 0;
+}
+
 // ---- operands into blocks --------------------------------------------------------------------------------------------
 
 // 2^e with max |row| 2^e in [2^13, 2^14) for rows held as two halves, and its inverse; 1 of a row of zeros or with infinities.
@@ -69,51 +122,86 @@ struct Lay {
   int kb, kt;             // blocks of 32 columns, and of 32 rows
   int4v *out, *turned;    // (rows, columns), and (columns, rows) or null
   float *unit;            // of two planes: each row's
-  uint32_t *top;          // the largest unit, or null
   const void *bias;
   int bias_type;
   float *bias_out;        // bias as float32, or null: no bias wanted
   Targets targets;        // of the rows (index null: none): one without any left counts as zeros, whatever it holds
+  List list;
+};
+template <typename T>
+struct Lays {
+  Lay<T> of[2];           // the weight and the rows, or one of them and nothing (kt 0)
+  uint32_t *clear;
 };
 
 constexpr int kSlab = 512;   // columns that pass through LDS at a time
 
-// 16 rows, a wave each; rows past the last are zero.
+// Piece i of a row of `cols` as it lies in memory, zeros past its end.
 template <typename T>
-__global__ __launch_bounds__(1024) void k_lay(const Lay<T> o) {
+__device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int i, int64_t cols) {
+  constexpr int N = Piece<T>::N;
+  if ((int64_t)i * N + N <= cols) return load_whole(row, i);
+  Raw16 p = {};
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e)
+    if ((int64_t)i * N + e < cols) {
+      const uint32_t b = to_bits(row[(int64_t)i * N + e]);
+      if constexpr (sizeof(T) == 4) p.v[e] = b;
+      else p.v[e / 2] |= b << (16 * (e & 1));
+    }
+  return p;
+}
+
+// 16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
+// its maximum to its planes; 0: rows of any length, read from memory once more for the maximum.
+template <typename T, int SLABS>
+__global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   using H = typename Multiplied<T>::H;
-  constexpr int P = Multiplied<T>::P, N = Piece<T>::N, PIECES = kSlab / (64 * N);
-  __shared__ __attribute__((aligned(16))) uint16_t lds[P][16][kSlab + 8];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = blockIdx.x;
+  constexpr int P = Multiplied<T>::P, N = Piece<T>::N, PIECES = kSlab / (64 * N), HELD = SLABS ? SLABS : 1;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][P][16][kSlab + 8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *lays.clear = 0u;
+  const bool second = (int)blockIdx.x >= 2 * lays.of[0].kt;
+  const Lay<T> &o = lays.of[second];
+  const int group = blockIdx.x - (second ? 2 * lays.of[0].kt : 0);
   const int64_t row = (int64_t)group * 16 + wave;
   bool in = row < o.rows;
   const T *src = o.src + (in ? row : 0) * o.ld;
-  if (in && o.targets.index) {
-    bool some = false;
-    for (int j = lane; j < o.targets.k; j += 64) {
-      float a;
-      some |= target_of(o.targets, row, j, a) != -1;
+  if (in && o.targets.index) in = list_row(o.targets, o.list, row, lane);
+  Raw16 held[HELD][PIECES];
+  auto fetch = [&](Raw16 (&p)[PIECES], int first) {
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int i = first / N + lane + 64 * j;
+      p[j] = in && (int64_t)i * N < o.cols ? load_raw(src, i, o.cols) : Raw16{};
     }
-    in = __ballot(some) != 0;
-  }
+  };
+  if constexpr (SLABS > 0)
+#pragma unroll
+    for (int s = 0; s < SLABS; ++s) fetch(held[s], s * kSlab);
   float unit = 1.0f;
   if constexpr (P == 2) {
     float top = 0.0f;
-    if (in)
-      for (int64_t i = lane; i * N < o.cols; i += 64) {
-        const Piece<T> p = load_piece(src, i, o.cols, 0.0f);
+    if constexpr (SLABS > 0) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(p.v[e]));
+      for (int s = 0; s < SLABS; ++s)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+#pragma unroll
+          for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(element<T>(held[s][j], e)));
+    } else if (in) {
+      for (int64_t i = lane; i * N < o.cols; i += 64) {
+        const Raw16 p = load_raw(src, (int)i, o.cols);
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(element<T>(p, e)));
       }
-    unit = unit_of(wave_reduce(top, [](float a, float b) { return nan_max(a, b); }));
-    if (lane == 0) {
-      o.unit[row] = unit;
-      if (in && o.top) raise(o.top, unit);
     }
+    unit = unit_of(wave_reduce(top, [](float a, float b) { return nan_max(a, b); }));
+    if (lane == 0) o.unit[row] = unit;
   }
   if (o.bias_out && lane == 0) {
     float b = 0.0f;
-    if (in && o.bias) {
+    if (row < o.rows && o.bias) {
       if (o.bias_type == FLY_F32) b = static_cast<const float *>(o.bias)[row];
       else if (o.bias_type == FLY_F16) b = static_cast<float>(static_cast<const _Float16 *>(o.bias)[row]);
       else b = static_cast<float>(static_cast<const bhalf *>(o.bias)[row]);
@@ -121,76 +209,90 @@ __global__ __launch_bounds__(1024) void k_lay(const Lay<T> o) {
     o.bias_out[row] = b;
   }
   const float inverse = 1.0f / unit;
-  for (int first = 0; first < o.kb * 32; first += kSlab) {
+  auto slab = [&](const Raw16 (&p)[PIECES], int first, int turn) {
+    auto &part = lds[turn];
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       const int at = (lane + 64 * j) * N;
-      Piece<T> p;
-      if (in && first + at < o.cols) p = load_piece(src, (first + at) / N, o.cols, 0.0f);
-      else
+      if constexpr (P == 1) {
+        *reinterpret_cast<int4v *>(&part[0][wave][at]) = int4v{(int)p[j].v[0], (int)p[j].v[1], (int)p[j].v[2], (int)p[j].v[3]};
+      } else {
+        uint32_t w[P][2];
 #pragma unroll
-        for (int e = 0; e < N; ++e) p.v[e] = 0.0f;
+        for (int e = 0; e < 2; ++e) {
+          uint32_t a[P], b[P];
+          planes_of<H, P>(element<T>(p[j], 2 * e) * inverse, a);
+          planes_of<H, P>(element<T>(p[j], 2 * e + 1) * inverse, b);
 #pragma unroll
-      for (int e = 0; e < N; e += 2) {
-        uint32_t a[P], b[P];
-        planes_of<H, P>(P == 2 ? p.v[e] * inverse : p.v[e], a);
-        planes_of<H, P>(P == 2 ? p.v[e + 1] * inverse : p.v[e + 1], b);
-#pragma unroll
-        for (int q = 0; q < P; ++q) *reinterpret_cast<uint32_t *>(&lds[q][wave][at + e]) = a[q] | b[q] << 16;
-      }
-    }
-    __syncthreads();
-    const int k = first / 32 + wave;
-    if (k < o.kb) {
-#pragma unroll
-      for (int q = 0; q < P; ++q)
-        o.out[(((int64_t)group * o.kb + k) * P + q) * 64 + lane] =
-            *reinterpret_cast<const int4v *>(&lds[q][lane & 15][32 * wave + 8 * (lane >> 4)]);
-      if (o.turned) {
-        const int at = 32 * wave + 16 * (lane >> 5) + (lane & 15), eight = (lane >> 4) & 1;
-        const int64_t block = ((int64_t)2 * k + (lane >> 5)) * o.kt + (group >> 1);
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = lds[q][8 * eight + 2 * e][at] | (uint32_t)lds[q][8 * eight + 2 * e + 1][at] << 16;
-          o.turned[(block * P + q) * 64 + 16 * (2 * (group & 1) + eight) + (lane & 15)] =
-              int4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+          for (int q = 0; q < P; ++q) w[q][e] = a[q] | b[q] << 16;
         }
+#pragma unroll
+        for (int q = 0; q < P; ++q) *reinterpret_cast<uint2 *>(&part[q][wave][at]) = make_uint2(w[q][0], w[q][1]);
       }
     }
-    __syncthreads();
+    __syncthreads();   // one a slab: its halves of LDS take turns, and every wave has read the other one by now
+    const int k = first / 32 + wave;
+    if (k >= o.kb) return;
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+      o.out[(((int64_t)group * o.kb + k) * P + q) * 64 + lane] =
+          *reinterpret_cast<const int4v *>(&part[q][lane & 15][32 * wave + 8 * (lane >> 4)]);
+    if (!o.turned) return;
+    const int at = 32 * wave + 16 * (lane >> 5) + (lane & 15), eight = (lane >> 4) & 1;
+    const int64_t block = ((int64_t)2 * k + (lane >> 5)) * o.kt + (group >> 1);
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = part[q][8 * eight + 2 * e][at] | (uint32_t)part[q][8 * eight + 2 * e + 1][at] << 16;
+      o.turned[(block * P + q) * 64 + 16 * (2 * (group & 1) + eight) + (lane & 15)] =
+          int4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+    }
+  };
+  if constexpr (SLABS > 0) {
+#pragma unroll
+    for (int s = 0; s < SLABS; ++s)
+      if (s * kSlab < o.kb * 32) slab(held[s], s * kSlab, s & 1);
+  } else {
+    for (int s = 0; s * kSlab < o.kb * 32; ++s) {
+      fetch(held[0], s * kSlab);
+      slab(held[0], s * kSlab, s & 1);
+    }
   }
 }
 
 // ---- logits ----------------------------------------------------------------------------------------------------------
 
-// Logits of a piece of rows, with each row's maximum and sum over a wave's columns.
+// How far a logit lies below its part's largest, in 16 bits: steps of 2^-12 up to 12, of 2^-8 from there to 76, and none at all
+// below.  The softmax then errs by 2^-13 relative where it is above 6e-6 of the part's largest, far less than 16-bit gradients
+// round by, and by 2^-9 where it is less.
+constexpr uint32_t kNone = 65535;
+__device__ __forceinline__ uint32_t code_of(float gap) {
+  return gap < 12.0f ? (uint32_t)rintf(gap * 4096.0f) : 49152u + (uint32_t)fminf(rintf((gap - 12.0f) * 256.0f), 16383.0f);
+}
+__device__ __forceinline__ float gap_of(uint32_t code) {
+  return code < 49152u ? (float)code * (1.0f / 4096.0f) : 12.0f + (float)(code - 49152u) * (1.0f / 256.0f);
+}
+
+// What is left of a piece of rows' logits: each row's maximum and sum over a wave's columns, its targets' logits, and for the
+// gradients the logits themselves (Keep: float32, or their distance from the maximum in 16 bits).
+enum Keep { kNothing, kFloats, kCodes };
+template <Keep KEEP>
 struct LogitsOut {
   const float *unit_m, *unit_n;   // or null
   const float *bias;
   const uint8_t *legal;
   int64_t ldl;
-  int rows, cols;
-  float *z;
-  int64_t ldz;
-  float2 *parts;      // (column part, row)
+  int rows, cols, padded;   // columns, and to a multiple of 32, as bias, units and logits are
+  void *z;
+  float2 *parts;      // (row, column part)
   int64_t ld_parts;
+  List list;
   template <int FN, int FM>
-  __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int part, float *turn) const {
+  __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int part, int, float *turn) const {
+    constexpr int PITCH = 16 * FN + 4;
     const int quad = 4 * (lane >> 4);
-    float4v b[FN], un[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int c = n0 + 16 * j + quad;
-      b[j] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-      un[j] = float4v{1.0f, 1.0f, 1.0f, 1.0f};
-      if (c < cols) {   // the arrays are padded to a multiple of 32
-        b[j] = *reinterpret_cast<const float4v *>(bias + c);
-        if (unit_n) un[j] = *reinterpret_cast<const float4v *>(unit_n + c);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int m = m0 + 16 * i + (lane & 15);
@@ -200,14 +302,25 @@ struct LogitsOut {
       PartSum p{-INFINITY, 0.0f};
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        const int c = n0 + 16 * j + quad;
+        const int c = n0 + 16 * j + quad, at = min(c, padded - 4);
+        const float4v b = *reinterpret_cast<const float4v *>(bias + at);
+        const float4v un = unit_n ? *reinterpret_cast<const float4v *>(unit_n + at) : float4v{1.0f, 1.0f, 1.0f, 1.0f};
+        uint32_t shown = 0x01010101u;
+        if (seen) {
+          struct __attribute__((packed)) Bytes {
+            uint32_t w;
+          };
+          if (c + 4 <= cols) shown = reinterpret_cast<const Bytes *>(seen + c)->w;
+          else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (c + e < cols && !seen[c + e]) shown &= ~(1u << (8 * e));
+        }
         float l[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          // a load for each column, of one that is there where this one is not: no branch around each
-          const uint8_t shown = seen ? seen[min(c + e, cols - 1)] : 1;
-          const float x = (unit_n ? acc[j][i][e] * um * un[j][e] : acc[j][i][e]) + b[j][e];
-          l[e] = c + e < cols && shown ? x : -INFINITY;
+          const float x = (unit_n ? acc[j][i][e] * um * un[e] : acc[j][i][e]) + b[e];
+          l[e] = c + e < cols && ((shown >> (8 * e)) & 0xffu) ? x : -INFINITY;
           p.top = fmaxf(p.top, l[e]);
         }
         v[j] = float4v{l[0], l[1], l[2], l[3]};
@@ -226,11 +339,32 @@ struct LogitsOut {
 #pragma unroll
         for (int e = 0; e < 4; ++e) p.sum += exp2_of((v[j][e] - base) * kLog2e);
       p.sum = four(p.sum, [](float x, float y) { return x + y; });
-      if (lane < 16 && m < rows) parts[part * ld_parts + m] = make_float2(p.top, p.sum);
-      turn_over<FN>(v, turn, lane, [&](int row, int c, const float4v &four_) {
+      if (lane < 16) {
+        if (m < rows) parts[m * ld_parts + part] = make_float2(p.top, p.sum);
+        turn[lane * PITCH + 16 * FN] = p.top;   // in the row's padding
+      }
+      turn_over<FN>(v, turn, lane, [&](int row, int c, const float4v &z4) {
         const int mm = m0 + 16 * i + row;
-        if (mm < rows && n0 + c < ldz) *reinterpret_cast<float4v *>(z + mm * ldz + n0 + c) = four_;
+        if (mm >= rows || n0 + c >= padded) return;
+        if constexpr (KEEP == kFloats) {
+          *reinterpret_cast<float4v *>(static_cast<float *>(z) + (int64_t)mm * padded + n0 + c) = z4;
+        } else if constexpr (KEEP == kCodes) {
+          const float top = turn[row * PITCH + 16 * FN];
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = code_of(top - z4[e]);
+          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(z) + (int64_t)mm * padded + n0 + c) =
+              make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+        }
       });
+      // the targets among these columns, 4 entries of 16 rows at a time
+      if (m < rows)
+        for (int j = lane >> 4; j < list.k; j += 4) {
+          const int64_t at = (int64_t)m * list.k + j;
+          const int c = list.column[at] - n0;
+          if (c >= 0 && c < 16 * FN) list.logit[at] = turn[(lane & 15) * PITCH + c];
+        }
+      asm volatile("" ::: "memory");
     }
   }
 };
@@ -242,47 +376,50 @@ struct RowInfo {
   float top, log_sum, share, whole;
 };
 
-// A wave per row.
+// A wave per row; a last workgroup finds the largest of the weights' units.
 __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ parts, int64_t ld_parts, int count, int rows,
-                                                   const Targets t, const float *__restrict__ z, int64_t ldz,
-                                                   const float *__restrict__ unit, const float *__restrict__ row_scale,
-                                                   float grad_scale, float *__restrict__ loss, RowInfo *__restrict__ info,
+                                                   const List l, const float *__restrict__ unit,
+                                                   const float *__restrict__ row_scale, float grad_scale,
+                                                   float *__restrict__ loss, RowInfo *__restrict__ info,
                                                    float *__restrict__ factor, float *__restrict__ turned_factor,
-                                                   uint32_t *__restrict__ most) {
+                                                   const float *__restrict__ unit_n, int cols, Maxima *__restrict__ maxima) {
   const int lane = threadIdx.x & 63;
+  if (unit_n && blockIdx.x == gridDim.x - 1) {
+    __shared__ float share[4];
+    float most = 0.0f;
+    for (int c = threadIdx.x; c < cols; c += 256) most = fmaxf(most, unit_n[c]);
+    most = wave_max(most);
+    if (lane == 0) share[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) maxima->weight = __float_as_uint(fmaxf(fmaxf(share[0], share[1]), fmaxf(share[2], share[3])));
+    return;
+  }
   const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
   if (row >= rows) return;
+  const float2 sums = l.sums[row];
   PartSum p{-INFINITY, 0.0f};
   for (int i = lane; i < count; i += 64) {
-    const float2 v = parts[i * ld_parts + row];
+    const float2 v = parts[row * ld_parts + i];
     const float top = fmaxf(p.top, v.x), base = base_of(top);
     p.sum = p.sum * exp2_of((p.top - base) * kLog2e) + v.y * exp2_of((v.x - base) * kLog2e);
     p.top = top;
   }
   p = wave_part(p, kLog2e);
   const float log_sum = log2_of(p.sum);
-  float sum = 0.0f, share = 0.0f, whole = 0.0f;
-  for (int j = lane; j < t.k; j += 64) {
-    float a;
-    const int c = target_of(t, row, j, a);
-    if (c == -1) continue;
-    const float far = c == -2 ? __builtin_nanf("") : (p.top - z[row * ldz + c]) + kLn2 * log_sum;
-    sum += a * far;
-    share += c == -2 ? __builtin_nanf("") : a;
-    whole += fabsf(a);
-  }
+  float sum = 0.0f;
+  for (int j = lane; j < l.k; j += 64)
+    if (l.column[row * l.k + j] >= 0)
+      sum += l.weight[row * l.k + j] * ((p.top - l.logit[row * l.k + j]) + kLn2 * log_sum);
   sum = wave_sum(sum);
-  share = wave_sum(share);
-  whole = wave_sum(whole);
   if (lane) return;
-  const bool some = whole != 0.0f;   // NaN too
-  if (loss) loss[row] = some ? sum : 0.0f;
+  const bool some = sums.y != 0.0f;   // NaN too
+  if (loss) loss[row] = !some ? 0.0f : sums.y == sums.y ? sum : sums.y;
   if (!info) return;
-  info[row] = RowInfo{base_of(p.top), log_sum, some ? share / whole : 0.0f, whole};
-  const float f = some ? whole * (row_scale ? row_scale[row] : 1.0f) * grad_scale : 0.0f, ft = unit ? f * unit[row] : f;
+  info[row] = RowInfo{base_of(p.top), log_sum, some ? sums.x / sums.y : 0.0f, sums.y};
+  const float f = some ? sums.y * (row_scale ? row_scale[row] : 1.0f) * grad_scale : 0.0f, ft = unit ? f * unit[row] : f;
   factor[row] = f;
   turned_factor[row] = ft;
-  raise(most, fabsf(ft));
+  raise(&maxima->row, fabsf(ft));
 }
 
 // ---- the logits' gradient --------------------------------------------------------------------------------------------
@@ -290,18 +427,19 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ pa
 constexpr int kGradRows = 64, kGradCols = 128, kGradPitch = 130;
 
 // u of 64 rows x 128 columns into blocks, by rows (times the columns' units) and turned (times the rows' factors), and its
-// columns' sums.
-template <typename H, int P>
-__global__ __launch_bounds__(256) void k_logits_grad(const float *__restrict__ z, int64_t ldz, int rows, const Targets t,
+// columns' sums.  Parts of 2^shift columns.
+template <typename H, int P, Keep KEEP>
+__global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z, int64_t ldz, int rows, int cols, const List l,
+                                                     const float2 *__restrict__ parts, int64_t ld_parts, int shift,
                                                      const RowInfo *__restrict__ info, const float *__restrict__ factor,
                                                      const float *__restrict__ turned_factor,
                                                      const float *__restrict__ unit_n, const Maxima *__restrict__ maxima,
                                                      int rb, int vb, int4v *__restrict__ out, int4v *__restrict__ turned,
                                                      float *__restrict__ sums, int64_t ld_sums) {
   __shared__ __attribute__((aligned(16))) float u[kGradRows][kGradPitch];
-  __shared__ float col_sum[2][kGradCols], f_row[kGradRows], ft_row[kGradRows], un_col[kGradCols];
+  __shared__ float col_sum[2][kGradCols], f_row[kGradRows], ft_row[kGradRows], un_col[kGradCols], f_part[kGradRows][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c0 = blockIdx.x * kGradCols, r0 = blockIdx.y * kGradRows, cols = t.cols;
+  const int c0 = blockIdx.x * kGradCols, r0 = blockIdx.y * kGradRows;
   if (tid < kGradRows) {
     const int r = r0 + tid;
     const float most = __uint_as_float(maxima->row);
@@ -312,32 +450,57 @@ __global__ __launch_bounds__(256) void k_logits_grad(const float *__restrict__ z
     const int c = c0 + tid - 128;
     un_col[tid - 128] = P == 2 && c < cols ? unit_n[c] / __uint_as_float(maxima->weight) * kUnit : kUnit;
   }
+  if constexpr (KEEP == kFloats) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = (tid >> 5) + 8 * i, c = 4 * (tid & 31);
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r0 + r < rows && c0 + c < cols) {
-      const RowInfo f = info[r0 + r];
-      const float4v at = *reinterpret_cast<const float4v *>(z + (int64_t)(r0 + r) * ldz + c0 + c);
+    for (int i = 0; i < 8; ++i) {
+      const int r = (tid >> 5) + 8 * i, c = 4 * (tid & 31);
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r0 + r < rows && c0 + c < cols) {
+        const RowInfo f = info[r0 + r];
+        const float4v at = *reinterpret_cast<const float4v *>(static_cast<const float *>(z) + (r0 + r) * ldz + c0 + c);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (c0 + c + e < cols && f.share != 0.0f) v[e] = f.share * exp2_of((at[e] - f.top) * kLog2e - f.log_sum);
+        for (int e = 0; e < 4; ++e)
+          if (c0 + c + e < cols && f.share != 0.0f) v[e] = f.share * exp2_of((at[e] - f.top) * kLog2e - f.log_sum);
+      }
+      *reinterpret_cast<float2 *>(&u[r][c]) = make_float2(v[0], v[1]);
+      *reinterpret_cast<float2 *>(&u[r][c + 2]) = make_float2(v[2], v[3]);
     }
-    *reinterpret_cast<float2 *>(&u[r][c]) = make_float2(v[0], v[1]);
-    *reinterpret_cast<float2 *>(&u[r][c + 2]) = make_float2(v[2], v[3]);
-  }
-  __syncthreads();
-  {
-    // the targets of a row, in their order, a thread for each quarter of its columns
-    const int r = tid & 63, q0 = c0 + 32 * (tid >> 6);
-    if (r0 + r < rows && info[r0 + r].whole != 0.0f) {
-      const float whole = info[r0 + r].whole;
-      for (int j = 0; j < t.k; ++j) {
-        float a;
-        const int64_t c = target_at(t, (int64_t)(r0 + r) * t.k + j);
-        if (c >= q0 && c < q0 + 32 && target_of(t, r0 + r, j, a) >= 0) u[r][c - c0] -= a / whole;
+  } else {
+    {
+      // a part's largest p, times the share
+      const int r = tid >> 2, q = tid & 3;
+      float f = 0.0f;
+      if (r0 + r < rows && c0 + (q << shift) < cols && (q << shift) < kGradCols) {
+        const RowInfo i = info[r0 + r];
+        const float top = parts[(r0 + r) * ld_parts + (c0 >> shift) + q].x;
+        if (i.share != 0.0f) f = i.share * exp2_of((top - i.top) * kLog2e - i.log_sum);
+      }
+      f_part[r][q] = f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 4) + 16 * i, c = 8 * (tid & 15);
+      int4v w = {-1, -1, -1, -1};
+      if (r0 + r < rows && c0 + c < ldz) w = *reinterpret_cast<const int4v *>(static_cast<const uint16_t *>(z) + (r0 + r) * ldz + c0 + c);
+      const float f = f_part[r][c >> shift];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a = (uint32_t)w[e] & 0xffffu, b = (uint32_t)w[e] >> 16;
+        *reinterpret_cast<float2 *>(&u[r][c + 2 * e]) =
+            make_float2(f * (a == kNone ? 0.0f : exp2_of(gap_of(a) * -kLog2e)), f * (b == kNone ? 0.0f : exp2_of(gap_of(b) * -kLog2e)));
       }
     }
+  }
+  __syncthreads();
+  // the targets among these columns, each once
+  for (int at = tid; at < min(kGradRows, rows - r0) * l.k; at += 256) {
+    const int64_t from = (int64_t)r0 * l.k + at;
+    const int c = l.column[from];
+    if (c < c0 || c >= c0 + kGradCols) continue;
+    const int r = at / l.k;
+    const RowInfo f = info[r0 + r];
+    u[r][c - c0] = f.share * exp2_of((l.logit[from] - f.top) * kLog2e - f.log_sum) - l.weight[from] / f.whole;
   }
   __syncthreads();
   typedef uint32_t words[4];
@@ -393,22 +556,30 @@ __global__ __launch_bounds__(256) void k_logits_grad(const float *__restrict__ z
   if (half == 0 && c0 + c < cols) sums[blockIdx.y * ld_sums + c0 + c] = s + col_sum[1][c];
 }
 
-// The columns' sums over all tiles of rows, after what earlier pieces of rows gave.
+// The columns' sums over all tiles of rows, after what earlier pieces of rows gave: 64 columns, each wave every 16th tile.
 template <typename T>
-__global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ sums, int64_t ld_sums, int tiles, int cols,
-                                                   const float *__restrict__ before, float *__restrict__ after,
-                                                   T *__restrict__ out) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
-  float s = before ? before[c] : 0.0f;
-  for (int i = 0; i < tiles; ++i) s += sums[i * ld_sums + c];
+__global__ __launch_bounds__(1024) void k_bias_grad(const float *__restrict__ sums, int64_t ld_sums, int tiles, int cols,
+                                                    const float *__restrict__ before, float *__restrict__ after,
+                                                    T *__restrict__ out) {
+  __shared__ float share[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (c < cols)
+    for (int i = wave; i < tiles; i += 16) s += sums[i * ld_sums + c];
+  share[wave][lane] = s;
+  __syncthreads();
+  if (wave || c >= cols) return;
+  s = before ? before[c] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += share[i][lane];
   if (after) after[c] = s;
   else out[c] = static_cast<T>(s);
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------------------
 
-// out[m][n] = sum * row[m] * *scale / 2^14, after what earlier pieces of rows gave.
+// out[m][n] = sum * row[m] * *scale / 2^14, after what earlier pieces of rows gave.  Where k runs in parts, the sums of each go
+// to `share` and k_join adds them up.
 template <typename T>
 struct GradOut {
   const float *row;          // or null
@@ -416,12 +587,37 @@ struct GradOut {
   int rows, cols;
   const float *before;
   float *after;              // or null: the last piece, into out
-  int64_t ld_sum;
+  int64_t ld_sum;            // columns, to a multiple of 32
   T *out;
   int64_t ld;
+  float *share;              // (part, row, column) or null
+  __device__ __forceinline__ float unit() const { return (scale ? __uint_as_float(*scale) : 1.0f) / kUnit; }
+  __device__ __forceinline__ void put(int m, int n, const float4v &sum, float unit) const {
+    const float f = row ? unit * row[m] : unit;
+    float4v w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = sum[e] * f;
+    if (before) w += *reinterpret_cast<const float4v *>(before + m * ld_sum + n);
+    if (after) {
+      *reinterpret_cast<float4v *>(after + m * ld_sum + n) = w;
+      return;
+    }
+    struct __attribute__((packed, aligned(sizeof(T)))) Four {
+      T v[4];
+    };
+    T *to = out + m * ld + n;
+    if (n + 4 <= cols)
+      *reinterpret_cast<Four *>(to) =
+          Four{{static_cast<T>(w[0]), static_cast<T>(w[1]), static_cast<T>(w[2]), static_cast<T>(w[3])}};
+    else
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (n + e < cols) to[e] = static_cast<T>(w[e]);
+  }
   template <int FN, int FM>
-  __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int, float *turn) const {
-    const float s = (scale ? __uint_as_float(*scale) : 1.0f) / kUnit;
+  __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int, int split, float *turn) const {
+    const float s = unit();
+    float *to = share ? share + (int64_t)split * rows * ld_sum : nullptr;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       float4v v[FN];
@@ -430,30 +626,26 @@ struct GradOut {
       turn_over<FN>(v, turn, lane, [&](int r, int c, const float4v &four) {
         const int m = m0 + 16 * i + r, n = n0 + c;
         if (m >= rows || n >= cols) return;
-        const float f = row ? s * row[m] : s;
-        float4v w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = four[e] * f;
-        if (before) w += *reinterpret_cast<const float4v *>(before + m * ld_sum + n);
-        if (after) {
-          *reinterpret_cast<float4v *>(after + m * ld_sum + n) = w;
-          return;
-        }
-        struct __attribute__((packed, aligned(sizeof(T)))) Four {
-          T v[4];
-        };
-        T *to = out + m * ld + n;
-        if (n + 4 <= cols)
-          *reinterpret_cast<Four *>(to) =
-              Four{{static_cast<T>(w[0]), static_cast<T>(w[1]), static_cast<T>(w[2]), static_cast<T>(w[3])}};
-        else
-#pragma unroll
-          for (int e = 0; e < 3; ++e)
-            if (n + e < cols) to[e] = static_cast<T>(w[e]);
+        if (to) *reinterpret_cast<float4v *>(to + m * ld_sum + n) = four;
+        else put(m, n, four, s);
       });
     }
   }
 };
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(const GradOut<T> g, int splits) {
+  const int64_t per = g.ld_sum / 4, all = g.rows * per, stride = g.rows * g.ld_sum;
+  const float s = g.unit();
+  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int m = (int)(i / per), n = 4 * (int)(i % per);
+    if (n >= g.cols) continue;
+    const float *from = g.share + m * g.ld_sum + n;
+    float4v sum = *reinterpret_cast<const float4v *>(from);
+    for (int p = 1; p < splits; ++p) sum += *reinterpret_cast<const float4v *>(from + p * stride);
+    g.put(m, n, sum, s);
+  }
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, int64_t rows, int64_t cols) {
@@ -463,19 +655,63 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 
 // ---- the call --------------------------------------------------------------------------------------------------------
 
+
 struct Call {
   int32_t type;
-  int64_t rows, d, v;
+  int64_t rows, d, v, k;
   bool gx, gw, gb;
   bool grads() const { return gx || gw || gb; }
 };
 
-template <typename H, int P, typename EP>
-void product(const Blocks &o, const EP &ep, hipStream_t st) {
-  if constexpr (P == 1) launch_blocks<H, P, 2, 4, 4, 2, 4>(o, ep, st);
-  else launch_blocks<H, P, 2, 4, 4, 2, 3>(o, ep, st);
+// The workgroup's tile of a product of m x n, n x m rows of it.  One plane: 256 x 256 from 128 tiles on, 128 x 128 from 100 on,
+// else 64 x 64; two planes: 128 x 192 from 150 tiles on, else 64 x 64.
+enum Shape { kSmall, kMedium, kLarge };
+Shape shape_of(int planes, int64_t m, int64_t n) {
+  auto tiles = [&](int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
+  if (planes == 2) return tiles(192, 128) >= 150 ? kLarge : kSmall;
+  return tiles(256, 256) >= 128 ? kLarge : tiles(128, 128) >= 100 ? kMedium : kSmall;
 }
-constexpr int kTileN = 128, kPartN = 64;
+// Parts of a row's columns that the waves of a shape hold, for `cols` columns.
+int parts_of(int planes, Shape s, int64_t cols) {
+  const int64_t tile = s == kSmall ? 64 : s == kMedium || planes == 2 ? 128 : 256, wave = s == kSmall ? 32 : 64;
+  return (int)((cols + tile - 1) / tile * (tile / wave));
+}
+template <typename H, int P, typename EP, int COUNT>
+void product(Shape shape, const Products<EP, COUNT> &p, hipStream_t st) {
+  if (shape == kSmall) launch_blocks<H, P, 2, 2, 2, 2, 4>(p, st);
+  else if constexpr (P == 2) launch_blocks<H, P, 2, 4, 4, 3, 3>(p, st);
+  else if (shape == kMedium) launch_blocks<H, P, 2, 4, 4, 2, 4>(p, st);
+  else launch_blocks<H, P, 4, 4, 4, 4, 4>(p, st);
+}
+
+// In how many parts the k of the gradients' products run, side by side in one launch.  Jobs are counted in blocks of k of one
+// tile; one that is longer than 0.7 of what each of the CU's places gets keeps the others waiting.  A part costs its sums' way to
+// memory and back, so none is shorter than 16 blocks, and all parts' sums fit kShareBytes.
+constexpr int64_t kShareBytes = (int64_t)64 << 20;
+struct Splits {
+  int x = 1, w = 1;
+};
+Shape grad_shape(int planes, const Call &c, int64_t rows) {
+  return shape_of(planes, (c.gx ? rows : 0) + (c.gw ? c.v : 0), c.d);
+}
+Splits splits_of(int planes, const Call &c, int64_t rows) {
+  const Shape s = grad_shape(planes, c, rows);
+  const int64_t tm = s == kSmall ? 64 : planes == 2 ? 192 : s == kMedium ? 128 : 256;
+  const int64_t tn = s == kSmall ? 64 : planes == 2 || s == kMedium ? 128 : 256;
+  const int64_t places = planes == 2 ? (s == kSmall ? 512 : 256) : s == kLarge ? 256 : 512;
+  auto tiles = [&](int64_t m) { return ((m + tm - 1) / tm) * ((c.d + tn - 1) / tn); };
+  const int64_t kx = (c.v + 31) / 32, kw = (rows + 31) / 32;
+  const int64_t all = (c.gx ? tiles(rows) * kx : 0) + (c.gw ? tiles(c.v) * kw : 0);
+  const double most = std::max(16.0, 0.7 * (double)all / (double)places);
+  auto parts = [&](int64_t m, int64_t k) {
+    const int64_t fit = kShareBytes / 2 / (m * round_up(c.d, 32) * 4);
+    return (int)std::max<int64_t>(1, std::min((int64_t)((double)k / most + 0.99), fit));
+  };
+  Splits p;
+  if (c.gx) p.x = parts(rows, kx);
+  if (c.gw) p.w = parts(c.v, kw);
+  return p;
+}
 
 // Where everything lies in the workspace.
 struct Space {
@@ -483,12 +719,16 @@ struct Space {
   int64_t db, vb, rb; // blocks of 32
   int parts;
   bool several;
-  size_t x, xt, w, wt, z, g, gt, unit_x, unit_w, bias, stat, info, factor, turned, sums, maxima, acc_w, acc_b, bytes;
+  size_t x, xt, w, wt, z, g, gt, unit_x, unit_w, bias, stat, info, factor, turned, sums, maxima, acc_w, acc_b, column, weight,
+      logit, list_sums, share_x, share_w, bytes;
   Space(const Call &c, int planes) {
     db = (c.d + 31) / 32;
     vb = (c.v + 31) / 32;
-    parts = (int)((vb * 32 + kTileN - 1) / kTileN * (kTileN / kPartN));
-    const int64_t each = vb * 32 * (4 + 2 * planes * ((c.gx ? 1 : 0) + (c.gw ? 1 : 0))) + db * 64 * planes * (c.gw ? 2 : 1);
+    parts = parts_of(planes, kSmall, vb * 32);   // the most that a shape has, but for a tile's rounding
+    parts = (int)round_up(parts, 4);
+    const int64_t kept = c.grads() ? planes * 2 : 0;   // bytes of a logit
+    const int64_t each = vb * 32 * (kept + 2 * planes * ((c.gx ? 1 : 0) + (c.gw ? 1 : 0))) + db * 64 * planes * (c.gw ? 2 : 1) +
+                         12 * c.k + 8 * parts_of(planes, kSmall, vb * 32);
     piece = std::min({round_up(c.rows, 64), std::max<int64_t>(kPieceBytes / each / 64 * 64, 64), kPieceRows});
     several = piece < c.rows;
     rb = piece / 32;
@@ -503,7 +743,7 @@ struct Space {
     xt = c.gw ? take(rb * db * block) : 0;
     w = take(vb * db * block);
     wt = c.gx ? take(vb * db * block) : 0;
-    z = take(piece * vb * 32 * 4);
+    z = kept ? take(piece * vb * 32 * kept) : 0;
     g = c.gx ? take(rb * vb * block) : 0;
     gt = c.gw ? take(rb * vb * block) : 0;
     unit_x = take(rb * 32 * 4);
@@ -517,6 +757,13 @@ struct Space {
     maxima = take(sizeof(Maxima));
     acc_w = several && c.gw ? take(c.v * db * 32 * 4) : 0;
     acc_b = several && c.gb ? take(vb * 32 * 4) : 0;
+    column = take(piece * c.k * 4);
+    weight = take(piece * c.k * 4);
+    logit = take(piece * c.k * 4);
+    list_sums = take(piece * 8);
+    const Splits p = splits_of(planes, c, piece < c.rows ? piece : c.rows);
+    share_x = several && c.gx ? take(kShareBytes / 2) : p.x > 1 ? take(p.x * c.rows * db * 128) : 0;
+    share_w = several && c.gw ? take(kShareBytes / 2) : p.w > 1 ? take(p.w * c.v * db * 128) : 0;
     bytes = at;
   }
 };
@@ -554,60 +801,89 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
   Maxima *maxima = reinterpret_cast<Maxima *>(at(s.maxima));
   float *unit_x = P == 2 ? floats(s.unit_x) : nullptr, *unit_w = P == 2 ? floats(s.unit_w) : nullptr;
   RowInfo *info = c.grads() ? reinterpret_cast<RowInfo *>(at(s.info)) : nullptr;
-  hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, maxima);
-  check_launch("read-out loss");
-  auto lay = [&](const Lay<T> &l) {
-    hipLaunchKernelGGL(k_lay<T>, dim3((unsigned)(2 * l.kt)), dim3(1024), 0, st, l);
-    check_launch("read-out operands");
-  };
-  lay(Lay<T>{static_cast<const T *>(g.w), g.ldw, c.v, c.d, (int)s.db, (int)s.vb, blocks(s.w), c.gx ? blocks(s.wt) : nullptr,
-             unit_w, P == 2 ? &maxima->weight : nullptr, g.bias, g.bias_type, floats(s.bias), Targets{}});
+  const int padded = (int)s.vb * 32;
   for (int64_t first = 0; first < c.rows; first += s.piece) {
     const int rows = (int)std::min(s.piece, c.rows - first);
     const bool last = first + rows == c.rows;
     const int rb = (rows + 31) / 32, tiles = (rows + kGradRows - 1) / kGradRows;
-    const int64_t ldz = s.vb * 32;
-    if (first) {
-      hipLaunchKernelGGL(k_clear_row, dim3(1), dim3(1), 0, st, maxima);
-      check_launch("read-out loss");
-    }
     Targets t = g.targets;
     t.index = static_cast<const char *>(t.index) + first * t.k * (t.wide ? 8 : 4);
     if (t.weight) t.weight += first * t.k;
     if (t.legal) t.legal += first * t.ldl;
-    lay(Lay<T>{static_cast<const T *>(g.x) + first * g.ldx, g.ldx, rows, c.d, (int)s.db, rb, blocks(s.x),
-               c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, nullptr, 0, nullptr, t});
-    product<H, P>(Blocks{blocks(s.w), blocks(s.x), (int)(2 * s.vb), 2 * rb, (int)s.db, 0, 0, 0},
-                  LogitsOut{unit_x, unit_w, floats(s.bias), t.legal, t.ldl, rows, (int)c.v, floats(s.z), ldz,
-                            reinterpret_cast<float2 *>(at(s.stat)), s.piece},
-                  st);
-    hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4)), dim3(256), 0, st, reinterpret_cast<const float2 *>(at(s.stat)),
-                       s.piece, s.parts, rows, t, floats(s.z), ldz, unit_x,
-                       g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, g.loss ? g.loss + first : nullptr, info,
-                       floats(s.factor), floats(s.turned), &maxima->row);
+    const List list{reinterpret_cast<int *>(at(s.column)), floats(s.weight), floats(s.logit),
+                    reinterpret_cast<float2 *>(at(s.list_sums)), t.k};
+    Lays<T> lays{};
+    if (!first)
+      lays.of[0] = Lay<T>{static_cast<const T *>(g.w), g.ldw, c.v, c.d, (int)s.db, (int)s.vb, blocks(s.w),
+                          c.gx ? blocks(s.wt) : nullptr, unit_w, g.bias, g.bias_type, floats(s.bias), Targets{}, List{}};
+    lays.of[1] = Lay<T>{static_cast<const T *>(g.x) + first * g.ldx, g.ldx, rows, c.d, (int)s.db, rb, blocks(s.x),
+                        c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, 0, nullptr, t, list};
+    lays.clear = &maxima->row;
+    const unsigned groups = (unsigned)(2 * (lays.of[0].kt + rb));
+    auto lay = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, st, lays); };
+    const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // a row of up to 3,072 columns stays in registers
+    if (slabs <= 2) lay(k_lay<T, 2>);
+    else if (slabs <= 6) lay(k_lay<T, 6>);
+    else lay(k_lay<T, 0>);
+    check_launch("read-out operands");
+    const Shape wide = shape_of(P, rows, c.v);
+    const int parts = parts_of(P, wide, padded);
+    const float2 *stat = reinterpret_cast<const float2 *>(at(s.stat));
+    auto logits = [&](auto keep) {
+      constexpr Keep KEEP = decltype(keep)::value;
+      product<H, P>(wide,
+                    Products<LogitsOut<KEEP>, 1>{
+                        {Blocks{blocks(s.w), blocks(s.x), (int)(2 * s.vb), 2 * rb, (int)s.db, 1, 0, 0, 0}},
+                        {LogitsOut<KEEP>{unit_x, unit_w, floats(s.bias), t.legal, t.ldl, rows, (int)c.v, padded, at(s.z),
+                                         reinterpret_cast<float2 *>(at(s.stat)), s.parts, list}}},
+                    st);
+    };
+    constexpr Keep KEPT = P == 1 ? kCodes : kFloats;
+    if (c.grads()) logits(std::integral_constant<Keep, KEPT>{});
+    else logits(std::integral_constant<Keep, kNothing>{});
+    hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4) + (P == 2)), dim3(256), 0, st, stat, s.parts, parts, rows, list,
+                       unit_x, g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, g.loss ? g.loss + first : nullptr,
+                       info, floats(s.factor), floats(s.turned), unit_w, (int)c.v, maxima);
     check_launch("read-out loss");
     if (!c.grads()) continue;
-    hipLaunchKernelGGL((k_logits_grad<H, P>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, floats(s.z), ldz,
-                       rows, t, info, floats(s.factor), floats(s.turned), unit_w, maxima, 2 * rb, (int)s.vb,
-                       c.gx ? blocks(s.g) : nullptr, c.gw ? blocks(s.gt) : nullptr, c.gb ? floats(s.sums) : nullptr, ldz);
+    hipLaunchKernelGGL((k_logits_grad<H, P, KEPT>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, at(s.z),
+                       (int64_t)padded, rows, (int)c.v, list, stat, s.parts, wide == kSmall ? 5 : 6, info, floats(s.factor),
+                       floats(s.turned), unit_w, maxima, 2 * rb, (int)s.vb, c.gx ? blocks(s.g) : nullptr,
+                       c.gw ? blocks(s.gt) : nullptr, c.gb ? floats(s.sums) : nullptr, (int64_t)padded);
     check_launch("read-out gradient");
     if (c.gb)
       by_type(g.bias_type, "the bias must be float32, float16 or bfloat16", [&](auto b) {
         using B = decltype(b);
-        hipLaunchKernelGGL(k_bias_grad<B>, dim3(blocks_for(c.v, 256)), dim3(256), 0, st, floats(s.sums), ldz, tiles, (int)c.v,
-                           first ? floats(s.acc_b) : nullptr, last ? nullptr : floats(s.acc_b), static_cast<B *>(g.gb));
+        hipLaunchKernelGGL(k_bias_grad<B>, dim3(blocks_for(c.v, 64)), dim3(1024), 0, st, floats(s.sums), (int64_t)padded, tiles,
+                           (int)c.v, first ? floats(s.acc_b) : nullptr, last ? nullptr : floats(s.acc_b),
+                           static_cast<B *>(g.gb));
         check_launch("read-out gradient");
       });
-    if (c.gx)
-      product<H, P>(Blocks{blocks(s.wt), blocks(s.g), (int)(2 * s.db), 2 * rb, (int)s.vb, 0, 0, 0},
-                    GradOut<T>{floats(s.factor), P == 2 ? &maxima->weight : nullptr, rows, (int)c.d, nullptr, nullptr, 0,
-                               static_cast<T *>(g.gx) + first * g.ldgx, g.ldgx},
+    const Shape shape = grad_shape(P, c, rows);
+    const Splits splits = splits_of(P, c, rows);
+    const int64_t ld_sum = s.db * 32;
+    const Blocks by_rows{blocks(s.wt), blocks(s.g), (int)(2 * s.db), 2 * rb, (int)s.vb, splits.x, 0, 0, 0};
+    const Blocks by_columns{blocks(s.xt), blocks(s.gt), (int)(2 * s.db), (int)(2 * s.vb), rb, splits.w, 0, 0, 0};
+    const GradOut<T> to_x{floats(s.factor), P == 2 ? &maxima->weight : nullptr, rows, (int)c.d, nullptr, nullptr, ld_sum,
+                          c.gx ? static_cast<T *>(g.gx) + first * g.ldgx : nullptr, g.ldgx, splits.x > 1 ? floats(s.share_x) : nullptr};
+    const GradOut<T> to_w{nullptr, &maxima->row, (int)c.v, (int)c.d, first ? floats(s.acc_w) : nullptr,
+                          last ? nullptr : floats(s.acc_w), ld_sum, static_cast<T *>(g.gw), g.ldgw,
+                          splits.w > 1 ? floats(s.share_w) : nullptr};
+    if (c.gx && c.gw)   // the longer sums first
+      product<H, P>(shape,
+                    s.vb / splits.x >= rb / splits.w ? Products<GradOut<T>, 2>{{by_rows, by_columns}, {to_x, to_w}}
+                                                     : Products<GradOut<T>, 2>{{by_columns, by_rows}, {to_w, to_x}},
                     st);
-    if (c.gw)
-      product<H, P>(Blocks{blocks(s.xt), blocks(s.gt), (int)(2 * s.db), (int)(2 * s.vb), rb, 0, 0, 0},
-                    GradOut<T>{nullptr, &maxima->row, (int)c.v, (int)c.d, first ? floats(s.acc_w) : nullptr,
-                               last ? nullptr : floats(s.acc_w), s.db * 32, static_cast<T *>(g.gw), g.ldgw},
-                    st);
+    else if (c.gx) product<H, P>(shape, Products<GradOut<T>, 1>{{by_rows}, {to_x}}, st);
+    else if (c.gw) product<H, P>(shape, Products<GradOut<T>, 1>{{by_columns}, {to_w}}, st);
+    auto join = [&](const GradOut<T> &o, int parts_of_k) {
+      if (!o.share) return;
+      hipLaunchKernelGGL(k_join<T>, dim3((unsigned)std::min<int64_t>((o.rows * ld_sum / 4 + 255) / 256, 4096)), dim3(256), 0, st, o,
+                         parts_of_k);
+      check_launch("read-out gradient");
+    };
+    if (c.gx) join(to_x, splits.x);
+    if (c.gw) join(to_w, splits.w);
   }
 }
 
@@ -616,6 +892,7 @@ void require_call(const Call &c) {
   FLY_REQUIRE(c.rows >= 0 && c.rows < (int64_t)1 << 40 && c.d >= 1 && c.d <= (int64_t)1 << 16 && c.v >= 1 &&
                   c.v <= (int64_t)1 << 20,
               "size out of range");
+  FLY_REQUIRE(c.k >= 1 && c.k <= 1024, "k must lie in 1..1024");
 }
 size_t call_ws(const Call &c) { return c.rows ? Space(c, c.type == FLY_F32 ? 2 : 1).bytes : 0; }
 
@@ -624,8 +901,8 @@ size_t call_ws(const Call &c) { return c.rows ? Space(c, c.type == FLY_F32 ? 2 :
 
 using namespace fly;
 
-extern "C" size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t wanted) {
-  const Call c{type, rows, d, v, (wanted & FLY_GRAD_X) != 0, (wanted & FLY_GRAD_W) != 0, (wanted & FLY_GRAD_B) != 0};
+extern "C" size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t k, int32_t wanted) {
+  const Call c{type, rows, d, v, k, (wanted & FLY_GRAD_X) != 0, (wanted & FLY_GRAD_W) != 0, (wanted & FLY_GRAD_B) != 0};
   size_t bytes = 0;
   guard([&] {
     require_call(c);
@@ -640,11 +917,10 @@ extern "C" int fly_readout_loss(const void *x, int32_t type, int64_t ldx, int64_
                                 const float *row_scale, float grad_scale, void *gx, int64_t ldgx, void *gw, int64_t ldgw,
                                 void *gb, void *ws, size_t ws_bytes, void *stream) {
   return guard([&] {
-    const Call c{type, rows, d, v, gx != nullptr, gw != nullptr, gb != nullptr};
+    const Call c{type, rows, d, v, k, gx != nullptr, gw != nullptr, gb != nullptr};
     require_call(c);
     FLY_REQUIRE(bias_type >= FLY_F32 && bias_type <= FLY_BF16, "the bias must be float32, float16 or bfloat16");
     FLY_REQUIRE(index_type == FLY_I32 || index_type == FLY_I64, "the targets must be int32 or int64");
-    FLY_REQUIRE(k >= 1 && k <= 1024, "k must lie in 1..1024");
     FLY_REQUIRE(w && (!rows || (x && index)), "null pointer");
     FLY_REQUIRE(!rows || loss || c.grads(), "neither loss nor gradients are wanted");
     FLY_REQUIRE(ldx >= d && ldw >= d && (!legal || ldl >= v) && (!gx || ldgx >= d) && (!gw || ldgw >= d), "rows overlap");

@@ -524,7 +524,7 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
  * outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums, but for rows of
  * x without a target, which count as zeros whatever they hold. */
 enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };
-size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t wanted);
+size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t k, int32_t wanted);
 int fly_readout_loss(const void *x_dev, int32_t type, int64_t ldx, int64_t rows, int64_t d, const void *w_dev, int64_t ldw,
                      int64_t v, const void *bias_dev, int32_t bias_type, const uint8_t *legal_dev, int64_t ldl,
                      const void *index_dev, int32_t index_type, const float *weight_dev, int32_t k, float *loss_dev,

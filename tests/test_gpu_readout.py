@@ -216,21 +216,32 @@ def test_no_rows():
 
 
 def test_rows_in_pieces():
-    """2^20 columns: 256 rows' logits fit a piece.  A row's results do not depend on its piece."""
+    """2^20 columns: 300 rows' logits fit no piece.  Against the formula in float64, each gradient within the roundings of u and
+    of itself, the steps of the logits that wait, and float32 sums of as many steps as the columns or rows have blocks of 32."""
     from chessfly.readout import readout_loss_and_grad
-    v, d, rows = 1 << 20, 4, 300
+    v, d, rows = 1 << 20, 4, 700
     g = torch.Generator(device=DEV).manual_seed(1)
     x, w = (torch.randn(n, d, generator=g, device=DEV).half() for n in (rows, v))
     b, t = torch.randn(v, generator=g, device=DEV), torch.randint(0, v, (rows,), generator=g, device=DEV)
     loss, grads = readout_loss_and_grad(x, w, b, t)
-    parts = [readout_loss_and_grad(x[i], w, b, t[i]) for i in (slice(0, 150), slice(150, rows))]
-    assert torch.equal(loss, torch.cat([p[0] for p in parts]))
-    assert torch.equal(grads.x, torch.cat([p[1].x for p in parts]))
-    # each part is rounded once more than the whole, and its u once on another scale
-    whole, apart = grads.weight.float(), sum(p[1].weight.float() for p in parts)
-    size = sum(p[1].weight.float().abs() for p in parts)
-    assert ((whole - apart).abs() <= 6 * 2.0 ** -11 * size + 2.0 ** -23).all()
-    assert torch.allclose(grads.bias, sum(p[1].bias for p in parts), rtol=1e-4, atol=1e-9)
+    want, gx = torch.zeros_like(loss, dtype=torch.float64), torch.zeros(rows, d, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(gx)
+    gw, gw_size, gb = torch.zeros(v, d, dtype=torch.float64, device=DEV), torch.zeros(v, d, dtype=torch.float64, device=DEV), 0.0
+    for i in range(0, rows, 100):
+        p = slice(i, i + 100)
+        z = x[p].double() @ w.double().t() + b.double()
+        want[p] = torch.logsumexp(z, 1) - z.gather(1, t[p, None])[:, 0]
+        u = torch.softmax(z, 1)
+        u.scatter_add_(1, t[p, None], torch.full((100, 1), -1.0, dtype=torch.float64, device=DEV))
+        gx[p], size[p] = u @ w.double(), u.abs() @ w.double().abs()
+        gw += u.t() @ x[p].double()
+        gw_size += u.abs().t() @ x[p].double().abs()
+        gb = gb + u.sum(0)
+    assert ((loss - want).abs() <= 1e-5 * want).all()
+    off = lambda a, e, s, n: ((a.double() - e).abs() / ((2.0 ** -11 + 2.0 ** -13 + (n / 32 + 64) * 2.0 ** -24) * s
+                                                        + 2.0 ** -11 * e.abs() + 2.0 ** -24)).max()
+    assert off(grads.x, gx, size, v) <= 1 and off(grads.weight, gw, gw_size, rows) <= 1
+    assert ((grads.bias - gb).abs() <= 2.0 ** -9 * (gb.abs() + 2 * torch.bincount(t, minlength=v))).all()
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
