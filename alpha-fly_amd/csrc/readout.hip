@@ -7,6 +7,7 @@
 //
 // Rows run in pieces whose logits and u fit a bounded workspace.
 #include "blocks.hpp"
+#include "readout.hpp"
 
 #include <cmath>
 
@@ -14,64 +15,33 @@ namespace fly {
 namespace {
 
 constexpr float kUnit = 16384.0f;            // u is multiplied as 2^14 u: float16 then holds it from 2^-28 on without loss
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kPieceBytes = (int64_t)1 << 31;   // of a piece of rows: its logits, u, and x laid out
 constexpr int64_t kPieceRows = (int64_t)1 << 19;    // a piece at most: tiles of rows are counted in 16 bits
 
-// Maxima over all rows that the scales of products over rows are taken by: bits of floats that are not negative.
+// The largest of the weights' units and of the rows' factors times theirs, by which products over columns and over rows are scaled.
 struct Maxima {
-  uint32_t weight, row;
+  float weight, row;
 };
-// Raises *to to a finite v.  A look first: thousands of rows' factors are alike, and as many atomics on one address took 12 ns
-// each.
-__device__ __forceinline__ void raise(uint32_t *to, float v) {
-  if (v > 0.0f && v <= 3.4028234663852886e38f &&
-      __float_as_uint(v) > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-    atomicMax(to, __float_as_uint(v));
-}
-
 // ---- targets ---------------------------------------------------------------------------------------------------------
-
-struct Targets {
-  const void *index;
-  int wide;               // index of 8 bytes
-  const float *weight;    // null: 1
-  int k;
-  const uint8_t *legal;
-  int64_t ldl;
-  int cols;
-};
-__device__ __forceinline__ int64_t target_at(const Targets &t, int64_t at) {
-  return t.wide ? static_cast<const int64_t *>(t.index)[at] : static_cast<const int32_t *>(t.index)[at];
-}
-// Whether entry j of a row counts: -1 none, -2 it lies past the columns, else its column.
-__device__ __forceinline__ int target_of(const Targets &t, int64_t row, int j, float &weight) {
-  const int64_t c = target_at(t, row * t.k + j);
-  weight = t.weight ? t.weight[row * t.k + j] : 1.0f;
-  if (c < 0 || weight == 0.0f) return -1;
-  if (c >= t.cols) return -2;
-  return t.legal && !t.legal[row * t.ldl + c] ? -1 : (int)c;
-}
 
 // A row's targets as the later kernels take them: each column once (-1: none) with its weights added up, and over the row the sum
 // of the weights and of their sizes.
 struct List {
-  int *column;      // (row, k)
+  int *column;      // (k, row)
   float *weight;
   float *logit;     // filled in by the product
   float2 *sums;     // (row)
+  int64_t ld;       // rows of a piece
   int k;
 };
 
-// By a wave; whether any target counts.
-__device__ __forceinline__ bool list_row(const Targets &t, const List &l, int64_t row, int lane) {
+// By a wave; the sum of the weights' sizes, 0 of a row where no target counts.
+__device__ __forceinline__ float list_row(const Targets &t, const List &l, int64_t row, int lane) {
   float share = 0.0f, whole = 0.0f;
-  bool some = false;
   for (int first = 0; first < t.k; first += 64) {
     const int j = first + lane;
     float a = 0.0f;
     int c = j < t.k ? target_of(t, row, j, a) : -1;
-    some |= c != -1;
     if (c == -2) share = whole = __builtin_nanf("");
     if (c < 0) a = 0.0f;
     share += a;
@@ -95,14 +65,14 @@ __device__ __forceinline__ bool list_row(const Targets &t, const List &l, int64_
         }
       }
     if (j < t.k) {
-      l.column[row * t.k + j] = again ? -1 : c;
-      l.weight[row * t.k + j] = sum;
+      l.column[j * l.ld + row] = again ? -1 : c;
+      l.weight[j * l.ld + row] = sum;
     }
   }
   share = wave_sum(share);
   whole = wave_sum(whole);
   if (lane == 0) l.sums[row] = make_float2(share, whole);
-  return __ballot(some) != 0;
+  return whole;
 }
 
 // ---- operands into blocks --------------------------------------------------------------------------------------------
@@ -127,30 +97,16 @@ struct Lay {
   float *bias_out;        // bias as float32, or null: no bias wanted
   Targets targets;        // of the rows (index null: none): one without any left counts as zeros, whatever it holds
   List list;
+  const float *row_scale;
+  float grad_scale;
+  float *factor, *turned_factor;   // B row_scale grad_scale of a row, and times its unit; or null
 };
 template <typename T>
 struct Lays {
-  Lay<T> of[2];           // the weight and the rows, or one of them and nothing (kt 0)
-  uint32_t *clear;
+  Lay<T> of[2];           // the weight and the rows, or the rows alone after nothing (kt 0)
 };
 
 constexpr int kSlab = 512;   // columns that pass through LDS at a time
-
-// Piece i of a row of `cols` as it lies in memory, zeros past its end.
-template <typename T>
-__device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int i, int64_t cols) {
-  constexpr int N = Piece<T>::N;
-  if ((int64_t)i * N + N <= cols) return load_whole(row, i);
-  Raw16 p = {};
-#pragma unroll
-  for (int e = 0; e < N - 1; ++e)
-    if ((int64_t)i * N + e < cols) {
-      const uint32_t b = to_bits(row[(int64_t)i * N + e]);
-      if constexpr (sizeof(T) == 4) p.v[e] = b;
-      else p.v[e / 2] |= b << (16 * (e & 1));
-    }
-  return p;
-}
 
 // 16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
 // its maximum to its planes; 0: rows of any length, read from memory once more for the maximum.
@@ -160,14 +116,17 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   constexpr int P = Multiplied<T>::P, N = Piece<T>::N, PIECES = kSlab / (64 * N), HELD = SLABS ? SLABS : 1;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][P][16][kSlab + 8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *lays.clear = 0u;
   const bool second = (int)blockIdx.x >= 2 * lays.of[0].kt;
   const Lay<T> &o = lays.of[second];
   const int group = blockIdx.x - (second ? 2 * lays.of[0].kt : 0);
   const int64_t row = (int64_t)group * 16 + wave;
   bool in = row < o.rows;
   const T *src = o.src + (in ? row : 0) * o.ld;
-  if (in && o.targets.index) in = list_row(o.targets, o.list, row, lane);
+  float whole = 0.0f;
+  if (in && o.targets.index) {
+    whole = list_row(o.targets, o.list, row, lane);
+    in = whole != 0.0f;   // NaN too
+  }
   Raw16 held[HELD][PIECES];
   auto fetch = [&](Raw16 (&p)[PIECES], int first) {
 #pragma unroll
@@ -201,12 +160,13 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   }
   if (o.bias_out && lane == 0) {
     float b = 0.0f;
-    if (row < o.rows && o.bias) {
-      if (o.bias_type == FLY_F32) b = static_cast<const float *>(o.bias)[row];
-      else if (o.bias_type == FLY_F16) b = static_cast<float>(static_cast<const _Float16 *>(o.bias)[row]);
-      else b = static_cast<float>(static_cast<const bhalf *>(o.bias)[row]);
-    }
+    if (row < o.rows && o.bias) b = bias_at(o.bias, o.bias_type, row);
     o.bias_out[row] = b;
+  }
+  if (o.factor && lane == 0 && row < o.rows) {
+    const float f = in ? whole * (o.row_scale ? o.row_scale[row] : 1.0f) * o.grad_scale : 0.0f;
+    o.factor[row] = f;
+    o.turned_factor[row] = f * unit;
   }
   const float inverse = 1.0f / unit;
   auto slab = [&](const Raw16 (&p)[PIECES], int first, int turn) {
@@ -264,19 +224,16 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
 
 // ---- logits ----------------------------------------------------------------------------------------------------------
 
-// How far a logit lies below its part's largest, in 16 bits: steps of 2^-12 up to 12, of 2^-8 from there to 76, and none at all
-// below.  The softmax then errs by 2^-13 relative where it is above 6e-6 of the part's largest, far less than 16-bit gradients
-// round by, and by 2^-9 where it is less.
+// How far a logit lies below its part's largest, in 65,535 steps up to 32, from where on it counts as none (its p is below 2e-14 of
+// the part's largest).  The softmax errs by half a step, 2^-12 relative, about half of what the rounding of its gradient to float16
+// may add.  v_cvt_pknorm makes two of them in an instruction.
+constexpr float kSteps = 65535.0f / 32.0f;
 constexpr uint32_t kNone = 65535;
-__device__ __forceinline__ uint32_t code_of(float gap) {
-  return gap < 12.0f ? (uint32_t)rintf(gap * 4096.0f) : 49152u + (uint32_t)fminf(rintf((gap - 12.0f) * 256.0f), 16383.0f);
-}
-__device__ __forceinline__ float gap_of(uint32_t code) {
-  return code < 49152u ? (float)code * (1.0f / 4096.0f) : 12.0f + (float)(code - 49152u) * (1.0f / 256.0f);
-}
 
 // What is left of a piece of rows' logits: each row's maximum and sum over a wave's columns, its targets' logits, and for the
-// gradients the logits themselves (Keep: float32, or their distance from the maximum in 16 bits).
+// gradients the logits themselves (Keep: float32, or their distance from the maximum in 16 bits).  Those lie in blocks of 16 rows x
+// 16 columns as the lanes hold them (lane l: row l & 15, columns 4 (l >> 4) .. + 3), so a wave's 64 columns leave as whole kilobytes
+// and are not turned over in LDS.
 enum Keep { kNothing, kFloats, kCodes };
 template <Keep KEEP>
 struct LogitsOut {
@@ -303,8 +260,13 @@ struct LogitsOut {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int c = n0 + 16 * j + quad, at = min(c, padded - 4);
-        const float4v b = *reinterpret_cast<const float4v *>(bias + at);
-        const float4v un = unit_n ? *reinterpret_cast<const float4v *>(unit_n + at) : float4v{1.0f, 1.0f, 1.0f, 1.0f};
+        v[j] = acc[j][i];
+        if (unit_n) {
+          const float4v un = *reinterpret_cast<const float4v *>(unit_n + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] * um * un[e];
+        }
+        v[j] += *reinterpret_cast<const float4v *>(bias + at);
         uint32_t shown = 0x01010101u;
         if (seen) {
           struct __attribute__((packed)) Bytes {
@@ -316,54 +278,57 @@ struct LogitsOut {
             for (int e = 0; e < 3; ++e)
               if (c + e < cols && !seen[c + e]) shown &= ~(1u << (8 * e));
         }
-        float l[4];
+        if (legal || n0 + 16 * FN > cols) {
+          float l[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = (unit_n ? acc[j][i][e] * um * un[e] : acc[j][i][e]) + b[e];
-          l[e] = c + e < cols && ((shown >> (8 * e)) & 0xffu) ? x : -INFINITY;
-          p.top = fmaxf(p.top, l[e]);
+          for (int e = 0; e < 4; ++e) l[e] = c + e < cols && (shown & (0xffu << (8 * e))) ? v[j][e] : -INFINITY;
+          v[j] = float4v{l[0], l[1], l[2], l[3]};
         }
-        v[j] = float4v{l[0], l[1], l[2], l[3]};
+        p.top = fmaxf(p.top, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
       }
-      // over the four lanes of the row
-      auto four = [](float x, auto &&f) {
-        const auto h = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
-        x = f(__int_as_float(h[0]), __int_as_float(h[1]));
-        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
-        return f(__int_as_float(w[0]), __int_as_float(w[1]));
-      };
-      p.top = four(p.top, [](float x, float y) { return fmaxf(x, y); });
+      p.top = over_four(p.top, [](float x, float y) { return fmaxf(x, y); });
       const float base = base_of(p.top);
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) p.sum += exp2_of((v[j][e] - base) * kLog2e);
-      p.sum = four(p.sum, [](float x, float y) { return x + y; });
-      if (lane < 16) {
-        if (m < rows) parts[m * ld_parts + part] = make_float2(p.top, p.sum);
-        turn[lane * PITCH + 16 * FN] = p.top;   // in the row's padding
-      }
-      turn_over<FN>(v, turn, lane, [&](int row, int c, const float4v &z4) {
-        const int mm = m0 + 16 * i + row;
-        if (mm >= rows || n0 + c >= padded) return;
-        if constexpr (KEEP == kFloats) {
-          *reinterpret_cast<float4v *>(static_cast<float *>(z) + (int64_t)mm * padded + n0 + c) = z4;
-        } else if constexpr (KEEP == kCodes) {
-          const float top = turn[row * PITCH + 16 * FN];
-          uint32_t w[4];
+      p.sum = over_four(p.sum, [](float x, float y) { return x + y; });
+      if (lane < 16 && m < rows) parts[m * ld_parts + part] = make_float2(p.top, p.sum);
+      if constexpr (KEEP != kNothing) {
+        const int64_t block = ((int64_t)(m0 >> 4) + i) * (padded >> 4) + (n0 >> 4);
+        if (m0 + 16 * i < rows)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = code_of(top - z4[e]);
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(z) + (int64_t)mm * padded + n0 + c) =
-              make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+          for (int j = 0; j < FN; ++j)
+            if (n0 + 16 * j < padded) {
+              if constexpr (KEEP == kFloats) {
+                static_cast<float4v *>(z)[(block + j) * 64 + lane] = v[j];
+              } else {
+                float g[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[e] = (p.top - v[j][e]) * (1.0f / 32.0f);
+                static_cast<uint2 *>(z)[(block + j) * 64 + lane] =
+                    make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(g[0], g[1])),
+                               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(g[2], g[3])));
+              }
+            }
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) *reinterpret_cast<float4v *>(turn + (lane & 15) * PITCH + 16 * j + quad) = v[j];
+      asm volatile("" ::: "memory");   // other lanes read what this one wrote: a wave's LDS accesses keep their order
+      // the targets among these columns: 4 entries of 16 rows in a load, 8 loads in flight
+      const int64_t mine = min(m, rows - 1);
+      for (int first = 0; first < list.k; first += 32) {
+        int at[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int entry = first + 4 * j + (lane >> 4);
+          at[j] = (entry < list.k ? list.column[entry * list.ld + mine] : -1) - n0;
         }
-      });
-      // the targets among these columns, 4 entries of 16 rows at a time
-      if (m < rows)
-        for (int j = lane >> 4; j < list.k; j += 4) {
-          const int64_t at = (int64_t)m * list.k + j;
-          const int c = list.column[at] - n0;
-          if (c >= 0 && c < 16 * FN) list.logit[at] = turn[(lane & 15) * PITCH + c];
-        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (m < rows && at[j] >= 0 && at[j] < 16 * FN)
+            list.logit[(first + 4 * j + (lane >> 4)) * list.ld + mine] = turn[(lane & 15) * PITCH + at[j]];
+      }
       asm volatile("" ::: "memory");
     }
   }
@@ -371,30 +336,34 @@ struct LogitsOut {
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
 
-// What a row's gradient is made of: p = exp2((z - top) log2 e - log_sum), u = share p - a / whole.
-struct RowInfo {
-  float top, log_sum, share, whole;
-};
-
-// A wave per row; a last workgroup finds the largest of the weights' units.
+// A wave per row; a first workgroup finds the largest factors.
 __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ parts, int64_t ld_parts, int count, int rows,
-                                                   const List l, const float *__restrict__ unit,
-                                                   const float *__restrict__ row_scale, float grad_scale,
-                                                   float *__restrict__ loss, RowInfo *__restrict__ info,
-                                                   float *__restrict__ factor, float *__restrict__ turned_factor,
-                                                   const float *__restrict__ unit_n, int cols, Maxima *__restrict__ maxima) {
-  const int lane = threadIdx.x & 63;
-  if (unit_n && blockIdx.x == gridDim.x - 1) {
-    __shared__ float share[4];
-    float most = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += 256) most = fmaxf(most, unit_n[c]);
-    most = wave_max(most);
-    if (lane == 0) share[threadIdx.x >> 6] = most;
+                                                   const List l, float *__restrict__ loss, RowInfo *__restrict__ info,
+                                                   const float *__restrict__ turned_factor, const float *__restrict__ unit_n,
+                                                   int cols, Maxima *__restrict__ maxima) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (info && blockIdx.x == 0) {
+    __shared__ float share[2][4];
+    float w = 0.0f, r = 0.0f;
+    auto raise = [](float &most, float v) {   // finite ones
+      v = fabsf(v);
+      if (v <= 3.4028234663852886e38f) most = fmaxf(most, v);
+    };
+    if (unit_n)
+#pragma unroll 8
+      for (int c = threadIdx.x; c < cols; c += 256) raise(w, unit_n[c]);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < rows; i += 256) raise(r, turned_factor[i]);
+    w = wave_max(w);
+    r = wave_max(r);
+    if (lane == 0) share[0][wave] = w, share[1][wave] = r;
     __syncthreads();
-    if (threadIdx.x == 0) maxima->weight = __float_as_uint(fmaxf(fmaxf(share[0], share[1]), fmaxf(share[2], share[3])));
+    if (threadIdx.x == 0)
+      *maxima = Maxima{fmaxf(fmaxf(share[0][0], share[0][1]), fmaxf(share[0][2], share[0][3])),
+                       fmaxf(fmaxf(share[1][0], share[1][1]), fmaxf(share[1][2], share[1][3]))};
     return;
   }
-  const int64_t row = blockIdx.x * (int64_t)4 + (threadIdx.x >> 6);
+  const int64_t row = (blockIdx.x - (info ? 1 : 0)) * (int64_t)4 + wave;
   if (row >= rows) return;
   const float2 sums = l.sums[row];
   PartSum p{-INFINITY, 0.0f};
@@ -408,18 +377,13 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ pa
   const float log_sum = log2_of(p.sum);
   float sum = 0.0f;
   for (int j = lane; j < l.k; j += 64)
-    if (l.column[row * l.k + j] >= 0)
-      sum += l.weight[row * l.k + j] * ((p.top - l.logit[row * l.k + j]) + kLn2 * log_sum);
+    if (l.column[j * l.ld + row] >= 0)
+      sum += l.weight[j * l.ld + row] * ((p.top - l.logit[j * l.ld + row]) + kLn2 * log_sum);
   sum = wave_sum(sum);
   if (lane) return;
   const bool some = sums.y != 0.0f;   // NaN too
   if (loss) loss[row] = !some ? 0.0f : sums.y == sums.y ? sum : sums.y;
-  if (!info) return;
-  info[row] = RowInfo{base_of(p.top), log_sum, some ? sums.x / sums.y : 0.0f, sums.y};
-  const float f = some ? sums.y * (row_scale ? row_scale[row] : 1.0f) * grad_scale : 0.0f, ft = unit ? f * unit[row] : f;
-  factor[row] = f;
-  turned_factor[row] = ft;
-  raise(&maxima->row, fabsf(ft));
+  if (info) info[row] = RowInfo{base_of(p.top), log_sum, some ? sums.x / sums.y : 0.0f, sums.y};
 }
 
 // ---- the logits' gradient --------------------------------------------------------------------------------------------
@@ -442,66 +406,63 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
   const int c0 = blockIdx.x * kGradCols, r0 = blockIdx.y * kGradRows;
   if (tid < kGradRows) {
     const int r = r0 + tid;
-    const float most = __uint_as_float(maxima->row);
+    const float most = maxima->row;
     f_row[tid] = r < rows ? factor[r] : 0.0f;
     ft_row[tid] = r < rows && most > 0.0f ? turned_factor[r] / most * kUnit : 0.0f;
   }
   if (tid >= 128) {
     const int c = c0 + tid - 128;
-    un_col[tid - 128] = P == 2 && c < cols ? unit_n[c] / __uint_as_float(maxima->weight) * kUnit : kUnit;
+    un_col[tid - 128] = P == 2 && c < cols ? unit_n[c] / maxima->weight * kUnit : kUnit;
   }
-  if constexpr (KEEP == kFloats) {
+  // 4 x 8 blocks of 16 x 16 logits, 8 for each wave
+  const int64_t block0 = (int64_t)(r0 >> 4) * (ldz >> 4) + (c0 >> 4);
+  if constexpr (KEEP == kCodes) {
+    // a part's largest p, times the share
+    const int r = tid >> 2, q = tid & 3;
+    float f = 0.0f;
+    if (r0 + r < rows && c0 + (q << shift) < cols && (q << shift) < kGradCols) {
+      const RowInfo i = info[r0 + r];
+      const float top = parts[(r0 + r) * ld_parts + (c0 >> shift) + q].x;
+      if (i.share != 0.0f) f = i.share * exp2_of((top - i.top) * kLog2e - i.log_sum);
+    }
+    f_part[r][q] = f;
+    __syncthreads();
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = (tid >> 5) + 8 * i, c = 4 * (tid & 31);
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (r0 + r < rows && c0 + c < cols) {
+  for (int i = 0; i < 8; ++i) {
+    const int rg = wave, cg = i, r = 16 * rg + (lane & 15), c = 16 * cg + 4 * (lane >> 4);
+    const int64_t at = (block0 + rg * (ldz >> 4) + cg) * 64 + lane;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (r0 + r < rows && c0 + c < ldz) {
+      if constexpr (KEEP == kFloats) {
         const RowInfo f = info[r0 + r];
-        const float4v at = *reinterpret_cast<const float4v *>(static_cast<const float *>(z) + (r0 + r) * ldz + c0 + c);
+        const float4v z4 = static_cast<const float4v *>(z)[at];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (c0 + c + e < cols && f.share != 0.0f) v[e] = f.share * exp2_of((at[e] - f.top) * kLog2e - f.log_sum);
-      }
-      *reinterpret_cast<float2 *>(&u[r][c]) = make_float2(v[0], v[1]);
-      *reinterpret_cast<float2 *>(&u[r][c + 2]) = make_float2(v[2], v[3]);
-    }
-  } else {
-    {
-      // a part's largest p, times the share
-      const int r = tid >> 2, q = tid & 3;
-      float f = 0.0f;
-      if (r0 + r < rows && c0 + (q << shift) < cols && (q << shift) < kGradCols) {
-        const RowInfo i = info[r0 + r];
-        const float top = parts[(r0 + r) * ld_parts + (c0 >> shift) + q].x;
-        if (i.share != 0.0f) f = i.share * exp2_of((top - i.top) * kLog2e - i.log_sum);
-      }
-      f_part[r][q] = f;
-    }
-    __syncthreads();
+          if (f.share != 0.0f) v[e] = f.share * exp2_of((z4[e] - f.top) * kLog2e - f.log_sum);
+      } else {
+        const uint2 w = static_cast<const uint2 *>(z)[at];
+        const float f = f_part[r][c >> shift];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (tid >> 4) + 16 * i, c = 8 * (tid & 15);
-      int4v w = {-1, -1, -1, -1};
-      if (r0 + r < rows && c0 + c < ldz) w = *reinterpret_cast<const int4v *>(static_cast<const uint16_t *>(z) + (r0 + r) * ldz + c0 + c);
-      const float f = f_part[r][c >> shift];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t a = (uint32_t)w[e] & 0xffffu, b = (uint32_t)w[e] >> 16;
-        *reinterpret_cast<float2 *>(&u[r][c + 2 * e]) =
-            make_float2(f * (a == kNone ? 0.0f : exp2_of(gap_of(a) * -kLog2e)), f * (b == kNone ? 0.0f : exp2_of(gap_of(b) * -kLog2e)));
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t code = e < 2 ? (w.x >> (16 * e)) & 0xffffu : (w.y >> (16 * (e - 2))) & 0xffffu;
+          v[e] = f * (code == kNone ? 0.0f : exp2_of((float)code * (-kLog2e / kSteps)));
+        }
       }
     }
+    *reinterpret_cast<float2 *>(&u[r][c]) = make_float2(v[0], v[1]);
+    *reinterpret_cast<float2 *>(&u[r][c + 2]) = make_float2(v[2], v[3]);
   }
   __syncthreads();
   // the targets among these columns, each once
-  for (int at = tid; at < min(kGradRows, rows - r0) * l.k; at += 256) {
-    const int64_t from = (int64_t)r0 * l.k + at;
-    const int c = l.column[from];
-    if (c < c0 || c >= c0 + kGradCols) continue;
-    const int r = at / l.k;
-    const RowInfo f = info[r0 + r];
-    u[r][c - c0] = f.share * exp2_of((l.logit[from] - f.top) * kLog2e - f.log_sum) - l.weight[from] / f.whole;
-  }
+  if (r0 + lane < rows)
+    for (int j = wave; j < l.k; j += 4) {
+      const int64_t from = j * l.ld + r0 + lane;
+      const int c = l.column[from];
+      if (c < c0 || c >= c0 + kGradCols) continue;
+      const RowInfo f = info[r0 + lane];
+      u[lane][c - c0] = f.share * exp2_of((l.logit[from] - f.top) * kLog2e - f.log_sum) - l.weight[from] / f.whole;
+    }
   __syncthreads();
   typedef uint32_t words[4];
 #pragma unroll
@@ -583,7 +544,7 @@ __global__ __launch_bounds__(1024) void k_bias_grad(const float *__restrict__ su
 template <typename T>
 struct GradOut {
   const float *row;          // or null
-  const uint32_t *scale;     // a maximum's bits, or null
+  const float *scale;        // a maximum, or null
   int rows, cols;
   const float *before;
   float *after;              // or null: the last piece, into out
@@ -591,7 +552,7 @@ struct GradOut {
   T *out;
   int64_t ld;
   float *share;              // (part, row, column) or null
-  __device__ __forceinline__ float unit() const { return (scale ? __uint_as_float(*scale) : 1.0f) / kUnit; }
+  __device__ __forceinline__ float unit() const { return (scale ? *scale : 1.0f) / kUnit; }
   __device__ __forceinline__ void put(int m, int n, const float4v &sum, float unit) const {
     const float f = row ? unit * row[m] : unit;
     float4v w;
@@ -656,12 +617,6 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 // ---- the call --------------------------------------------------------------------------------------------------------
 
 
-struct Call {
-  int32_t type;
-  int64_t rows, d, v, k;
-  bool gx, gw, gb;
-  bool grads() const { return gx || gw || gb; }
-};
 
 // The workgroup's tile of a product of m x n, n x m rows of it.  One plane: 256 x 256 from 128 tiles on, 128 x 128 from 100 on,
 // else 64 x 64; two planes: 128 x 192 from 150 tiles on, else 64 x 64.
@@ -768,28 +723,6 @@ struct Space {
   }
 };
 
-struct Given {
-  const void *x, *w, *bias;
-  int64_t ldx, ldw;
-  int32_t bias_type;
-  Targets targets;
-  const float *row_scale;
-  float grad_scale;
-  float *loss;
-  void *gx, *gw, *gb;
-  int64_t ldgx, ldgw;
-};
-
-template <typename F>
-void by_type(int32_t type, const char *what, F &&f) {
-  switch (type) {
-    case FLY_F32: f(float{}); break;
-    case FLY_F16: f(_Float16{}); break;
-    case FLY_BF16: f(bhalf{}); break;
-    default: FLY_REQUIRE(false, what);
-  }
-}
-
 template <typename T>
 void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
   using H = typename Multiplied<T>::H;
@@ -811,14 +744,15 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     if (t.weight) t.weight += first * t.k;
     if (t.legal) t.legal += first * t.ldl;
     const List list{reinterpret_cast<int *>(at(s.column)), floats(s.weight), floats(s.logit),
-                    reinterpret_cast<float2 *>(at(s.list_sums)), t.k};
+                    reinterpret_cast<float2 *>(at(s.list_sums)), s.piece, t.k};
     Lays<T> lays{};
     if (!first)
       lays.of[0] = Lay<T>{static_cast<const T *>(g.w), g.ldw, c.v, c.d, (int)s.db, (int)s.vb, blocks(s.w),
-                          c.gx ? blocks(s.wt) : nullptr, unit_w, g.bias, g.bias_type, floats(s.bias), Targets{}, List{}};
+                          c.gx ? blocks(s.wt) : nullptr, unit_w, g.bias, g.bias_type, floats(s.bias), Targets{}, List{}, nullptr, 0.0f, nullptr, nullptr};
     lays.of[1] = Lay<T>{static_cast<const T *>(g.x) + first * g.ldx, g.ldx, rows, c.d, (int)s.db, rb, blocks(s.x),
-                        c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, 0, nullptr, t, list};
-    lays.clear = &maxima->row;
+                        c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, 0, nullptr, t, list,
+                        g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, c.grads() ? floats(s.factor) : nullptr,
+                        floats(s.turned)};
     const unsigned groups = (unsigned)(2 * (lays.of[0].kt + rb));
     auto lay = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, st, lays); };
     const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // a row of up to 3,072 columns stays in registers
@@ -841,9 +775,8 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     constexpr Keep KEPT = P == 1 ? kCodes : kFloats;
     if (c.grads()) logits(std::integral_constant<Keep, KEPT>{});
     else logits(std::integral_constant<Keep, kNothing>{});
-    hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4) + (P == 2)), dim3(256), 0, st, stat, s.parts, parts, rows, list,
-                       unit_x, g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, g.loss ? g.loss + first : nullptr,
-                       info, floats(s.factor), floats(s.turned), unit_w, (int)c.v, maxima);
+    hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4) + c.grads()), dim3(256), 0, st, stat, s.parts, parts, rows, list,
+                       g.loss ? g.loss + first : nullptr, info, floats(s.turned), unit_w, (int)c.v, maxima);
     check_launch("read-out loss");
     if (!c.grads()) continue;
     hipLaunchKernelGGL((k_logits_grad<H, P, KEPT>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, at(s.z),
@@ -894,7 +827,9 @@ void require_call(const Call &c) {
               "size out of range");
   FLY_REQUIRE(c.k >= 1 && c.k <= 1024, "k must lie in 1..1024");
 }
-size_t call_ws(const Call &c) { return c.rows ? Space(c, c.type == FLY_F32 ? 2 : 1).bytes : 0; }
+size_t call_ws(const Call &c) {
+  return !c.rows ? 0 : few_rows(c) ? few_ws(c) : Space(c, c.type == FLY_F32 ? 2 : 1).bytes;
+}
 
 }  // namespace
 }  // namespace fly
@@ -941,6 +876,7 @@ extern "C" int fly_readout_loss(const void *x, int32_t type, int64_t ldx, int64_
     const Given g{x, w, bias, ldx, ldw, bias_type,
                   Targets{index, index_type == FLY_I64, weight, k, legal, ldl, (int)v}, row_scale, grad_scale, loss, gx, gw, gb,
                   ldgx, ldgw};
-    by_type(type, "", [&](auto t) { run<decltype(t)>(c, g, static_cast<char *>(ws), st); });
+    if (few_rows(c)) run_few(c, g, static_cast<char *>(ws), st);
+    else by_type(type, "", [&](auto t) { run<decltype(t)>(c, g, static_cast<char *>(ws), st); });
   });
 }

@@ -1,0 +1,101 @@
+// What the two ways of the read-out loss share: its arguments, targets and rows.
+#pragma once
+
+#include "rows.hpp"
+
+namespace fly {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Call {
+  int32_t type;
+  int64_t rows, d, v, k;
+  bool gx, gw, gb;
+  bool grads() const { return gx || gw || gb; }
+};
+
+struct Targets {
+  const void *index;
+  int wide;               // index of 8 bytes
+  const float *weight;    // null: 1
+  int k;
+  const uint8_t *legal;
+  int64_t ldl;
+  int cols;
+};
+__device__ __forceinline__ int64_t target_at(const Targets &t, int64_t at) {
+  return t.wide ? static_cast<const int64_t *>(t.index)[at] : static_cast<const int32_t *>(t.index)[at];
+}
+// Whether entry j of a row counts: -1 none, -2 it lies past the columns, else its column.
+__device__ __forceinline__ int target_of(const Targets &t, int64_t row, int j, float &weight) {
+  const int64_t c = target_at(t, row * t.k + j);
+  weight = t.weight ? t.weight[row * t.k + j] : 1.0f;
+  if (c < 0 || weight == 0.0f) return -1;
+  if (c >= t.cols) return -2;
+  return t.legal && !t.legal[row * t.ldl + c] ? -1 : (int)c;
+}
+
+struct Given {
+  const void *x, *w, *bias;
+  int64_t ldx, ldw;
+  int32_t bias_type;
+  Targets targets;
+  const float *row_scale;
+  float grad_scale;
+  float *loss;
+  void *gx, *gw, *gb;
+  int64_t ldgx, ldgw;
+};
+
+// What a row's gradient is made of: p = exp2((z - top) log2 e - log_sum), u = share p - a / whole.
+struct RowInfo {
+  float top, log_sum, share, whole;
+};
+
+// Piece i of a row of `cols` as it lies in memory, zeros past its end.
+template <typename T>
+__device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int i, int64_t cols) {
+  constexpr int N = Piece<T>::N;
+  if ((int64_t)i * N + N <= cols) return load_whole(row, i);
+  Raw16 p = {};
+#pragma unroll
+  for (int e = 0; e < N - 1; ++e)
+    if ((int64_t)i * N + e < cols) {
+      const uint32_t b = to_bits(row[(int64_t)i * N + e]);
+      if constexpr (sizeof(T) == 4) p.v[e] = b;
+      else p.v[e / 2] |= b << (16 * (e & 1));
+    }
+  return p;
+}
+
+// The sum or maximum over the four lanes that hold a row of a matrix instruction's result (lane & 15 alike), in each of them.
+template <typename F>
+__device__ __forceinline__ float over_four(float x, F &&f) {
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+  x = f(__int_as_float(h[0]), __int_as_float(h[1]));
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+  return f(__int_as_float(w[0]), __int_as_float(w[1]));
+}
+
+__device__ __forceinline__ float bias_at(const void *bias, int type, int64_t c) {
+  if (type == FLY_F32) return static_cast<const float *>(bias)[c];
+  if (type == FLY_F16) return static_cast<float>(static_cast<const _Float16 *>(bias)[c]);
+  return static_cast<float>(static_cast<const bhalf *>(bias)[c]);
+}
+
+template <typename F>
+inline void by_type(int32_t type, const char *what, F &&f) {
+  switch (type) {
+    case FLY_F32: f(float{}); break;
+    case FLY_F16: f(_Float16{}); break;
+    case FLY_BF16: f(bhalf{}); break;
+    default: FLY_REQUIRE(false, what);
+  }
+}
+
+// Few rows, without laying the operands out (readout_few.hip): whether a call goes that way, and what it takes.
+bool few_rows(const Call &c);
+size_t few_ws(const Call &c);
+void run_few(const Call &c, const Given &g, char *ws, hipStream_t st);
+
+}  // namespace fly

@@ -18,9 +18,9 @@ U = 2.0 ** -24
 OPERAND = {"float32": 3 * 2.0 ** -22, "float16": 0.0, "bfloat16": 0.0}
 # u as it is multiplied: one rounding to the 16-bit type, or two halves; float16 holds 2^14 u down to 2^-24 steps, the low half 2^11 finer.
 HELD = {"float32": 2.0 ** -22, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
-# With 16-bit operands the logits wait for their rows' sums in steps of 2^-12 below their part's largest, up to 12 below it, of 2^-8
-# up to 76 below, and count as none further down: p errs by e^(half a step) - 1, or by e^-76.
-STEP = 2.0 ** -13 * (1 + 2.0 ** -12), 2.0 ** -9 * (1 + 2.0 ** -8)
+# With 16-bit operands the logits wait for their rows' sums as their distance from their part's largest, in 65,535 steps up to 32 and
+# as none from there on: p errs by e^(half a step) - 1, or by e^-32 of the part's largest.
+STEP = 16.0 / 65535 * (1 + 2.0 ** -11)
 HELD_LEAST = {"float32": 2.0 ** -49, "float16": 2.0 ** -38, "bfloat16": 2.0 ** -120}
 
 
@@ -99,7 +99,7 @@ def bounds(x, w, b, index, dtype, weight=None, legal=None, scale=None, bias_dtyp
     ep = p * np.expm1(ez + e_lse[:, None] + 6 * U * (gap + 1) + 2.0 ** -21)
     if dtype != "float32":
         listed = t != 0                      # the targets' own logits are kept in float32
-        ep = ep + np.where(listed, 0.0, p * np.where(gap < 12, STEP[0], STEP[1]) * 1.01 + np.exp(-76.0))
+        ep = ep + np.where(listed, 0.0, p * STEP * 1.01 + np.exp(-32.0))
     u_size = np.abs(a[:, None] * p - t)
     eg = np.abs(a)[:, None] * ep + (n + 8) * U * (np.abs(a)[:, None] * p + np.abs(t))
     held = HELD[dtype] * (u_size + eg) + 4 * U * u_size + 1e-38

@@ -13,7 +13,10 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 TYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.bfloat16}
 SIZES = [(1, 1, 1), (1, 70, 333), (2, 5, 3), (3, 33, 31), (16, 32, 32), (17, 31, 33), (31, 65, 129), (33, 64, 128), (64, 100, 257),
-         (65, 513, 300), (130, 257, 1000), (257, 40, 520)]
+         (65, 513, 300), (130, 257, 1000), (257, 40, 520), (300, 1, 1), (259, 33, 31), (310, 97, 129), (385, 600, 200), (513, 31, 2000)]
+
+
+FEW, MANY = 40, 280    # rows that take the kernels of few rows, and those of many, whatever the type
 
 
 def case(rows, d, v, dtype, seed=0, k=1, legal=False, bias="own", index=torch.int64, spread=2.0):
@@ -82,25 +85,28 @@ def test_visits_over_legal_moves(rows, d, v, dtype, k):
     check(call(*t, grad_scale=2.0, row_scale=scale.to(DEV)), t, dtype, 2.0 * scale.double().numpy())
 
 
+@pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_weights_of_both_signs_without_bias(dtype):
-    t = list(case(40, 50, 60, dtype, k=4, bias=None))
-    t[4] = torch.randn(40, 4, generator=torch.Generator().manual_seed(3)) * 100
+def test_weights_of_both_signs_without_bias(dtype, rows):
+    t = list(case(rows, 50, 60, dtype, k=4, bias=None))
+    t[4] = torch.randn(rows, 4, generator=torch.Generator().manual_seed(3)) * 100
     check(call(*t), t, dtype)
 
 
+@pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_confident_rows(dtype):
+def test_confident_rows(dtype, rows):
     """Logits of up to some 100, whose softmax is all but 0 and 1."""
-    t = case(60, 64, 200, dtype, seed=5, k=3, spread=30.0)
+    t = case(rows, 64, 200, dtype, seed=5, k=3, spread=30.0)
     check(call(*t), t, dtype)
 
 
-def test_rows_and_weights_of_very_different_size():
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_rows_and_weights_of_very_different_size(rows):
     """float32 rows are multiplied by units of their own."""
-    x, w, b, index, weight, legal = case(50, 40, 90, "float32", seed=9, k=3)
+    x, w, b, index, weight, legal = case(rows, 40, 90, "float32", seed=9, k=3)
     g = torch.Generator().manual_seed(2)
-    x = x * 10.0 ** torch.randint(-6, 1, (50, 1), generator=g)
+    x = x * 10.0 ** torch.randint(-6, 1, (rows, 1), generator=g)
     w = w * 10.0 ** torch.randint(-6, 1, (90, 1), generator=g)
     t = (x, w, b, index, weight, legal)
     check(call(*t), t, "float32")
@@ -108,57 +114,61 @@ def test_rows_and_weights_of_very_different_size():
     check(call(*t), t, "float32")
 
 
+@pytest.mark.parametrize("rows", [37, 277])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_strides(dtype):
+def test_strides(dtype, rows):
     """Rows apart, columns apart, a transposed weight, every second target, a mask that is a part of a larger one."""
     from chessfly.readout import Visits, readout_loss_and_grad
-    x, w, b, index, weight, legal = on(*case(37, 70, 150, dtype, k=4, legal=True))
+    x, w, b, index, weight, legal = on(*case(rows, 70, 150, dtype, k=4, legal=True))
     want = readout_loss_and_grad(x, w, b, Visits(index, weight), legal=legal)
-    wide = torch.zeros(37, 101, dtype=x.dtype, device=DEV)
+    wide = torch.zeros(rows, 101, dtype=x.dtype, device=DEV)
     wide[:, 3:73] = x
     apart = torch.zeros(150, 140, dtype=x.dtype, device=DEV)
     apart[:, ::2] = w
-    large = torch.zeros(40, 155, dtype=torch.bool, device=DEV)
-    large[1:38, 2:152] = legal
-    idx = torch.zeros(37, 8, dtype=index.dtype, device=DEV)
+    large = torch.zeros(rows + 3, 155, dtype=torch.bool, device=DEV)
+    large[1:rows + 1, 2:152] = legal
+    idx = torch.zeros(rows, 8, dtype=index.dtype, device=DEV)
     idx[:, ::2] = index
     bb = torch.zeros(300, dtype=b.dtype, device=DEV)
     bb[::2] = b
     variants = [(wide[:, 3:73], w, b, index, weight, legal), (x, w.t().contiguous().t(), b, index, weight, legal),
-                (x, apart[:, ::2], bb[::2], idx[:, ::2], weight.t().contiguous().t(), large[1:38, 2:152]),
+                (x, apart[:, ::2], bb[::2], idx[:, ::2], weight.t().contiguous().t(), large[1:rows + 1, 2:152]),
                 (x, w, b, index, weight, legal.to(torch.uint8))]
     for x_, w_, b_, i_, a_, l_ in variants:
         got = readout_loss_and_grad(x_, w_, b_, Visits(i_, a_), legal=l_)
         assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
 
 
-def test_broadcast_rows():
+@pytest.mark.parametrize("rows", [20, 300])
+def test_broadcast_rows(rows):
     """One row for all, and one mask: strides of 0."""
     from chessfly.readout import readout_loss_and_grad
-    x, w, b, index, _, legal = on(*case(20, 33, 47, "float32", legal=True))
+    x, w, b, index, _, legal = on(*case(rows, 33, 47, "float32", legal=True))
     legal[0] = True
-    a = readout_loss_and_grad(x[:1].expand(20, 33), w, b, index, legal=legal[:1].expand(20, 47))
-    e = readout_loss_and_grad(x[:1].repeat(20, 1), w, b, index, legal=legal[:1].repeat(20, 1))
+    a = readout_loss_and_grad(x[:1].expand(rows, 33), w, b, index, legal=legal[:1].expand(rows, 47))
+    e = readout_loss_and_grad(x[:1].repeat(rows, 1), w, b, index, legal=legal[:1].repeat(rows, 1))
     assert torch.equal(a[0], e[0]) and all(torch.equal(p, q) for p, q in zip(a[1], e[1]))
 
 
+@pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_a_row_that_is_not_finite_stays_its_own(dtype):
-    t = list(case(40, 50, 60, dtype, k=3))
+def test_a_row_that_is_not_finite_stays_its_own(dtype, rows):
+    t = list(case(rows, 50, 60, dtype, k=3))
     t[3] = t[3].abs()
     want = call(*t)
     for bad in (float("nan"), float("inf")):
         x = t[0].clone()
         x[11, 5] = bad
         loss, grads = call(x, *t[1:])
-        others = torch.arange(40) != 11
+        others = torch.arange(rows) != 11
         assert loss[11].isnan() and grads.x[11].isnan().any()
         assert torch.equal(loss[others], want[0][others]) and torch.equal(grads.x[others], want[1].x[others])
 
 
+@pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_rows_left_out_may_hold_anything(dtype):
-    t = list(case(40, 50, 60, dtype, k=3))
+def test_rows_left_out_may_hold_anything(dtype, rows):
+    t = list(case(rows, 50, 60, dtype, k=3))
     t[3][10:14] = -1
     want = call(*t)
     x = t[0].clone()
@@ -168,10 +178,11 @@ def test_rows_left_out_may_hold_anything(dtype):
     assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
 
 
+@pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_hidden_columns_may_hold_anything(dtype):
+def test_hidden_columns_may_hold_anything(dtype, rows):
     """NaN and infinite biases of columns that no row sees; a type's lowest value in place of a mask."""
-    x, w, b, index, weight, legal = case(40, 50, 60, dtype, k=3, legal=True)
+    x, w, b, index, weight, legal = case(rows, 50, 60, dtype, k=3, legal=True)
     hidden = torch.arange(60) % 5 == 2
     legal = legal & ~hidden
     want = call(x, w, b, index, weight, legal)
@@ -180,18 +191,19 @@ def test_hidden_columns_may_hold_anything(dtype):
         assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
     seen = ~hidden[index.clamp(min=0)]
     weight = torch.where(seen, weight, 0.0)
-    want = call(x, w, b, index, weight, (~hidden).expand(40, 60))
+    want = call(x, w, b, index, weight, (~hidden).expand(rows, 60))
     got = call(x, w, torch.where(hidden, torch.tensor(torch.finfo(b.dtype).min, dtype=b.dtype), b), index, weight, None)
     assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
 
 
-def test_targets_past_the_columns():
-    t = list(case(40, 50, 60, "float32", k=3))
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_targets_past_the_columns(rows):
+    t = list(case(rows, 50, 60, "float32", k=3))
     want = call(*t)
     t[3][7, 1] = 60
     t[3][9, 0] = 2 ** 40
     loss, grads = call(*t)
-    bad = torch.isin(torch.arange(40), torch.tensor([7, 9]))
+    bad = torch.isin(torch.arange(rows), torch.tensor([7, 9]))
     assert loss[bad].isnan().all() and grads.x[bad].isnan().all()
     assert torch.equal(loss[~bad], want[0][~bad]) and torch.equal(grads.x[~bad], want[1].x[~bad])
 
@@ -244,13 +256,14 @@ def test_rows_in_pieces():
     assert ((grads.bias - gb).abs() <= 2.0 ** -9 * (gb.abs() + 2 * torch.bincount(t, minlength=v))).all()
 
 
+@pytest.mark.parametrize("rows", [50, 300])
 @pytest.mark.parametrize("dtype", list(TYPES))
-def test_autograd(dtype):
+def test_autograd(dtype, rows):
     """The gradients of readout_loss are those of readout_loss_and_grad, for the leaves that want one."""
     from chessfly.readout import Visits, readout_loss
-    t = case(50, 33, 70, dtype, k=3, legal=True)
+    t = case(rows, 33, 70, dtype, k=3, legal=True)
     x, w, b, index, weight, legal = on(*t)
-    loss, grads = call(*t, grad_scale=1 / 50)
+    loss, grads = call(*t, grad_scale=1 / rows)
     for wants in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
         leaves = [p.clone().requires_grad_(bool(n)) for p, n in zip((x, w, b), wants)]
         out = readout_loss(*leaves, Visits(index, weight), legal)
@@ -286,7 +299,7 @@ def test_autograd_by_rows_and_shared_leaves():
         readout_loss(forward_ad.make_dual(x, torch.ones_like(x)), w.detach(), b, index)
 
 
-@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("rows", [3, 200, 400])
 def test_in_a_graph(rows):
     """Captured with its workspace and replayed between eager calls."""
     from chessfly.readout import readout_loss
@@ -334,10 +347,11 @@ def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
         assert torch.equal(grad, 2 * eager)
 
 
-def test_streams_and_repeats():
+@pytest.mark.parametrize("rows", [60, 500])
+def test_streams_and_repeats(rows):
     """The same bits on another stream and on every call."""
     from chessfly.readout import Visits, readout_loss_and_grad
-    x, w, b, index, weight, legal = on(*case(500, 300, 700, "bfloat16", k=4, legal=True))
+    x, w, b, index, weight, legal = on(*case(rows, 300, 700, "bfloat16", k=4, legal=True))
     want = readout_loss_and_grad(x, w, b, Visits(index, weight), legal=legal)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(3)]
