@@ -132,7 +132,8 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       const int i = first / N + lane + 64 * j;
-      p[j] = in && (int64_t)i * N < o.cols ? load_raw(src, i, o.cols) : Raw16{};
+      if constexpr (SLABS > 0) p[j] = load_clamped(src, i, (int)o.cols);
+      else p[j] = in && (int64_t)i * N < o.cols ? load_raw(src, i, o.cols) : Raw16{};
     }
   };
   if constexpr (SLABS > 0)
@@ -148,6 +149,7 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
         for (int j = 0; j < PIECES; ++j)
 #pragma unroll
           for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(element<T>(held[s][j], e)));
+      if (!in) top = 0.0f;
     } else if (in) {
       for (int64_t i = lane; i * N < o.cols; i += 64) {
         const Raw16 p = load_raw(src, (int)i, o.cols);
@@ -169,8 +171,16 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
     o.turned_factor[row] = f * unit;
   }
   const float inverse = 1.0f / unit;
-  auto slab = [&](const Raw16 (&p)[PIECES], int first, int turn) {
+  auto slab = [&](Raw16 (&p)[PIECES], int first, int turn) {
     auto &part = lds[turn];
+    if constexpr (SLABS > 0) {
+      if (first + kSlab > o.cols)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) settle<T>(p[j], first / N + lane + 64 * j, (int)o.cols);
+      if (!in)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) p[j] = Raw16{};
+    }
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {
       const int at = (lane + 64 * j) * N;
@@ -756,7 +766,8 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     const unsigned groups = (unsigned)(2 * (lays.of[0].kt + rb));
     auto lay = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, st, lays); };
     const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // a row of up to 3,072 columns stays in registers
-    if (slabs <= 2) lay(k_lay<T, 2>);
+    if (c.d < Piece<T>::N) lay(k_lay<T, 0>);
+    else if (slabs <= 2) lay(k_lay<T, 2>);
     else if (slabs <= 6) lay(k_lay<T, 6>);
     else lay(k_lay<T, 0>);
     check_launch("read-out operands");

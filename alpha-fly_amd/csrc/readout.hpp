@@ -68,6 +68,27 @@ __device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int i, int6
   return p;
 }
 
+// The same in two steps, for loads that are to be in flight together: with a branch around its tail, each load is waited for where
+// the branches meet.  Rows have a whole piece at least; a piece past the end holds the row's last elements until it is settled.
+template <typename T>
+__device__ __forceinline__ Raw16 load_clamped(const T *__restrict__ row, int i, int cols) {
+  return *reinterpret_cast<const Raw16 *>(row + min(i * Piece<T>::N, cols - Piece<T>::N));
+}
+template <typename T>
+__device__ __forceinline__ void settle(Raw16 &p, int i, int cols) {
+  const int past = i * Piece<T>::N + Piece<T>::N - cols;   // elements
+  if (past <= 0) return;
+  const int bits = past * 8 * (int)sizeof(T);
+  uint64_t lo = p.v[0] | (uint64_t)p.v[1] << 32, hi = p.v[2] | (uint64_t)p.v[3] << 32;
+  if (bits >= 128) lo = hi = 0;
+  else if (bits >= 64) lo = hi >> (bits - 64), hi = 0;
+  else lo = lo >> bits | hi << (64 - bits), hi >>= bits;
+  p.v[0] = (uint32_t)lo;
+  p.v[1] = (uint32_t)(lo >> 32);
+  p.v[2] = (uint32_t)hi;
+  p.v[3] = (uint32_t)(hi >> 32);
+}
+
 // The sum or maximum over the four lanes that hold a row of a matrix instruction's result (lane & 15 alike), in each of them.
 template <typename F>
 __device__ __forceinline__ float over_four(float x, F &&f) {

@@ -23,85 +23,117 @@ __device__ __forceinline__ float4v product4(float a, float b, float4v c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// 16 NB columns x 16 MB rows.  A wave takes every 8th step of 64 bytes of each row, U of them in flight.
-template <typename T, int NB, int MB>
+// 16 columns x 16 MB rows.  Rounds of BYTES of each row pass through LDS, so that a wave loads whole kilobytes of a row: read as the
+// matrix cores take them, 64 bytes of 16 rows at a time, 4,168 x 2,333 float32 took 18 us at best.  Of the weights two rounds are
+// in flight while a third is multiplied, of the rows, which the L2 holds, one.
+template <typename T, int MB, int BYTES>
 __global__ __launch_bounds__(64 * kWaves) void k_few_logits(const T *__restrict__ x, int64_t ldx, int rows,
                                                             const T *__restrict__ w, int64_t ldw, int v, int d,
                                                             const void *__restrict__ bias, int bias_type,
                                                             const uint8_t *__restrict__ legal, int64_t ldl,
                                                             float *__restrict__ z, int64_t ldz, float2 *__restrict__ parts,
                                                             int64_t ld_parts) {
-  constexpr int N = Piece<T>::N, U = NB + MB <= 3 ? 8 : 4;
-  __shared__ float4v sums[kWaves][NB * MB][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int v0 = blockIdx.x * 16 * NB, r0 = blockIdx.y * 16 * MB;
-  const T *wr[NB], *xr[MB];
+  constexpr int N = Piece<T>::N, PER = BYTES / 16, PITCH = BYTES + 16;   // pieces of a row in a round
+  constexpr int LOADS = 16 * PER / (64 * kWaves), STEPS = PER / 4 / kWaves;   // a thread's of 16 rows; a wave's steps of 4 pieces
+  static_assert(LOADS >= 1 && STEPS >= 1, "a round is shared by all waves");
+  __shared__ __attribute__((aligned(16))) char lds[16 * (1 + MB) * PITCH];
+  static_assert(sizeof(lds) >= kWaves * MB * 1024, "the sums fit in the operands' place");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int v0 = blockIdx.x * 16, r0 = blockIdx.y * 16 * MB;
+  float4v acc[MB];
 #pragma unroll
-  for (int n = 0; n < NB; ++n) wr[n] = w + min(v0 + 16 * n + (lane & 15), v - 1) * ldw;   // rows past the last repeat it
+  for (int m = 0; m < MB; ++m) acc[m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+  const int rounds = (d + PER * N - 1) / (PER * N);
+  auto piece = [&](const T *base, int64_t ld, int row, int last, int at) {   // rows past the last repeat it
+    return load_clamped(base + min(row, last) * ld, at, d);
+  };
+  Raw16 a[2][LOADS], b[MB][LOADS];
+  auto load_w = [&](Raw16 (&to)[LOADS], int round) {
 #pragma unroll
-  for (int m = 0; m < MB; ++m) xr[m] = x + min(r0 + 16 * m + (lane & 15), rows - 1) * ldx;
-  float4v acc[NB][MB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int m = 0; m < MB; ++m) acc[n][m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-  const int steps = (d + 4 * N - 1) / (4 * N);
-  for (int first = wave; first < steps; first += kWaves * U) {
-    Raw16 a[U][NB], b[U][MB];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int piece = 4 * (first + kWaves * u) + (lane >> 4);
-#pragma unroll
-      for (int n = 0; n < NB; ++n) a[u][n] = piece * N < d ? load_raw(wr[n], piece, d) : Raw16{};
-#pragma unroll
-      for (int m = 0; m < MB; ++m) b[u][m] = piece * N < d ? load_raw(xr[m], piece, d) : Raw16{};
+    for (int i = 0; i < LOADS; ++i) {
+      const int at = tid + 64 * kWaves * i;
+      to[i] = piece(w, ldw, v0 + at / PER, v - 1, round * PER + at % PER);
     }
+  };
+  auto load_x = [&](int round) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (first + kWaves * u >= steps) break;   // the same for the whole wave
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int i = 0; i < LOADS; ++i) {
+        const int at = tid + 64 * kWaves * i;
+        b[m][i] = piece(x, ldx, r0 + 16 * m + at / PER, rows - 1, round * PER + at % PER);
+      }
+  };
+  auto put = [&](Raw16 (&from)[LOADS], int block, int round) {
+    if (round == rounds - 1)
 #pragma unroll
-        for (int m = 0; m < MB; ++m) {
-          if constexpr (N == 4) {
+      for (int i = 0; i < LOADS; ++i) settle<T>(from[i], round * PER + (tid + 64 * kWaves * i) % PER, d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[n][m] = product4(__uint_as_float(a[u][n].v[e]), __uint_as_float(b[u][m].v[e]), acc[n][m]);
-          } else {
-            acc[n][m] = product16<T>(__builtin_bit_cast(int4v, a[u][n]), __builtin_bit_cast(int4v, b[u][m]), acc[n][m]);
-          }
+    for (int i = 0; i < LOADS; ++i) {
+      const int at = tid + 64 * kWaves * i;
+      *reinterpret_cast<int4v *>(lds + (16 * block + at / PER) * PITCH + 16 * (at % PER)) = __builtin_bit_cast(int4v, from[i]);
+    }
+  };
+  auto get = [&](int block, int step) {
+    return *reinterpret_cast<const int4v *>(lds + (16 * block + (lane & 15)) * PITCH + 64 * (wave * STEPS + step) + 16 * (lane >> 4));
+  };
+  load_w(a[0], 0);
+  load_x(0);
+  load_w(a[1], 1);
+  auto round_of = [&](Raw16 (&mine)[LOADS], int round) {
+    put(mine, 0, round);
+#pragma unroll
+    for (int m = 0; m < MB; ++m) put(b[m], 1 + m, round);
+    __syncthreads();
+    load_x(round + 1);   // first: loads retire in order, and a wait for these must not wait for the weights behind them
+    load_w(mine, round + 2);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int4v p = get(0, s);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const int4v q = get(1 + m, s);
+        if constexpr (N == 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m] = product4(__int_as_float(p[e]), __int_as_float(q[e]), acc[m]);
+        } else {
+          acc[m] = product16<T>(p, q, acc[m]);
         }
+      }
     }
+    __syncthreads();
+  };
+  for (int round = 0; round < rounds; round += 2) {
+    round_of(a[0], round);
+    if (round + 1 < rounds) round_of(a[1], round + 1);
   }
+  float4v(*sums)[MB][64] = reinterpret_cast<float4v(*)[MB][64]>(lds);
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
-#pragma unroll
-    for (int m = 0; m < MB; ++m) sums[wave][n * MB + m][lane] = acc[n][m];
+  for (int m = 0; m < MB; ++m) sums[wave][m][lane] = acc[m];
   __syncthreads();
-  for (int b = wave; b < NB * MB; b += kWaves) {
-    float4v sum = sums[0][b][lane];
+  if (wave >= MB) return;
+  float4v sum = sums[0][wave][lane];
 #pragma unroll
-    for (int o = 1; o < kWaves; ++o) sum += sums[o][b][lane];
-    const int r = r0 + 16 * (b % MB) + (lane & 15), c0 = v0 + 16 * (b / MB), c = c0 + 4 * (lane >> 4);
-    float l[4];
-    PartSum p{-INFINITY, 0.0f};
+  for (int o = 1; o < kWaves; ++o) sum += sums[o][wave][lane];
+  const int r = r0 + 16 * wave + (lane & 15), c = v0 + 4 * (lane >> 4);
+  float l[4];
+  PartSum p{-INFINITY, 0.0f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int at = min(c + e, v - 1);
-      const uint8_t shown = legal && r < rows ? legal[r * ldl + at] : 1;
-      const float value = sum[e] + (bias ? bias_at(bias, bias_type, at) : 0.0f);
-      l[e] = c + e < v && shown ? value : -INFINITY;
-      p.top = fmaxf(p.top, l[e]);
-    }
-    p.top = over_four(p.top, [](float q, float y) { return fmaxf(q, y); });
-    const float base = base_of(p.top);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) p.sum += exp2_of((l[e] - base) * kLog2e);
-    p.sum = over_four(p.sum, [](float q, float y) { return q + y; });
-    if (r >= rows || c0 >= ldz) continue;
-    if (lane < 16) parts[r * ld_parts + (c0 >> 4)] = make_float2(p.top, p.sum);
-    *reinterpret_cast<float4v *>(z + r * ldz + c) = float4v{l[0], l[1], l[2], l[3]};
+  for (int e = 0; e < 4; ++e) {
+    const int at = min(c + e, v - 1);
+    const uint8_t shown = legal && r < rows ? legal[r * ldl + at] : 1;
+    const float value = sum[e] + (bias ? bias_at(bias, bias_type, at) : 0.0f);
+    l[e] = c + e < v && shown ? value : -INFINITY;
+    p.top = fmaxf(p.top, l[e]);
   }
+  p.top = over_four(p.top, [](float q, float y) { return fmaxf(q, y); });
+  const float base = base_of(p.top);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) p.sum += exp2_of((l[e] - base) * kLog2e);
+  p.sum = over_four(p.sum, [](float q, float y) { return q + y; });
+  if (r >= rows) return;
+  if (lane < 16) parts[r * ld_parts + blockIdx.x] = make_float2(p.top, p.sum);
+  *reinterpret_cast<float4v *>(z + r * ldz + c) = float4v{l[0], l[1], l[2], l[3]};
 }
 
 struct Factors {
@@ -199,23 +231,24 @@ __global__ __launch_bounds__(1024) void k_few_u(const float2 *__restrict__ parts
   gb[c] = static_cast<B>(sum);
 }
 
-// 4 neighbours of a row as floats, zeros past its end.
+// 4 neighbours of a row, loaded without a branch (see load_clamped) and settled to floats, zeros past the row's end.
 template <typename T>
-__device__ __forceinline__ float4v load_four(const T *__restrict__ row, int at, int cols) {
-  struct __attribute__((packed, aligned(sizeof(T)))) Four {
-    T v[4];
-  };
-  float4v f = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (at + 4 <= cols) {
-    const Four p = *reinterpret_cast<const Four *>(row + at);
+struct __attribute__((packed, aligned(sizeof(T)))) Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> four_at(const T *__restrict__ row, int at, int cols) {
+  return *reinterpret_cast<const Four<T> *>(row + min(at, cols - 4));
+}
+template <typename T>
+__device__ __forceinline__ float4v settled(const Four<T> &p, int at, int cols) {
+  float4v f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(p.v[e]);
-  } else {
-    float p[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (at + e < cols) p[e] = static_cast<float>(row[at + e]);
-    f = float4v{p[0], p[1], p[2], 0.0f};
+  for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(p.v[e]);
+  const int past = at + 4 - cols;   // elements
+  if (past > 0) {
+    const float a = past == 1 ? f[1] : past == 2 ? f[2] : f[3], b = past == 1 ? f[2] : f[3];
+    f = float4v{past < 4 ? a : 0.0f, past < 3 ? b : 0.0f, past < 2 ? f[3] : 0.0f, 0.0f};
   }
   return f;
 }
@@ -245,7 +278,7 @@ __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
   if (job >= o.jobs) return;
   if (job < o.jobs_x) {
     const int d0 = 64 * (job % o.nd), part = job / o.nd % o.splits, r0 = 16 * MB * (job / o.nd / o.splits);
-    const int end = min(o.v, (part + 1) * o.chunk);
+    const int end = min(o.v, (part + 1) * o.chunk), last = (int)o.ldz - 4 - 4 * high;   // the last 4 of a row of g
     const float *gr[MB];
 #pragma unroll
     for (int m = 0; m < MB; ++m) gr[m] = o.g + min(r0 + 16 * m + low, o.rows - 1) * o.ldz + 4 * high;
@@ -254,27 +287,33 @@ __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = MB <= 2 ? 2 : 1;
+    constexpr int U = MB == 1 ? 4 : MB == 2 ? 2 : 1;
     for (int c = part * o.chunk; c < end; c += 16 * U) {
-      float4v a[U][MB], b[U][4];
+      float4v a[U][MB];
+      Four<T> b[U][4];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int at = c + 16 * u;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          b[u][t] = load_four(o.w + min(at + 4 * high + t, o.v - 1) * o.ldw, d0 + 4 * low, o.d);   // g is 0 past the columns
+        for (int m = 0; m < MB; ++m) a[u][m] = *reinterpret_cast<const float4v *>(gr[m] + min(at, last));
 #pragma unroll
-        for (int m = 0; m < MB; ++m)
-          a[u][m] = at + 4 * high < end ? *reinterpret_cast<const float4v *>(gr[m] + at) : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < 4; ++t) b[u][t] = four_at(o.w + min(at + 4 * high + t, o.v - 1) * o.ldw, d0 + 4 * low, o.d);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (c + 16 * u >= end) break;
+        if (c + 16 * u > last)   // g is 0 past the columns, but may end within the 16
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+          for (int m = 0; m < MB; ++m) a[u][m] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float4v w = settled(b[u][t], d0 + 4 * low, o.d);
 #pragma unroll
           for (int m = 0; m < MB; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][e] = product4(a[u][m][t], b[u][t][e], acc[m][e]);
+            for (int e = 0; e < 4; ++e) acc[m][e] = product4(a[u][m][t], w[e], acc[m][e]);
+        }
+      }
     }
 #pragma unroll
     for (int m = 0; m < MB; ++m)
@@ -296,21 +335,28 @@ __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
     for (int e = 0; e < 4; ++e) acc[f][e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int U = 4;
   for (int r0 = 0; r0 < o.rows; r0 += 4 * U) {
-    float4v a[U], b[U];
+    float4v a[U];
+    Four<T> b[U];
+    float factor[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + 4 * u + high;
-      const bool in = r < o.rows && o.factor[min(r, o.rows - 1)] != 0.0f;   // rows left out count as zeros, whatever they hold
-      a[u] = in && v0 + 4 * low < o.ldz ? *reinterpret_cast<const float4v *>(o.g + r * o.ldz + v0 + 4 * low)
-                                        : float4v{0.0f, 0.0f, 0.0f, 0.0f};
-      b[u] = in ? load_four(o.x + r * o.ldx, d0 + 4 * low, o.d) : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+      const int64_t r = min(r0 + 4 * u + high, o.rows - 1);
+      factor[u] = o.factor[r];
+      a[u] = *reinterpret_cast<const float4v *>(o.g + r * o.ldz + min(v0 + 4 * low, (int)o.ldz - 4));   // columns past the end go nowhere
+      b[u] = four_at(o.x + r * o.ldx, d0 + 4 * low, o.d);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      if (r0 + 4 * u >= o.rows) break;
+      const bool in = r0 + 4 * u + high < o.rows && factor[u] != 0.0f;   // rows left out count as zeros, whatever they hold
+      const float4v x = settled(b[u], d0 + 4 * low, o.d);
 #pragma unroll
-      for (int f = 0; f < 4; ++f)
+      for (int e = 0; e < 4; ++e) {
+        const float xe = in ? x[e] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[f][e] = product4(a[u][f], b[u][e], acc[f][e]);
+        for (int f = 0; f < 4; ++f) acc[f][e] = product4(in ? a[u][f] : 0.0f, xe, acc[f][e]);
+      }
+    }
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q)
@@ -318,13 +364,10 @@ __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
     for (int f = 0; f < 4; ++f) {
       const int c = v0 + 4 * (4 * high + q) + f, at = d0 + 4 * low;
       if (c >= o.v || at >= o.d) continue;
-      struct __attribute__((packed, aligned(sizeof(T)))) Four {
-        T v[4];
-      };
       T *to = o.gw + c * o.ldgw + at;
-      const Four four{{static_cast<T>(acc[f][0][q]), static_cast<T>(acc[f][1][q]), static_cast<T>(acc[f][2][q]),
+      const Four<T> four{{static_cast<T>(acc[f][0][q]), static_cast<T>(acc[f][1][q]), static_cast<T>(acc[f][2][q]),
                        static_cast<T>(acc[f][3][q])}};
-      if (at + 4 <= o.d) *reinterpret_cast<Four *>(to) = four;
+      if (at + 4 <= o.d) *reinterpret_cast<Four<T> *>(to) = four;
       else
 #pragma unroll
         for (int e = 0; e < 3; ++e)
@@ -382,15 +425,15 @@ void few(const Call &c, const Given &g, char *ws, hipStream_t st) {
   float2 *stat = reinterpret_cast<float2 *>(ws + s.stat);
   const T *x = static_cast<const T *>(g.x), *w = static_cast<const T *>(g.w);
   const int rows = (int)c.rows, v = (int)c.v, d = (int)c.d;
-  auto logits = [&](auto kernel, int nb, int mb) {
-    hipLaunchKernelGGL(kernel, dim3(blocks_for(c.v, 16 * nb), blocks_for(c.rows, 16 * mb)), dim3(64 * kWaves), 0, st, x, g.ldx,
-                       rows, w, g.ldw, v, d, g.bias, g.bias_type, g.targets.legal, g.targets.ldl, floats(s.z), s.ldz, stat,
+  auto logits = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(blocks_for(c.v, 16), blocks_for(c.rows, 16 * s.mb)), dim3(64 * kWaves), 0, st, x, g.ldx, rows,
+                       w, g.ldw, v, d, g.bias, g.bias_type, g.targets.legal, g.targets.ldl, floats(s.z), s.ldz, stat,
                        (int64_t)s.parts);
     check_launch("read-out logits");
   };
-  if (s.mb == 1) logits(k_few_logits<T, 1, 1>, 1, 1);
-  else if (s.mb == 2) logits(k_few_logits<T, 1, 2>, 1, 2);
-  else logits(k_few_logits<T, 2, 4>, 2, 4);
+  if (s.mb == 1) logits(k_few_logits<T, 1, 2048>);
+  else if (s.mb == 2) logits(k_few_logits<T, 2, 1024>);
+  else logits(k_few_logits<T, 4, 1024>);
   const int parts = (v + 15) / 16;
   RowInfo *info = nullptr;
   if (!c.grads() || c.rows * parts > 8192) {
@@ -425,7 +468,15 @@ void few(const Call &c, const Given &g, char *ws, hipStream_t st) {
 
 }  // namespace
 
-bool few_rows(const Call &c) { return c.rows <= (c.type == FLY_F32 ? 256 : 64) && c.rows * c.v <= (int64_t)1 << 26; }
+// Up to 32 rows: at 32 of 2,333 into 4,168 the loss takes 27 us (float32) and 20 (bfloat16) against 43 and 34 with the operands laid
+// out, with gradients 63 and 56 against 95 and 72.  At 48 the loss takes 49 against 43; float32 with gradients 92 against 98, and at
+// 64 100 against 102 (1,024 into 32,000 219 against 250).  A small product's launches cost more than its work: 64 rows of 256 into
+// 2,000 33 us against 40, 96 rows 37 against 40.
+bool few_rows(const Call &c) {
+  if (c.d < (c.type == FLY_F32 ? 4 : 8)) return false;   // rows have a whole piece
+  const int64_t most = c.type == FLY_F32 && c.grads() ? 64 : 32;
+  return c.rows <= most || (c.rows <= 96 && c.rows * c.d * c.v <= (int64_t)1 << 26);
+}
 
 size_t few_ws(const Call &c) { return Few(c).bytes; }
 
