@@ -628,13 +628,18 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 
 
 
-// The workgroup's tile of a product of m x n, n x m rows of it.  One plane: 256 x 256 from 128 tiles on, 128 x 128 from 100 on,
-// else 64 x 64; two planes: 128 x 192 from 150 tiles on, else 64 x 64.
+// The workgroup's tile of the logits, by how many there are.  One plane: 256 x 256 (n x m), one workgroup of 16 waves per CU, from 128
+// tiles on where they fill 84% of their rounds of 256 workgroups (10,000 x 2,333 into 4,168 216 us, 223 with 128 x 128, 303 with 64 x
+// 64), else 128 x 128 from 100 on (4,096 rows, 272 of the large tiles: 108 us against 135; 1,120 rows into 32,000 116 against 130), else
+// 64 x 64 (256 rows 35 against 39).  Two planes: 128 x 192 from 150 tiles on (1,120 rows of 256 into 4,168 28 us against 35 with 64 x
+// 64; 543 rows of 2,333 into 419 78 against 40).
 enum Shape { kSmall, kMedium, kLarge };
+int64_t tiles_of(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 Shape shape_of(int planes, int64_t m, int64_t n) {
-  auto tiles = [&](int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
-  if (planes == 2) return tiles(192, 128) >= 150 ? kLarge : kSmall;
-  return tiles(256, 256) >= 128 ? kLarge : tiles(128, 128) >= 100 ? kMedium : kSmall;
+  if (planes == 2) return tiles_of(m, n, 192, 128) >= 150 ? kLarge : kSmall;
+  const int64_t large = tiles_of(m, n, 256, 256);
+  if (large >= 128 && large * 100 >= round_up(large, 256) * 84) return kLarge;
+  return tiles_of(m, n, 128, 128) >= 100 ? kMedium : kSmall;
 }
 // Parts of a row's columns that the waves of a shape hold, for `cols` columns.
 int parts_of(int planes, Shape s, int64_t cols) {
@@ -656,8 +661,15 @@ constexpr int64_t kShareBytes = (int64_t)64 << 20;
 struct Splits {
   int x = 1, w = 1;
 };
+// The tile of the gradients' products, whose tiles are counted together.  One plane: 256 x 256 from 500 tiles on (10,000 x 2,333 x
+// 4,168 655 us against 718 with 128 x 128; 4,096 rows, 330 tiles, 365 against 334), 128 x 128 from 600 of those on (1,120 rows 134
+// against 138 with 64 x 64), else, and up to 400 rows, whose product with the weight is soon over, 64 x 64 (256 rows 78 against 80
+// and 86).  Two planes: 128 x 192 but for few tiles.
 Shape grad_shape(int planes, const Call &c, int64_t rows) {
-  return shape_of(planes, (c.gx ? rows : 0) + (c.gw ? c.v : 0), c.d);
+  const int64_t m = (c.gx ? rows : 0) + (c.gw ? c.v : 0);
+  if (planes == 2) return shape_of(2, m, c.d);
+  if (rows <= 400) return kSmall;
+  return tiles_of(m, c.d, 256, 256) >= 500 ? kLarge : tiles_of(m, c.d, 128, 128) >= 600 ? kMedium : kSmall;
 }
 Splits splits_of(int planes, const Call &c, int64_t rows) {
   const Shape s = grad_shape(planes, c, rows);
