@@ -27,6 +27,7 @@ from .brain import ConnectomeRNN
 from .connectome import Connectome
 from .encoding import N_BASE, N_FEATURES, N_MOVES, move_squares
 from .int8 import Int8Linear
+from .readout import readout_loss
 
 READOUT_SUPERCLASSES = ("descending_neuron",)   # plus every efferent neuron (model.py:23)
 
@@ -173,11 +174,8 @@ class FlyChessNet(nn.Module):
         out = self.norm(r.T).contiguous()
         return policy(out), value(out)
 
-    def _forward_layers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        """The forward as separate differentiable layers (chessfly/model.py:95-105): training, or any call
-        with autograd enabled.  Under autograd the recurrence is float32 (its sparse products on the device);
-        without it, in training mode, the recurrence is the fused device forward_io in infer_dtype and the
-        normaliser updates its running statistics."""
+    def _outputs(self, x: torch.Tensor) -> torch.Tensor:
+        """The normalised output neurons by separate differentiable layers (see _forward_layers)."""
         dtype = torch.float32 if torch.is_grad_enabled() else self.infer_dtype
         if x.dtype != torch.float32:
             x = x.float()
@@ -186,9 +184,29 @@ class FlyChessNet(nn.Module):
         else:                                   # the attack planes are never seen and their weights get no gradient
             enc = nn.functional.linear(x[:, :N_BASE], self.encoder.weight[:, :N_BASE], self.encoder.bias)
         u_in = (enc * self.cfg.input_gain).to(dtype).T.contiguous()
-        r = self.norm(self.brain.forward_io(u_in, self.in_idx, self.out_idx, self.cfg.steps).T.float())
+        return self.norm(self.brain.forward_io(u_in, self.in_idx, self.out_idx, self.cfg.steps).T.float())
+
+    def _forward_layers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The forward as separate differentiable layers (chessfly/model.py:95-105): training, or any call
+        with autograd enabled.  Under autograd the recurrence is float32 (its sparse products on the device);
+        without it, in training mode, the recurrence is the fused device forward_io in infer_dtype and the
+        normaliser updates its running statistics."""
+        r = self._outputs(x)
         logits = self.policy(r) + self.policy_from(r) @ self.move_from_onehot + self.policy_to(r) @ self.move_to_onehot
         return logits, self.value(r)
+
+    def policy_loss(self, x: torch.Tensor, target, legal: torch.Tensor | None = None,
+                    reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor]:
+        """The policy's softmax cross entropy over the legal moves and the WDL logits, without the policy's logits: what a training
+        step needs of them (chessfly/train.py:126-132 takes the loss from kept logits).  target: readout.Visits, or a move a
+        position (readout.readout_loss).  Differentiable by every parameter; the layers run as forward's do under autograd."""
+        _hip.require_device(x, "FlyChessNet.policy_loss")
+        r = self._outputs(x)
+        # a move's logit is linear in the outputs, its from- and to-square terms included: one map of their sum
+        frm, to = self.move_from_onehot.t(), self.move_to_onehot.t()
+        weight = self.policy.weight + frm @ self.policy_from.weight + to @ self.policy_to.weight
+        bias = self.policy.bias + frm @ self.policy_from.bias + to @ self.policy_to.bias
+        return readout_loss(r, weight, bias, target, legal, reduction), self.value(r)
 
     def forward(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """x: (B, >= N_BASE) -> policy logits (B, N_MOVES), WDL logits (B, 3), both float32.  Half-precision

@@ -19,6 +19,7 @@ import torch.nn.functional as F
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."))
 
+from chessfly.clip import clip_grad_norm_  # noqa: E402
 from chessfly.distill import distill_loss, label  # noqa: E402
 from chessfly.encoding import N_MOVES  # noqa: E402
 from chessfly.synthetic import GraphSpec, synthetic_boards, synthetic_net  # noqa: E402
@@ -51,7 +52,7 @@ def run(steps: int = 40, batch: int = 256, moves: int = 24, temperature: float =
         value = F.cross_entropy(student_wdl, wdl.softmax(-1))
         optimiser.zero_grad(set_to_none=True)
         (policy + value).backward()
-        torch.nn.utils.clip_grad_norm_(student.parameters(), 5.0)
+        clip_grad_norm_(student.parameters(), 5.0)
         optimiser.step()
         losses.append(policy.detach())
     losses = [float(v) for v in torch.stack(losses)]

@@ -191,6 +191,7 @@ def train_bench(args, dev) -> dict:
     full synthetic graph at `--batch` positions."""
     import torch
     from chessfly import _hip
+    from chessfly.clip import clip_grad_norm_
     from chessfly.synthetic import synthetic_boards, synthetic_net
 
     net, conn = bench_net(args, dev)
@@ -205,7 +206,7 @@ def train_bench(args, dev) -> dict:
         loss = _train_loss(logits, wdl_logits, pi, legal, wdl)
         opt.zero_grad(set_to_none=True)
         loss.backward()
-        torch.nn.utils.clip_grad_norm_(net.parameters(), 5.0)
+        clip_grad_norm_(net.parameters(), 5.0)
         opt.step()
         return loss
 
