@@ -8,8 +8,8 @@ squares are summed in float64.  Gradients of norm below the limit are read and n
 
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from collections.abc import Iterable
 
 import torch
@@ -39,15 +39,7 @@ def _gradients(parameters, what: str) -> list[torch.Tensor]:
         parameters = (parameters,)
     elif not isinstance(parameters, Iterable):
         raise RuntimeError(f"{what}: parameters must be a tensor or tensors, got {type(parameters).__name__}")
-    grads = [g for p in parameters if (g := p.grad) is not None]
-    for g in grads:
-        if not g.is_cuda:
-            _hip.require_device(g, what)
-        if g.dtype not in FLOATS or g.layout is not torch.strided:
-            raise RuntimeError(f"{what}: gradients must be dense float32, float16 or bfloat16, got {g.dtype} {g.layout}")
-        if g.device != grads[0].device:
-            raise RuntimeError(f"{what}: gradients must be on one device, got {grads[0].device} and {g.device}")
-    return grads
+    return [g for p in parameters if (g := p.grad) is not None]
 
 
 def _run(grads: list[torch.Tensor], limit: float, norm_type: float, what: str) -> torch.Tensor:
@@ -56,21 +48,36 @@ def _run(grads: list[torch.Tensor], limit: float, norm_type: float, what: str) -
         raise RuntimeError(f"{what}: norm_type must be 2 or inf, got {norm_type}")
     if not grads:
         return torch.zeros(())
-    n, dev = len(grads), grads[0].device
-    kept = [g if _dense(g) else g.contiguous() for g in grads]
-    pointers = (ctypes.c_void_p * n)(*[g.data_ptr() for g in kept])
-    sizes = (ctypes.c_int64 * n)(*[g.numel() for g in kept])
-    types = (ctypes.c_int32 * n)(*[FLOATS[g.dtype] for g in kept])
+    n, dev, index = len(grads), grads[0].device, grads[0].get_device()
+    if index < 0:
+        _hip.require_device(grads[0], what)
+    kept, pointers, sizes, types = [], array("Q"), array("q"), array("i")
+    for g in grads:
+        kind = FLOATS.get(g.dtype)
+        if kind is None or g.layout is not torch.strided:
+            raise RuntimeError(f"{what}: gradients must be dense float32, float16 or bfloat16, got {g.dtype} {g.layout}")
+        if g.get_device() != index:
+            raise RuntimeError(f"{what}: gradients must be on one device, got {dev} and {g.device}")
+        k = g
+        if not _dense(g):
+            if limit >= 0 and not _apart(g):
+                raise RuntimeError(f"{what}: a gradient's elements overlap in memory")
+            k = g.contiguous()
+        kept.append(k)
+        pointers.append(k.data_ptr())
+        sizes.append(k.numel())
+        types.append(kind)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    need = _hip.load().fly_clip_workspace(sizes, types, n)
+    at = [a.buffer_info()[0] for a in (pointers, sizes, types)]      # the arrays outlive the call
+    need = _hip.load().fly_clip_workspace(*at[1:], n)
     ws = _hip.workspace(need, dev)
-    _hip.call("fly_clip_gradients", dev.index, pointers, sizes, types, n, 0 if norm_type == math.inf else 2, limit,
-              norm.data_ptr(), ws.data_ptr(), need)
+    _hip.call("fly_clip_gradients", index, *at, n, 0 if norm_type == math.inf else 2, limit, norm.data_ptr(),
+              ws.data_ptr(), need)
     if limit >= 0:
         for g, k in zip(grads, kept):
             if g is not k:
                 g.copy_(k)
-        torch.autograd.graph.increment_version([g for g in kept if not g.is_inference()])
+        torch.autograd.graph.increment_version(kept)
     return norm
 
 
@@ -90,9 +97,6 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     if not max_norm >= 0:
         raise RuntimeError(f"{what}: max_norm must be at least 0, got {max_norm}")
     grads = _gradients(parameters, what)
-    for g in grads:
-        if not _dense(g) and not _apart(g):
-            raise RuntimeError(f"{what}: a gradient's elements overlap in memory")
     if error_if_nonfinite and grads:
         norm = _run(grads, -1.0, norm_type, what)
         if not math.isfinite(norm):
