@@ -260,11 +260,51 @@ struct LogitsOut {
   __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int part, int, float *turn) const {
     constexpr int PITCH = 16 * FN + 4;
     const int quad = 4 * (lane >> 4);
+    // What 16 rows need from memory is loaded while the 16 before them are done, without branches: the bytes of the mask (the last
+    // ones of a row moved down to their columns) and the first 32 entries of the lists.
+    struct __attribute__((packed)) Bytes {
+      uint32_t w;
+    };
+    struct Ahead {
+      uint32_t shown[FN];
+      int column[8];
+      float unit;
+    };
+    auto entries = [&](int (&to)[8], int first, int64_t row) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] = list.column[min(first + 4 * j + (lane >> 4), list.k - 1) * list.ld + row];
+    };
+    auto fetch = [&](int i) {
+      Ahead a;
+      const int64_t row = min(m0 + 16 * i + (lane & 15), rows - 1);
+      a.unit = unit_m ? unit_m[row] : 1.0f;
+      if (legal) {
+        const uint8_t *seen = legal + row * ldl;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int c = n0 + 16 * j + quad, most = max(cols - 4, 0);
+          if (cols >= 4) {
+            const int past = c - most;   // columns
+            const uint32_t w = reinterpret_cast<const Bytes *>(seen + min(c, most))->w;
+            a.shown[j] = past <= 0 ? w : past < 4 ? w >> (8 * past) : 0u;
+          } else {
+            a.shown[j] = 0u;
+            for (int e = 0; e < cols; ++e)
+              if (c == 0 && seen[e]) a.shown[j] |= 1u << (8 * e);
+          }
+        }
+      }
+      entries(a.column, 0, row);
+      return a;
+    };
+    constexpr bool AHEAD = FM < 4;   // 16 waves of 64 x 64 have no registers for it: the loads of 16 rows go together, and are waited for
+    Ahead next;
+    if constexpr (AHEAD) next = fetch(0);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int m = m0 + 16 * i + (lane & 15);
-      const float um = unit_m && m < rows ? unit_m[m] : 1.0f;
-      const uint8_t *seen = legal && m < rows ? legal + m * ldl : nullptr;
+      const Ahead mine = AHEAD ? next : fetch(i);
+      if (AHEAD && i + 1 < FM) next = fetch(i + 1);
       float4v v[FN];
       PartSum p{-INFINITY, 0.0f};
 #pragma unroll
@@ -274,21 +314,11 @@ struct LogitsOut {
         if (unit_n) {
           const float4v un = *reinterpret_cast<const float4v *>(unit_n + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] * um * un[e];
+          for (int e = 0; e < 4; ++e) v[j][e] *= mine.unit * un[e];   // powers of 2, whose product is no larger than a logit needs
         }
         v[j] += *reinterpret_cast<const float4v *>(bias + at);
-        uint32_t shown = 0x01010101u;
-        if (seen) {
-          struct __attribute__((packed)) Bytes {
-            uint32_t w;
-          };
-          if (c + 4 <= cols) shown = reinterpret_cast<const Bytes *>(seen + c)->w;
-          else
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-              if (c + e < cols && !seen[c + e]) shown &= ~(1u << (8 * e));
-        }
         if (legal || n0 + 16 * FN > cols) {
+          const uint32_t shown = legal ? mine.shown[j] : 0x01010101u;
           float l[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) l[e] = c + e < cols && (shown & (0xffu << (8 * e))) ? v[j][e] : -INFINITY;
@@ -326,18 +356,20 @@ struct LogitsOut {
       for (int j = 0; j < FN; ++j) *reinterpret_cast<float4v *>(turn + (lane & 15) * PITCH + 16 * j + quad) = v[j];
       asm volatile("" ::: "memory");   // other lanes read what this one wrote: a wave's LDS accesses keep their order
       // the targets among these columns: 4 entries of 16 rows in a load, 8 loads in flight
-      const int64_t mine = min(m, rows - 1);
-      for (int first = 0; first < list.k; first += 32) {
-        int at[8];
+      const int64_t row = min(m, rows - 1);
+      auto found = [&](const int (&column)[8], int first) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int entry = first + 4 * j + (lane >> 4);
-          at[j] = (entry < list.k ? list.column[entry * list.ld + mine] : -1) - n0;
+          const int entry = first + 4 * j + (lane >> 4), at = column[j] - n0;
+          if (m < rows && entry < list.k && at >= 0 && at < 16 * FN)
+            list.logit[entry * list.ld + row] = turn[(lane & 15) * PITCH + at];
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (m < rows && at[j] >= 0 && at[j] < 16 * FN)
-            list.logit[(first + 4 * j + (lane >> 4)) * list.ld + mine] = turn[(lane & 15) * PITCH + at[j]];
+      };
+      found(mine.column, 0);
+      for (int first = 32; first < list.k; first += 32) {
+        int column[8];
+        entries(column, first, row);
+        found(column, first);
       }
       asm volatile("" ::: "memory");
     }
@@ -414,18 +446,30 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
   __shared__ float col_sum[2][kGradCols], f_row[kGradRows], ft_row[kGradRows], un_col[kGradCols], f_part[kGradRows][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c0 = blockIdx.x * kGradCols, r0 = blockIdx.y * kGradRows;
+  // 4 x 8 blocks of 16 x 16 logits, 8 for each wave; all loads first, without branches, then what is made of them
+  using Kept = std::conditional_t<KEEP == kFloats, float4v, uint2>;
+  const int row_blocks = (rows + 15) >> 4;   // that were stored
+  const int64_t block0 = (int64_t)min((r0 >> 4) + wave, row_blocks - 1) * (ldz >> 4);
+  Kept kept[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    kept[i] = static_cast<const Kept *>(z)[(block0 + min((c0 >> 4) + i, (int)(ldz >> 4) - 1)) * 64 + lane];
+  const int64_t list_row = min(r0 + lane, rows - 1);
+  int column[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) column[j] = l.column[min(wave + 4 * j, l.k - 1) * l.ld + list_row];
+  const RowInfo mine = info[list_row];   // of a row of the lists
+  const float most = maxima->row, most_weight = maxima->weight;
   if (tid < kGradRows) {
-    const int r = r0 + tid;
-    const float most = maxima->row;
-    f_row[tid] = r < rows ? factor[r] : 0.0f;
-    ft_row[tid] = r < rows && most > 0.0f ? turned_factor[r] / most * kUnit : 0.0f;
+    const bool in = r0 + tid < rows;
+    const float f = factor[list_row], ft = turned_factor[list_row];
+    f_row[tid] = in ? f : 0.0f;
+    ft_row[tid] = in && most > 0.0f ? ft / most * kUnit : 0.0f;
   }
   if (tid >= 128) {
     const int c = c0 + tid - 128;
-    un_col[tid - 128] = P == 2 && c < cols ? unit_n[c] / maxima->weight * kUnit : kUnit;
+    un_col[tid - 128] = P == 2 && c < cols ? unit_n[c] / most_weight * kUnit : kUnit;
   }
-  // 4 x 8 blocks of 16 x 16 logits, 8 for each wave
-  const int64_t block0 = (int64_t)(r0 >> 4) * (ldz >> 4) + (c0 >> 4);
   if constexpr (KEEP == kCodes) {
     // a part's largest p, times the share
     const int r = tid >> 2, q = tid & 3;
@@ -438,41 +482,41 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
     f_part[r][q] = f;
     __syncthreads();
   }
+  const int r16 = 16 * wave + (lane & 15);
+  RowInfo row{};
+  if constexpr (KEEP == kFloats) row = info[min(r0 + r16, rows - 1)];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int rg = wave, cg = i, r = 16 * rg + (lane & 15), c = 16 * cg + 4 * (lane >> 4);
-    const int64_t at = (block0 + rg * (ldz >> 4) + cg) * 64 + lane;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (r0 + r < rows && c0 + c < ldz) {
-      if constexpr (KEEP == kFloats) {
-        const RowInfo f = info[r0 + r];
-        const float4v z4 = static_cast<const float4v *>(z)[at];
+    const int c = 16 * i + 4 * (lane >> 4);
+    const bool in = r0 + r16 < rows && c0 + c < ldz;
+    float v[4];
+    if constexpr (KEEP == kFloats) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (f.share != 0.0f) v[e] = f.share * exp2_of((z4[e] - f.top) * kLog2e - f.log_sum);
-      } else {
-        const uint2 w = static_cast<const uint2 *>(z)[at];
-        const float f = f_part[r][c >> shift];
+      for (int e = 0; e < 4; ++e) {
+        const float p = row.share * exp2_of((kept[i][e] - row.top) * kLog2e - row.log_sum);
+        v[e] = in && row.share != 0.0f ? p : 0.0f;
+      }
+    } else {
+      const float f = in ? f_part[r16][c >> shift] : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t code = e < 2 ? (w.x >> (16 * e)) & 0xffffu : (w.y >> (16 * (e - 2))) & 0xffffu;
-          v[e] = f * (code == kNone ? 0.0f : exp2_of((float)code * (-kLog2e / kSteps)));
-        }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t code = e < 2 ? (kept[i].x >> (16 * e)) & 0xffffu : (kept[i].y >> (16 * (e - 2))) & 0xffffu;
+        v[e] = f * (code == kNone ? 0.0f : exp2_of((float)code * (-kLog2e / kSteps)));
       }
     }
-    *reinterpret_cast<float2 *>(&u[r][c]) = make_float2(v[0], v[1]);
-    *reinterpret_cast<float2 *>(&u[r][c + 2]) = make_float2(v[2], v[3]);
+    *reinterpret_cast<float2 *>(&u[r16][c]) = make_float2(v[0], v[1]);
+    *reinterpret_cast<float2 *>(&u[r16][c + 2]) = make_float2(v[2], v[3]);
   }
   __syncthreads();
   // the targets among these columns, each once
-  if (r0 + lane < rows)
-    for (int j = wave; j < l.k; j += 4) {
-      const int64_t from = j * l.ld + r0 + lane;
-      const int c = l.column[from];
-      if (c < c0 || c >= c0 + kGradCols) continue;
-      const RowInfo f = info[r0 + lane];
-      u[lane][c - c0] = f.share * exp2_of((l.logit[from] - f.top) * kLog2e - f.log_sum) - l.weight[from] / f.whole;
-    }
+  auto aim = [&](int j, int c) {
+    if (r0 + lane >= rows || j >= l.k || c < c0 || c >= c0 + kGradCols) return;
+    const int64_t from = j * l.ld + r0 + lane;
+    u[lane][c - c0] = mine.share * exp2_of((l.logit[from] - mine.top) * kLog2e - mine.log_sum) - l.weight[from] / mine.whole;
+  };
+#pragma unroll
+  for (int j = 0; j < 8; ++j) aim(wave + 4 * j, column[j]);
+  for (int j = wave + 32; j < l.k; j += 4) aim(j, l.column[j * l.ld + list_row]);
   __syncthreads();
   typedef uint32_t words[4];
 #pragma unroll
@@ -527,30 +571,10 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
   if (half == 0 && c0 + c < cols) sums[blockIdx.y * ld_sums + c0 + c] = s + col_sum[1][c];
 }
 
-// The columns' sums over all tiles of rows, after what earlier pieces of rows gave: 64 columns, each wave every 16th tile.
-template <typename T>
-__global__ __launch_bounds__(1024) void k_bias_grad(const float *__restrict__ sums, int64_t ld_sums, int tiles, int cols,
-                                                    const float *__restrict__ before, float *__restrict__ after,
-                                                    T *__restrict__ out) {
-  __shared__ float share[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (c < cols)
-    for (int i = wave; i < tiles; i += 16) s += sums[i * ld_sums + c];
-  share[wave][lane] = s;
-  __syncthreads();
-  if (wave || c >= cols) return;
-  s = before ? before[c] : 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s += share[i][lane];
-  if (after) after[c] = s;
-  else out[c] = static_cast<T>(s);
-}
-
 // ---- gradients -------------------------------------------------------------------------------------------------------
 
 // out[m][n] = sum * row[m] * *scale / 2^14, after what earlier pieces of rows gave.  Where k runs in parts, the sums of each go
-// to `share` and k_join adds them up.
+// to `share` and k_finish adds them up.
 template <typename T>
 struct GradOut {
   const float *row;          // or null
@@ -604,16 +628,52 @@ struct GradOut {
   }
 };
 
+// The last of a piece of rows, in one launch: the columns' sums over all tiles of rows, after what earlier pieces gave (workgroups of 32
+// columns, 32 lanes of tiles), and the parts of the products' k.
+template <typename B>
+struct BiasOut {
+  const float *sums;         // (tile, column) or null
+  int64_t ld;
+  int tiles, cols;
+  const float *before;
+  float *after;
+  B *out;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_join(const GradOut<T> g, int splits) {
+struct Join {
+  GradOut<T> out;
+  int splits, groups;        // workgroups, 0 without parts
+};
+template <typename T, typename B>
+__global__ __launch_bounds__(1024) void k_finish(const BiasOut<B> b, int bias_groups, const Join<T> x, const Join<T> w) {
+  __shared__ float share[32][33];
+  if ((int)blockIdx.x < bias_groups) {
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (c < b.cols)
+      for (int i = part; i < b.tiles; i += 32) s += b.sums[i * b.ld + c];
+    share[part][lane] = s;
+    __syncthreads();
+    if (part || c >= b.cols) return;
+    s = b.before ? b.before[c] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += share[i][lane];
+    if (b.after) b.after[c] = s;
+    else b.out[c] = static_cast<B>(s);
+    return;
+  }
+  int group = blockIdx.x - bias_groups;
+  const Join<T> &j = group < x.groups ? x : w;
+  if (group >= x.groups) group -= x.groups;
+  const GradOut<T> &g = j.out;
   const int64_t per = g.ld_sum / 4, all = g.rows * per, stride = g.rows * g.ld_sum;
   const float s = g.unit();
-  for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = group * (int64_t)1024 + threadIdx.x; i < all; i += (int64_t)j.groups * 1024) {
     const int m = (int)(i / per), n = 4 * (int)(i % per);
     if (n >= g.cols) continue;
     const float *from = g.share + m * g.ld_sum + n;
     float4v sum = *reinterpret_cast<const float4v *>(from);
-    for (int p = 1; p < splits; ++p) sum += *reinterpret_cast<const float4v *>(from + p * stride);
+    for (int p = 1; p < j.splits; ++p) sum += *reinterpret_cast<const float4v *>(from + p * stride);
     g.put(m, n, sum, s);
   }
 }
@@ -628,58 +688,77 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 
 
 
-// The workgroup's tile of the logits, by how many there are.  One plane: 256 x 256 (n x m), one workgroup of 16 waves per CU, from 128
-// tiles on where they fill 84% of their rounds of 256 workgroups (10,000 x 2,333 into 4,168 216 us, 223 with 128 x 128, 303 with 64 x
-// 64), else 128 x 128 from 100 on (4,096 rows, 272 of the large tiles: 108 us against 135; 1,120 rows into 32,000 116 against 130), else
-// 64 x 64 (256 rows 35 against 39).  Two planes: 128 x 192 from 150 tiles on (1,120 rows of 256 into 4,168 28 us against 35 with 64 x
-// 64; 543 rows of 2,333 into 419 78 against 40).
+// The workgroup's tile (m x n): one plane 64 x 64 (4 waves), 128 x 128 (8) or 256 x 256 (16), two planes 64 x 64 (4), 128 x 128 (16) or
+// 192 x 128 (8).  64 x 64, and 128 x 128 of one plane, run two workgroups per CU, the others one.
 enum Shape { kSmall, kMedium, kLarge };
-int64_t tiles_of(int64_t m, int64_t n, int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
-Shape shape_of(int planes, int64_t m, int64_t n) {
-  if (planes == 2) return tiles_of(m, n, 192, 128) >= 150 ? kLarge : kSmall;
-  const int64_t large = tiles_of(m, n, 256, 256);
-  if (large >= 128 && large * 100 >= round_up(large, 256) * 84) return kLarge;
-  return tiles_of(m, n, 128, 128) >= 100 ? kMedium : kSmall;
+struct Tile {
+  int m, n, places;   // and how many of them run at once
+};
+Tile tile_of(int planes, Shape s) {
+  if (s == kSmall) return {64, 64, 512};
+  if (s == kMedium) return {128, 128, planes == 2 ? 256 : 512};
+  return planes == 2 ? Tile{192, 128, 256} : Tile{256, 256, 256};
 }
-// Parts of a row's columns that the waves of a shape hold, for `cols` columns.
+int64_t tiles_of(const Tile &t, int64_t m, int64_t n) { return ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n); }
+
+// The logits' tile: the one whose rounds of workgroups cost least.  A round's cost, from one that fills it, in those of 128 x 128: one
+// plane 0.5 (64 x 64) and 1.85 (256 x 256), two planes 0.72 and 1.6 (192 x 128).  Measured, us of the loss, 64 x 64 / 128 x 128 /
+// large: bfloat16 2,333 into 4,168 256 rows 35 / 39 / 69, 1,120 rows 60 / 49 / 72, 4,096 rows 139 / 108 / 135, 10,000 rows 303 / 223 /
+// 216; 1,024 into 32,000 1,120 rows 158 / 116 / 130, 4,096 rows 445 / 320 / 306; float32 2,333 into 4,168 256 rows 52 / 59 / 79, 543
+// rows 76 / 62 / 81, 1,120 rows 105 / 105 / 88, 4,096 rows 301 / 259 / 239; 1,024 into 32,000 256 rows 116 / 101 / 119, 543 rows 191 /
+// 170 / 152.
+Shape logits_shape(int planes, int64_t m, int64_t n) {
+  const double cost[3] = {planes == 2 ? 0.72 : 0.5, 1.0, planes == 2 ? 1.6 : 1.85};
+  Shape best = kSmall;
+  double least = 0.0;
+  for (Shape s : {kSmall, kMedium, kLarge}) {
+    const Tile t = tile_of(planes, s);
+    const double c = cost[s] * (double)((tiles_of(t, m, n) + t.places - 1) / t.places);
+    if (s == kSmall || c < least) best = s, least = c;
+  }
+  return best;
+}
+// Columns of the logits that a wave of a shape holds, 2 to the this, and how many such parts a row of `cols` columns has.
+int part_shift(int planes, Shape s) { return s == kSmall || (planes == 2 && s == kMedium) ? 5 : 6; }
 int parts_of(int planes, Shape s, int64_t cols) {
-  const int64_t tile = s == kSmall ? 64 : s == kMedium || planes == 2 ? 128 : 256, wave = s == kSmall ? 32 : 64;
-  return (int)((cols + tile - 1) / tile * (tile / wave));
+  const Tile t = tile_of(planes, s);
+  return (int)((cols + t.n - 1) / t.n * (t.n >> part_shift(planes, s)));
 }
 template <typename H, int P, typename EP, int COUNT>
 void product(Shape shape, const Products<EP, COUNT> &p, hipStream_t st) {
   if (shape == kSmall) launch_blocks<H, P, 2, 2, 2, 2, 4>(p, st);
-  else if constexpr (P == 2) launch_blocks<H, P, 2, 4, 4, 3, 3>(p, st);
-  else if (shape == kMedium) launch_blocks<H, P, 2, 4, 4, 2, 4>(p, st);
+  else if constexpr (P == 2) {
+    if (shape == kMedium) launch_blocks<H, P, 4, 4, 2, 2, 4>(p, st);
+    else launch_blocks<H, P, 2, 4, 4, 3, 3>(p, st);
+  } else if (shape == kMedium) launch_blocks<H, P, 2, 4, 4, 2, 4>(p, st);
   else launch_blocks<H, P, 4, 4, 4, 4, 4>(p, st);
 }
 
-// In how many parts the k of the gradients' products run, side by side in one launch.  Jobs are counted in blocks of k of one
-// tile; one that is longer than 0.7 of what each of the CU's places gets keeps the others waiting.  A part costs its sums' way to
-// memory and back, so none is shorter than 16 blocks, and all parts' sums fit kShareBytes.
+// The tile of the gradients' products, whose tiles are counted together; parts of k even their rounds out.  One plane: up to 200 rows,
+// whose product with the rows is soon over, 64 x 64 (bfloat16, 100 rows of 1,024 into 32,000 118 us against 126 and 129), else 256 x 256
+// from 500 tiles on (1,120 rows 339 against 372; 2,333 into 4,168 4,096 rows, 330 tiles, 321 against 296), 128 x 128 from 600 on (1,120
+// rows 125 against 130), else 64 x 64.  Two planes: 128 x 128 from 400 tiles on (4,096 rows 724 us, with 192 x 128 787, with 64 x 64 893;
+// 256 rows 113, 124 and 117), else 64 x 64 (4,096 rows of 512 into 2,000 139 against 145).
+Shape grad_shape(int planes, const Call &c, int64_t rows) {
+  const int64_t m = (c.gx ? rows : 0) + (c.gw ? c.v : 0);
+  if (planes == 2) return tiles_of(tile_of(2, kMedium), m, c.d) >= 400 ? kMedium : kSmall;
+  if (rows <= 200) return kSmall;
+  if (tiles_of(tile_of(1, kLarge), m, c.d) >= 500) return kLarge;
+  return tiles_of(tile_of(1, kMedium), m, c.d) >= 600 ? kMedium : kSmall;
+}
+
+// In how many parts the k of the gradients' products run, side by side in one launch.  Jobs are counted in blocks of k of one tile; one
+// that is longer than what each of the CUs' places gets keeps the others waiting.  A part costs its sums' way to memory and back, so
+// none is shorter than 16 blocks, and all parts' sums fit kShareBytes.
 constexpr int64_t kShareBytes = (int64_t)64 << 20;
 struct Splits {
   int x = 1, w = 1;
 };
-// The tile of the gradients' products, whose tiles are counted together.  One plane: 256 x 256 from 500 tiles on (10,000 x 2,333 x
-// 4,168 655 us against 718 with 128 x 128; 4,096 rows, 330 tiles, 365 against 334), 128 x 128 from 600 of those on (1,120 rows 134
-// against 138 with 64 x 64), else, and up to 400 rows, whose product with the weight is soon over, 64 x 64 (256 rows 78 against 80
-// and 86).  Two planes: 128 x 192 but for few tiles.
-Shape grad_shape(int planes, const Call &c, int64_t rows) {
-  const int64_t m = (c.gx ? rows : 0) + (c.gw ? c.v : 0);
-  if (planes == 2) return shape_of(2, m, c.d);
-  if (rows <= 400) return kSmall;
-  return tiles_of(m, c.d, 256, 256) >= 500 ? kLarge : tiles_of(m, c.d, 128, 128) >= 600 ? kMedium : kSmall;
-}
 Splits splits_of(int planes, const Call &c, int64_t rows) {
-  const Shape s = grad_shape(planes, c, rows);
-  const int64_t tm = s == kSmall ? 64 : planes == 2 ? 192 : s == kMedium ? 128 : 256;
-  const int64_t tn = s == kSmall ? 64 : planes == 2 || s == kMedium ? 128 : 256;
-  const int64_t places = planes == 2 ? (s == kSmall ? 512 : 256) : s == kLarge ? 256 : 512;
-  auto tiles = [&](int64_t m) { return ((m + tm - 1) / tm) * ((c.d + tn - 1) / tn); };
+  const Tile t = tile_of(planes, grad_shape(planes, c, rows));
   const int64_t kx = (c.v + 31) / 32, kw = (rows + 31) / 32;
-  const int64_t all = (c.gx ? tiles(rows) * kx : 0) + (c.gw ? tiles(c.v) * kw : 0);
-  const double most = std::max(16.0, 0.7 * (double)all / (double)places);
+  const int64_t all = (c.gx ? tiles_of(t, rows, c.d) * kx : 0) + (c.gw ? tiles_of(t, c.v, c.d) * kw : 0);
+  const double most = std::max(16.0, (double)all / (double)t.places);
   auto parts = [&](int64_t m, int64_t k) {
     const int64_t fit = kShareBytes / 2 / (m * round_up(c.d, 32) * 4);
     return (int)std::max<int64_t>(1, std::min((int64_t)((double)k / most + 0.99), fit));
@@ -783,7 +862,7 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     else if (slabs <= 6) lay(k_lay<T, 6>);
     else lay(k_lay<T, 0>);
     check_launch("read-out operands");
-    const Shape wide = shape_of(P, rows, c.v);
+    const Shape wide = logits_shape(P, rows, c.v);
     const int parts = parts_of(P, wide, padded);
     const float2 *stat = reinterpret_cast<const float2 *>(at(s.stat));
     auto logits = [&](auto keep) {
@@ -803,18 +882,10 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     check_launch("read-out loss");
     if (!c.grads()) continue;
     hipLaunchKernelGGL((k_logits_grad<H, P, KEPT>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, at(s.z),
-                       (int64_t)padded, rows, (int)c.v, list, stat, s.parts, wide == kSmall ? 5 : 6, info, floats(s.factor),
+                       (int64_t)padded, rows, (int)c.v, list, stat, s.parts, part_shift(P, wide), info, floats(s.factor),
                        floats(s.turned), unit_w, maxima, 2 * rb, (int)s.vb, c.gx ? blocks(s.g) : nullptr,
                        c.gw ? blocks(s.gt) : nullptr, c.gb ? floats(s.sums) : nullptr, (int64_t)padded);
     check_launch("read-out gradient");
-    if (c.gb)
-      by_type(g.bias_type, "the bias must be float32, float16 or bfloat16", [&](auto b) {
-        using B = decltype(b);
-        hipLaunchKernelGGL(k_bias_grad<B>, dim3(blocks_for(c.v, 64)), dim3(1024), 0, st, floats(s.sums), (int64_t)padded, tiles,
-                           (int)c.v, first ? floats(s.acc_b) : nullptr, last ? nullptr : floats(s.acc_b),
-                           static_cast<B *>(g.gb));
-        check_launch("read-out gradient");
-      });
     const Shape shape = grad_shape(P, c, rows);
     const Splits splits = splits_of(P, c, rows);
     const int64_t ld_sum = s.db * 32;
@@ -833,13 +904,19 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     else if (c.gx) product<H, P>(shape, Products<GradOut<T>, 1>{{by_rows}, {to_x}}, st);
     else if (c.gw) product<H, P>(shape, Products<GradOut<T>, 1>{{by_columns}, {to_w}}, st);
     auto join = [&](const GradOut<T> &o, int parts_of_k) {
-      if (!o.share) return;
-      hipLaunchKernelGGL(k_join<T>, dim3((unsigned)std::min<int64_t>((o.rows * ld_sum / 4 + 255) / 256, 4096)), dim3(256), 0, st, o,
-                         parts_of_k);
-      check_launch("read-out gradient");
+      return Join<T>{o, parts_of_k, o.share ? (int)std::min<int64_t>((o.rows * ld_sum / 4 + 1023) / 1024, 1024) : 0};
     };
-    if (c.gx) join(to_x, splits.x);
-    if (c.gw) join(to_w, splits.w);
+    const Join<T> join_x = join(to_x, splits.x), join_w = join(to_w, splits.w);
+    const int bias_groups = c.gb ? (int)blocks_for(c.v, 32) : 0;
+    if (bias_groups + join_x.groups + join_w.groups)
+      by_type(g.bias_type, "the bias must be float32, float16 or bfloat16", [&](auto b) {
+        using B = decltype(b);
+        const BiasOut<B> bias{floats(s.sums), padded, tiles, (int)c.v, first ? floats(s.acc_b) : nullptr,
+                              last ? nullptr : floats(s.acc_b), static_cast<B *>(g.gb)};
+        hipLaunchKernelGGL((k_finish<T, B>), dim3((unsigned)(bias_groups + join_x.groups + join_w.groups)), dim3(1024), 0, st, bias,
+                           bias_groups, join_x, join_w);
+        check_launch("read-out gradient");
+      });
   }
 }
 
