@@ -15,7 +15,7 @@ namespace fly {
 namespace {
 
 constexpr float kUnit = 16384.0f;            // u is multiplied as 2^14 u: float16 then holds it from 2^-28 on without loss
-constexpr int64_t kPieceBytes = (int64_t)1 << 31;   // of a piece of rows: its logits, u, and x laid out
+constexpr int64_t kPieceBytes = (int64_t)1 << 32;   // of a piece of rows: its logits, u, and x laid out
 constexpr int64_t kPieceRows = (int64_t)1 << 19;    // a piece at most: tiles of rows are counted in 16 bits
 
 // The largest of the weights' units and of the rows' factors times theirs, by which products over columns and over rows are scaled.

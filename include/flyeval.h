@@ -520,7 +520,7 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
  *   gx (rows, ldgx), gw (v, ldgw) of `type` and gb (v) of bias_type: grad_scale times the gradient of sum_r row_scale[r] loss[r]
  *   (row_scale NULL: 1) by x, w and bias; of no rows they are 0.
  * Sums are float32; float32 operands are multiplied as two float16 each, 22 bits.  The workspace, 256-byte aligned, holds both
- * operands laid out and logits of as many rows as fit 2 GiB; it depends on `wanted`, the gradients that are not NULL.  The
+ * operands laid out and logits of as many rows as fit 4 GiB; it depends on `wanted`, the gradients that are not NULL.  The
  * outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums, but for rows of
  * x without a target, which count as zeros whatever they hold. */
 enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };

@@ -53,7 +53,7 @@ def test_readout_workspace(lib):
     assert need(0, -1, 8, 9, 1, 7) == 0 and need(5, 4, 8, 9, 1, 7) == 0 and need(0, 4, 8, 9, 0, 7) == 0
     assert 0 < need(1, 4, 8, 9, 1, 0) < need(1, 4, 8, 9, 1, 7)
     # rows beyond a piece take no more: the logits are not kept
-    assert need(2, 1 << 22, 64, 32000, 1, 7) == need(2, 1 << 30, 64, 32000, 1, 7) < (9 << 30) // 4
+    assert need(2, 1 << 22, 64, 32000, 1, 7) == need(2, 1 << 30, 64, 32000, 1, 7) < (9 << 30) // 2
 
 
 def _clip(lib, grads=(P,), sizes=(4,), types=(0,), kind=2, limit=1.0, norm=P, ws=P, need=1 << 20):
