@@ -5,7 +5,14 @@
 //   u_rv = (A_r p_rv - sum_{j: t_rj = v} a_rj) / B_r               A = sum_j a, B = sum_j |a|: |u| <= 2 whatever the weights
 //   dx_r = f_r sum_v u_rv w_v,  dw_v = sum_r f_r u_rv x_r,  db_v = sum_r f_r u_rv,   f = B row_scale grad_scale
 //
-// Rows run in pieces whose logits and u fit a bounded workspace.
+// Rows run in pieces whose logits and u fit a bounded workspace.  A piece is six launches:
+//   k_lay          the weight (once) and the rows into the matrix cores' blocks, for both directions; the rows' targets
+//   k_blocks       logits, and what is kept of them (LogitsOut)
+//   k_loss_rows    the rows' log-sum-exp and losses
+//   k_logits_grad  u into blocks for both directions, its columns' sums
+//   k_blocks       dx and dw side by side (GradOut)
+//   k_finish       db, and the sums of products that ran in parts
+// The loss alone is the first three.  Nothing depends on which workgroup comes first, so results repeat bit for bit.
 #include "blocks.hpp"
 #include "readout.hpp"
 
@@ -22,6 +29,7 @@ constexpr int64_t kPieceRows = (int64_t)1 << 19;    // a piece at most: tiles of
 struct Maxima {
   float weight, row;
 };
+
 // ---- targets ---------------------------------------------------------------------------------------------------------
 
 // A row's targets as the later kernels take them: each column once (-1: none) with its weights added up, and over the row the sum
@@ -108,7 +116,8 @@ struct Lays {
 
 constexpr int kSlab = 512;   // columns that pass through LDS at a time
 
-// 16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
+// Bound by memory: a float32 weight of 4,168 x 2,333 with 256 rows 27 us (41 MB in, 82 out: 4.5 TB/s), a bfloat16 one with 16,384 rows
+// 67 us (96 MB in, 192 out).  16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
 // its maximum to its planes; 0: rows of any length, read from memory once more for the maximum.
 template <typename T, int SLABS>
 __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
@@ -247,6 +256,7 @@ constexpr uint32_t kNone = 65535;
 enum Keep { kNothing, kFloats, kCodes };
 template <Keep KEEP>
 struct LogitsOut {
+  static constexpr bool kLogits = true;
   const float *unit_m, *unit_n;   // or null
   const float *bias;
   const uint8_t *legal;
@@ -433,7 +443,8 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ pa
 constexpr int kGradRows = 64, kGradCols = 128, kGradPitch = 130;
 
 // u of 64 rows x 128 columns into blocks, by rows (times the columns' units) and turned (times the rows' factors), and its
-// columns' sums.  Parts of 2^shift columns.
+// columns' sums.  Parts of 2^shift columns.  Bound by memory and by the way there: all loads go first, then the tile passes through
+// LDS (16,384 x 4,168 bfloat16 110 us, 137 MB in and 273 out; with each load behind the step before it 170).
 template <typename H, int P, Keep KEEP>
 __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z, int64_t ldz, int rows, int cols, const List l,
                                                      const float2 *__restrict__ parts, int64_t ld_parts, int shift,
@@ -577,6 +588,7 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
 // to `share` and k_finish adds them up.
 template <typename T>
 struct GradOut {
+  static constexpr bool kLogits = false;
   const float *row;          // or null
   const float *scale;        // a maximum, or null
   int rows, cols;
@@ -688,85 +700,16 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 
 
 
-// The workgroup's tile (m x n): one plane 64 x 64 (4 waves), 128 x 128 (8) or 256 x 256 (16), two planes 64 x 64 (4), 128 x 128 (16) or
-// 192 x 128 (8).  64 x 64, and 128 x 128 of one plane, run two workgroups per CU, the others one.
-enum Shape { kSmall, kMedium, kLarge };
-struct Tile {
-  int m, n, places;   // and how many of them run at once
-};
-Tile tile_of(int planes, Shape s) {
-  if (s == kSmall) return {64, 64, 512};
-  if (s == kMedium) return {128, 128, planes == 2 ? 256 : 512};
-  return planes == 2 ? Tile{192, 128, 256} : Tile{256, 256, 256};
-}
-int64_t tiles_of(const Tile &t, int64_t m, int64_t n) { return ((m + t.m - 1) / t.m) * ((n + t.n - 1) / t.n); }
-
-// The logits' tile: the one whose rounds of workgroups cost least.  A round's cost, from one that fills it, in those of 128 x 128: one
-// plane 0.5 (64 x 64) and 1.85 (256 x 256), two planes 0.72 and 1.6 (192 x 128).  Measured, us of the loss, 64 x 64 / 128 x 128 /
-// large: bfloat16 2,333 into 4,168 256 rows 35 / 39 / 69, 1,120 rows 60 / 49 / 72, 4,096 rows 139 / 108 / 135, 10,000 rows 303 / 223 /
-// 216; 1,024 into 32,000 1,120 rows 158 / 116 / 130, 4,096 rows 445 / 320 / 306; float32 2,333 into 4,168 256 rows 52 / 59 / 79, 543
-// rows 76 / 62 / 81, 1,120 rows 105 / 105 / 88, 4,096 rows 301 / 259 / 239; 1,024 into 32,000 256 rows 116 / 101 / 119, 543 rows 191 /
-// 170 / 152.
-Shape logits_shape(int planes, int64_t m, int64_t n) {
-  const double cost[3] = {planes == 2 ? 0.72 : 0.5, 1.0, planes == 2 ? 1.6 : 1.85};
-  Shape best = kSmall;
-  double least = 0.0;
-  for (Shape s : {kSmall, kMedium, kLarge}) {
-    const Tile t = tile_of(planes, s);
-    const double c = cost[s] * (double)((tiles_of(t, m, n) + t.places - 1) / t.places);
-    if (s == kSmall || c < least) best = s, least = c;
-  }
-  return best;
-}
-// Columns of the logits that a wave of a shape holds, 2 to the this, and how many such parts a row of `cols` columns has.
-int part_shift(int planes, Shape s) { return s == kSmall || (planes == 2 && s == kMedium) ? 5 : 6; }
-int parts_of(int planes, Shape s, int64_t cols) {
-  const Tile t = tile_of(planes, s);
-  return (int)((cols + t.n - 1) / t.n * (t.n >> part_shift(planes, s)));
-}
 template <typename H, int P, typename EP, int COUNT>
 void product(Shape shape, const Products<EP, COUNT> &p, hipStream_t st) {
   if (shape == kSmall) launch_blocks<H, P, 2, 2, 2, 2, 4>(p, st);
   else if constexpr (P == 2) {
-    if (shape == kMedium) launch_blocks<H, P, 4, 4, 2, 2, 4>(p, st);
-    else launch_blocks<H, P, 2, 4, 4, 3, 3>(p, st);
+    if constexpr (EP::kLogits) {   // the gradients' products never take it
+      if (shape == kLarge) return launch_blocks<H, P, 2, 4, 4, 3, 3>(p, st);
+    }
+    launch_blocks<H, P, 4, 4, 2, 2, 4>(p, st);
   } else if (shape == kMedium) launch_blocks<H, P, 2, 4, 4, 2, 4>(p, st);
   else launch_blocks<H, P, 4, 4, 4, 4, 4>(p, st);
-}
-
-// The tile of the gradients' products, whose tiles are counted together; parts of k even their rounds out.  One plane: up to 200 rows,
-// whose product with the rows is soon over, 64 x 64 (bfloat16, 100 rows of 1,024 into 32,000 118 us against 126 and 129), else 256 x 256
-// from 500 tiles on (1,120 rows 339 against 372; 2,333 into 4,168 4,096 rows, 330 tiles, 321 against 296), 128 x 128 from 600 on (1,120
-// rows 125 against 130), else 64 x 64.  Two planes: 128 x 128 from 400 tiles on (4,096 rows 724 us, with 192 x 128 787, with 64 x 64 893;
-// 256 rows 113, 124 and 117), else 64 x 64 (4,096 rows of 512 into 2,000 139 against 145).
-Shape grad_shape(int planes, const Call &c, int64_t rows) {
-  const int64_t m = (c.gx ? rows : 0) + (c.gw ? c.v : 0);
-  if (planes == 2) return tiles_of(tile_of(2, kMedium), m, c.d) >= 400 ? kMedium : kSmall;
-  if (rows <= 200) return kSmall;
-  if (tiles_of(tile_of(1, kLarge), m, c.d) >= 500) return kLarge;
-  return tiles_of(tile_of(1, kMedium), m, c.d) >= 600 ? kMedium : kSmall;
-}
-
-// In how many parts the k of the gradients' products run, side by side in one launch.  Jobs are counted in blocks of k of one tile; one
-// that is longer than what each of the CUs' places gets keeps the others waiting.  A part costs its sums' way to memory and back, so
-// none is shorter than 16 blocks, and all parts' sums fit kShareBytes.
-constexpr int64_t kShareBytes = (int64_t)64 << 20;
-struct Splits {
-  int x = 1, w = 1;
-};
-Splits splits_of(int planes, const Call &c, int64_t rows) {
-  const Tile t = tile_of(planes, grad_shape(planes, c, rows));
-  const int64_t kx = (c.v + 31) / 32, kw = (rows + 31) / 32;
-  const int64_t all = (c.gx ? tiles_of(t, rows, c.d) * kx : 0) + (c.gw ? tiles_of(t, c.v, c.d) * kw : 0);
-  const double most = std::max(16.0, (double)all / (double)t.places);
-  auto parts = [&](int64_t m, int64_t k) {
-    const int64_t fit = kShareBytes / 2 / (m * round_up(c.d, 32) * 4);
-    return (int)std::max<int64_t>(1, std::min((int64_t)((double)k / most + 0.99), fit));
-  };
-  Splits p;
-  if (c.gx) p.x = parts(rows, kx);
-  if (c.gw) p.w = parts(c.v, kw);
-  return p;
 }
 
 // Where everything lies in the workspace.

@@ -1,18 +1,12 @@
 // What the two ways of the read-out loss share: its arguments, targets and rows.
 #pragma once
 
+#include "readout_rules.hpp"
 #include "rows.hpp"
 
 namespace fly {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-struct Call {
-  int32_t type;
-  int64_t rows, d, v, k;
-  bool gx, gw, gb;
-  bool grads() const { return gx || gw || gb; }
-};
 
 struct Targets {
   const void *index;
@@ -114,8 +108,7 @@ inline void by_type(int32_t type, const char *what, F &&f) {
   }
 }
 
-// Few rows, without laying the operands out (readout_few.hip): whether a call goes that way, and what it takes.
-bool few_rows(const Call &c);
+// Few rows, without laying the operands out (readout_few.hip): what a call takes, and the call.
 size_t few_ws(const Call &c);
 void run_few(const Call &c, const Given &g, char *ws, hipStream_t st);
 

@@ -1,5 +1,5 @@
 // The read-out loss of few rows, where laying the weight out would cost more than the products: both operands come from memory as
-// they lie, straight into the matrix cores' registers.
+// they lie.
 //
 //   k_few_logits   z = x w^T + b by blocks of 16 columns, the sums over d shared among a workgroup's 8 waves
 //   k_few_rows     each row's log-sum-exp, targets and loss
@@ -25,7 +25,8 @@ __device__ __forceinline__ float4v product4(float a, float b, float4v c) {
 
 // 16 columns x 16 MB rows.  Rounds of BYTES of each row pass through LDS, so that a wave loads whole kilobytes of a row: read as the
 // matrix cores take them, 64 bytes of 16 rows at a time, 4,168 x 2,333 float32 took 18 us at best.  Of the weights two rounds are
-// in flight while a third is multiplied, of the rows, which the L2 holds, one.
+// in flight while a third is multiplied, of the rows, which the L2 holds, one.  Bound by the weight's bytes: 39 MB 15 us, 131 MB (32,000
+// x 1,024) 40 us.
 template <typename T, int MB, int BYTES>
 __global__ __launch_bounds__(64 * kWaves) void k_few_logits(const T *__restrict__ x, int64_t ldx, int rows,
                                                             const T *__restrict__ w, int64_t ldw, int v, int d,
@@ -270,7 +271,7 @@ struct FewGrads {
   int64_t ldgw;
 };
 
-// A job to each wave.  dx: 64 of d, 16 MB rows and a part of the columns.  dw: 64 x 64 over all rows.
+// Bound by memory, the weight read for dx and dw written: 13 rows of 2,333 into 4,168, 78 MB, 21 us.  A job to each wave.  dx: 64 of d, 16 MB rows and a part of the columns.  dw: 64 x 64 over all rows.
 template <typename T, int MB>
 __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
   const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
@@ -467,16 +468,6 @@ void few(const Call &c, const Given &g, char *ws, hipStream_t st) {
 }
 
 }  // namespace
-
-// Up to 32 rows: at 32 of 2,333 into 4,168 the loss takes 27 us (float32) and 20 (bfloat16) against 43 and 34 with the operands laid
-// out, with gradients 63 and 56 against 95 and 72.  At 48 the loss takes 49 against 43; float32 with gradients 92 against 98, and at
-// 64 100 against 102 (1,024 into 32,000 219 against 250).  A small product's launches cost more than its work: 64 rows of 256 into
-// 2,000 33 us against 40, 96 rows 37 against 40.
-bool few_rows(const Call &c) {
-  if (c.d < (c.type == FLY_F32 ? 4 : 8)) return false;   // rows have a whole piece
-  const int64_t most = c.type == FLY_F32 && c.grads() ? 64 : 32;
-  return c.rows <= most || (c.rows <= 96 && c.rows * c.d * c.v <= (int64_t)1 << 26);
-}
 
 size_t few_ws(const Call &c) { return Few(c).bytes; }
 
