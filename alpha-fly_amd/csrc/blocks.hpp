@@ -96,8 +96,8 @@ struct Products {
 
 // One plane: 16,384 x 2,333 into 4,168 270 us, 1.18e15 operations a second (the library 364 with k padded and 402 without), 256 x 256
 // tiles.  The matrix cores' power is what bounds it: the gradients' products of a masked batch, whose u is mostly zeros, take a tenth
-// less than those of the same batch without a mask.  Two planes: three products for one, 4,096 rows 724 us for all three directions,
-// 1.0e15; there LDS bounds it as much, whose reads (two planes of both operands) take as long as the products.
+// less than those of the same batch without a mask.  Two planes: three products for one, both gradients of 4,096 rows 426 us, 1.12e15;
+// there LDS bounds it as much, whose reads (two planes of both operands) take as long as the products.
 //
 // WN x WM waves, each FN x FM blocks of n x m; S stages of one block of k in LDS, loaded S - 1 ahead.  `ep` takes each wave's
 // sums: ep.tile<FN, FM>(acc, m0, n0, lane, part, split, turn) with a wave's m0 and n0 in rows, its column part, its part of k, and

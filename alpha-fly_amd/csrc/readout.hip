@@ -799,7 +799,7 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
                         floats(s.turned)};
     const unsigned groups = (unsigned)(2 * (lays.of[0].kt + rb));
     auto lay = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, st, lays); };
-    const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // a row of up to 3,072 columns stays in registers
+    const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // up to six slabs of a row stay in registers
     if (c.d < Piece<T>::N) lay(k_lay<T, 0>);
     else if (slabs <= 2) lay(k_lay<T, 2>);
     else if (slabs <= 6) lay(k_lay<T, 6>);

@@ -519,10 +519,10 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
  *   loss[r] = sum_j a_rj (log sum exp z_r - z_r,t_rj), 0 of a row with none;  any of loss, gx, gw, gb may be NULL
  *   gx (rows, ldgx), gw (v, ldgw) of `type` and gb (v) of bias_type: grad_scale times the gradient of sum_r row_scale[r] loss[r]
  *   (row_scale NULL: 1) by x, w and bias; of no rows they are 0.
- * Sums are float32; float32 operands are multiplied as two float16 each, 22 bits.  The workspace, 256-byte aligned, holds both
- * operands laid out and logits of as many rows as fit 4 GiB; it depends on `wanted`, the gradients that are not NULL.  The
- * outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums, but for rows of
- * x without a target, which count as zeros whatever they hold. */
+ * Sums are float32; float32 operands of more than a few rows are multiplied as two float16 each, 22 bits.  The workspace,
+ * 256-byte aligned, holds both operands laid out and logits of as many rows as fit 4 GiB; it depends on `wanted`, the gradients
+ * that are not NULL.  The outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums,
+ * but for rows of x without a target, which count as zeros whatever they hold. */
 enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };
 size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t k, int32_t wanted);
 int fly_readout_loss(const void *x_dev, int32_t type, int64_t ldx, int64_t rows, int64_t d, const void *w_dev, int64_t ldw,
