@@ -200,7 +200,9 @@ class FlyChessNet(nn.Module):
         """The policy's softmax cross entropy over the legal moves and the WDL logits, without the policy's logits: what a training
         step needs of them (chessfly/train.py:126-132 takes the loss from kept logits).  target: readout.Visits, or a move a
         position (readout.readout_loss).  Differentiable by every parameter; the layers run as forward's do under autograd."""
-        _hip.require_device(x, "FlyChessNet.policy_loss")
+        what = "FlyChessNet.policy_loss"
+        _hip.require_device(x, what)
+        nodes = _hip.held_leaves(what, *self.parameters()) if torch.is_grad_enabled() else ()  # noqa: F841  (see readout_loss)
         r = self._outputs(x)
         # a move's logit is linear in the outputs, its from- and to-square terms included: one map of their sum
         frm, to = self.move_from_onehot.t(), self.move_to_onehot.t()

@@ -96,6 +96,20 @@ def test_without_gradients_and_in_evaluation():
         net.policy_loss(x.cpu(), visits, legal)
 
 
+def test_a_networks_capture_beside_an_eager_graph_is_refused():
+    """Before any layer runs: the layers' weights are leaves as well, and the read-out's own are none."""
+    net = _net()
+    x, visits, _, legal, _ = _batch(16)
+    alive = net.policy_loss(x, visits, legal)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            net.policy_loss(x, visits, legal)
+    sum(t.sum() for t in alive).backward()
+    assert all(p.grad.isfinite().all() for p in net.parameters())
+
+
 @pytest.mark.parametrize("rows", [20, 300])
 def test_a_captured_step(rows):
     """Loss, backward, clipping and an update in one graph, replayed between eager steps from the same weights."""
