@@ -267,7 +267,7 @@ void launch_blocks(Products<EP, COUNT> p, hipStream_t st) {
     o.tiles = o.mt * o.nt;
     all += (int64_t)o.mt * o.nt * o.splits;
   }
-  FLY_REQUIRE(all < (int64_t)1 << 32 >> 10, "product too large");   // at up to 1,024 threads
+  FLY_REQUIRE(all < ((int64_t)1 << 32) / (64 * WN * WM), "product too large");   // a launch has fewer than 2^32 threads
   hipLaunchKernelGGL((k_blocks<H, P, WN, WM, FN, FM, S, EP, COUNT>), dim3((unsigned)all), dim3(64 * WN * WM), 0, st, p);
   check_launch("product of blocks");
 }

@@ -116,9 +116,10 @@ struct Lays {
 
 constexpr int kSlab = 512;   // columns that pass through LDS at a time
 
-// Bound by memory: a float32 weight of 4,168 x 2,333 with 256 rows 27 us (41 MB in, 82 out: 4.5 TB/s), a bfloat16 one with 16,384 rows
-// 67 us (96 MB in, 192 out).  16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
+// 16 rows, a wave each; rows past the last are zero.  SLABS > 0: the row stays in registers, all its loads in flight together, from
 // its maximum to its planes; 0: rows of any length, read from memory once more for the maximum.
+// Bound by memory: a float32 weight of 4,168 x 2,333 with 256 rows 27 us (41 MB in, 82 out: 4.5 TB/s), a bfloat16 one with 16,384 rows
+// 67 us (96 MB in, 192 out).
 template <typename T, int SLABS>
 __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   using H = typename Multiplied<T>::H;
@@ -698,8 +699,6 @@ __global__ __launch_bounds__(256) void k_zeros(T *__restrict__ out, int64_t ld, 
 
 // ---- the call --------------------------------------------------------------------------------------------------------
 
-
-
 template <typename H, int P, typename EP, int COUNT>
 void product(Shape shape, const Products<EP, COUNT> &p, hipStream_t st) {
   if (shape == kSmall) launch_blocks<H, P, 2, 2, 2, 2, 4>(p, st);
@@ -792,7 +791,8 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     Lays<T> lays{};
     if (!first)
       lays.of[0] = Lay<T>{static_cast<const T *>(g.w), g.ldw, c.v, c.d, (int)s.db, (int)s.vb, blocks(s.w),
-                          c.gx ? blocks(s.wt) : nullptr, unit_w, g.bias, g.bias_type, floats(s.bias), Targets{}, List{}, nullptr, 0.0f, nullptr, nullptr};
+                          c.gx ? blocks(s.wt) : nullptr, unit_w, g.bias, g.bias_type, floats(s.bias), Targets{}, List{}, nullptr,
+                          0.0f, nullptr, nullptr};
     lays.of[1] = Lay<T>{static_cast<const T *>(g.x) + first * g.ldx, g.ldx, rows, c.d, (int)s.db, rb, blocks(s.x),
                         c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, 0, nullptr, t, list,
                         g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, c.grads() ? floats(s.factor) : nullptr,
@@ -835,7 +835,8 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     const Blocks by_rows{blocks(s.wt), blocks(s.g), (int)(2 * s.db), 2 * rb, (int)s.vb, splits.x, 0, 0, 0};
     const Blocks by_columns{blocks(s.xt), blocks(s.gt), (int)(2 * s.db), (int)(2 * s.vb), rb, splits.w, 0, 0, 0};
     const GradOut<T> to_x{floats(s.factor), P == 2 ? &maxima->weight : nullptr, rows, (int)c.d, nullptr, nullptr, ld_sum,
-                          c.gx ? static_cast<T *>(g.gx) + first * g.ldgx : nullptr, g.ldgx, splits.x > 1 ? floats(s.share_x) : nullptr};
+                          c.gx ? static_cast<T *>(g.gx) + first * g.ldgx : nullptr, g.ldgx,
+                          splits.x > 1 ? floats(s.share_x) : nullptr};
     const GradOut<T> to_w{nullptr, &maxima->row, (int)c.v, (int)c.d, first ? floats(s.acc_w) : nullptr,
                           last ? nullptr : floats(s.acc_w), ld_sum, static_cast<T *>(g.gw), g.ldgw,
                           splits.w > 1 ? floats(s.share_w) : nullptr};

@@ -271,7 +271,8 @@ struct FewGrads {
   int64_t ldgw;
 };
 
-// Bound by memory, the weight read for dx and dw written: 13 rows of 2,333 into 4,168, 78 MB, 21 us.  A job to each wave.  dx: 64 of d, 16 MB rows and a part of the columns.  dw: 64 x 64 over all rows.
+// A job to each wave.  dx: 64 of d, 16 MB rows and a part of the columns.  dw: 64 x 64 over all rows.  Bound by memory, the weight read
+// for dx and dw written: 13 rows of 2,333 into 4,168, 78 MB, 21 us.
 template <typename T, int MB>
 __global__ __launch_bounds__(256) void k_few_grads(const FewGrads<T> o) {
   const int lane = threadIdx.x & 63, low = lane & 15, high = lane >> 4;
