@@ -87,10 +87,12 @@ def bounds(x, w, b, index, dtype, weight=None, legal=None, scale=None, bias_dtyp
     tree = (80 + v / 64) * U
     near = np.minimum(gap, 30.0).max(1)          # terms further down add less than their share of an error
     e_lse = ez_row + 3 * U * near + 2.0 ** -22 + tree + 2.0 ** -21 * np.log2(v + 2.0)
-    t, a, whole, bad = _targets(index, weight, legal, rows, v)
+    t, a, whole, _ = _targets(index, weight, legal, rows, v)
+    # n weights in any order err by (n - 1) U of their sizes' sum, which weights of both signs leave larger than their sum
+    sizes = t if weight is None else _targets(index, np.abs(weight), legal, rows, v)[0]
     n = max(1, np.prod(index.shape) // max(rows, 1))
     lse_gap = np.where(seen, gap, 0.0) + np.log(v)
-    e_loss = (np.abs(t) * (ez + e_lse[:, None] + 4 * U * lse_gap + (n + 8) * U * (lse_gap + 1))).sum(1) \
+    e_loss = (np.abs(t) * (ez + e_lse[:, None] + 4 * U * lse_gap) + sizes * (n + 8) * U * (lse_gap + 1)).sum(1) \
         + whole * (e_lse + 1e-7)
     # u: p by its exponent, the weights' sums, and how it is held
     s = np.abs(np.ones(rows) if scale is None else scale.astype(np.float64))
@@ -101,7 +103,7 @@ def bounds(x, w, b, index, dtype, weight=None, legal=None, scale=None, bias_dtyp
         listed = t != 0                      # the targets' own logits are kept in float32
         ep = ep + np.where(listed, 0.0, p * STEP * 1.01 + np.exp(-32.0))
     u_size = np.abs(a[:, None] * p - t)
-    eg = np.abs(a)[:, None] * ep + (n + 8) * U * (np.abs(a)[:, None] * p + np.abs(t))
+    eg = np.abs(a)[:, None] * ep + (n + 8) * U * (whole[:, None] * p + sizes)
     held = HELD[dtype] * (u_size + eg) + 4 * U * u_size + 1e-38
     eg_row = (eg + held + HELD_LEAST[dtype] * whole[:, None]) * s[:, None]
     size = u_size * s[:, None]

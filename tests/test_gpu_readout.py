@@ -93,6 +93,14 @@ def test_weights_of_both_signs_without_bias(dtype, rows):
     check(call(*t), t, dtype)
 
 
+@pytest.mark.parametrize("rows", [20, 479])
+def test_one_column_with_weights_of_both_signs(rows):
+    """The gradient is 0 but for the weights' sums, taken in two orders."""
+    t = list(case(rows, 17, 1, "bfloat16", k=70, bias="float32", seed=rows))
+    t[4] -= 0.5
+    check(call(*t, grad_scale=0.3), t, "bfloat16", np.full(rows, float(np.float32(0.3))))
+
+
 @pytest.mark.parametrize("rows", [FEW, MANY])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_confident_rows(dtype, rows):
