@@ -85,12 +85,16 @@ __device__ __forceinline__ float list_row(const Targets &t, const List &l, int64
 
 // ---- operands into blocks --------------------------------------------------------------------------------------------
 
-// 2^e with max |row| 2^e in [2^13, 2^14) for rows held as two halves, and its inverse; 1 of a row of zeros or with infinities.
+constexpr int kLeastUnit = -120;   // as a power of 2: its inverse and its products with a half stay in float32's range
+
+// What a row held as two halves is divided by: 2^e with max |row| / 2^e in [2^13, 2^14).  Of a row with NaN or infinities 1, of a row
+// of zeros the least there is: the units' maximum scales the other rows' products, and no bits of theirs may go to a row without any.
 __device__ __forceinline__ float unit_of(float top) {
-  if (!(top > 0.0f) || !(top <= 3.4028234663852886e38f)) return 1.0f;
+  if (top == 0.0f) return ldexpf(1.0f, kLeastUnit);
+  if (!(top <= 3.4028234663852886e38f)) return 1.0f;
   int e;
   (void)frexpf(top, &e);                  // top = m 2^e, m in [1/2, 1)
-  return ldexpf(1.0f, max(e - 14, -120));
+  return ldexpf(1.0f, max(e - 14, kLeastUnit));
 }
 
 template <typename T>
@@ -107,7 +111,7 @@ struct Lay {
   List list;
   const float *row_scale;
   float grad_scale;
-  float *factor, *turned_factor;   // B row_scale grad_scale of a row, and times its unit; or null
+  float *factor, *turned_factor;   // B row_scale grad_scale of a row, and times its unit (0 of zeros held as halves); or null
 };
 template <typename T>
 struct Lays {
@@ -150,6 +154,7 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
 #pragma unroll
     for (int s = 0; s < SLABS; ++s) fetch(held[s], s * kSlab);
   float unit = 1.0f;
+  bool zeros = false;
   if constexpr (P == 2) {
     float top = 0.0f;
     if constexpr (SLABS > 0) {
@@ -167,7 +172,9 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
         for (int e = 0; e < N; ++e) top = __builtin_elementwise_maximum(top, fabsf(element<T>(p, e)));
       }
     }
-    unit = unit_of(wave_reduce(top, [](float a, float b) { return nan_max(a, b); }));
+    top = wave_reduce(top, [](float a, float b) { return nan_max(a, b); });
+    zeros = top == 0.0f;
+    unit = unit_of(top);
     if (lane == 0) o.unit[row] = unit;
   }
   if (o.bias_out && lane == 0) {
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   if (o.factor && lane == 0 && row < o.rows) {
     const float f = in ? whole * (o.row_scale ? o.row_scale[row] : 1.0f) * o.grad_scale : 0.0f;
     o.factor[row] = f;
-    o.turned_factor[row] = f * unit;
+    o.turned_factor[row] = f * (zeros ? 0.0f : unit);
   }
   const float inverse = 1.0f / unit;
   auto slab = [&](Raw16 (&p)[PIECES], int first, int turn) {
