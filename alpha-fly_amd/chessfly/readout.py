@@ -108,7 +108,8 @@ def readout_loss_and_grad(x: torch.Tensor, weight: torch.Tensor, bias: torch.Ten
                           legal: torch.Tensor | None = None,
                           row_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, ReadoutGrads]:
     """The loss of each row (float32) and, in the same pass, the gradients of grad_scale * sum(row_scale * loss) by x, weight and
-    bias (grad_scale = 1 / rows: of the mean).  For training loops; autograd does not follow the results."""
+    bias (grad_scale = 1 / rows: of the mean).  A row whose row_scale is 0 reaches no gradient, whatever it holds.  For training loops;
+    autograd does not follow the results."""
     what = "readout_loss_and_grad"
     c = _checked(x.detach(), weight.detach(), bias.detach() if bias is not None else None, target, legal, what)
     rows = c.x.shape[0]
@@ -151,8 +152,8 @@ def readout_loss(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     columns) bool hides columns.  Differentiable once by x, weight and bias.  reduction: "mean" or "sum" over all rows, or "none"
     (rows) float32.
 
-    A target that `legal` hides, or of weight 0, is left out; a row with none left has loss and gradients 0, whatever it holds.  A
-    target past the columns makes its row NaN."""
+    A target that `legal` hides, or of weight 0, is left out; a row with none left has loss and gradients 0, whatever it holds, and one
+    whose loss gets an upstream gradient of 0 reaches no gradient.  A target past the columns makes its row NaN."""
     what = "readout_loss"
     if reduction not in ("mean", "sum", "none"):
         raise RuntimeError(f"{what}: reduction must be mean, sum or none, got {reduction!r}")

@@ -129,6 +129,7 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
   using H = typename Multiplied<T>::H;
   constexpr int P = Multiplied<T>::P, N = Piece<T>::N, PIECES = kSlab / (64 * N), HELD = SLABS ? SLABS : 1;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][P][16][kSlab + 8];
+  __shared__ __attribute__((aligned(16))) uint16_t passed[16];   // all bits, or none: rows that count for dw
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const bool second = (int)blockIdx.x >= 2 * lays.of[0].kt;
   const Lay<T> &o = lays.of[second];
@@ -182,11 +183,13 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
     if (row < o.rows && o.bias) b = bias_at(o.bias, o.bias_type, row);
     o.bias_out[row] = b;
   }
+  float f = 0.0f;
   if (o.factor && lane == 0 && row < o.rows) {
-    const float f = in ? whole * (o.row_scale ? o.row_scale[row] : 1.0f) * o.grad_scale : 0.0f;
+    if (in) f = whole * (o.row_scale ? o.row_scale[row] : 1.0f) * o.grad_scale;
     o.factor[row] = f;
     o.turned_factor[row] = f * (zeros ? 0.0f : unit);
   }
+  if (lane == 0) passed[wave] = !o.factor || f != 0.0f ? 0xffff : 0;   // read behind the first slab's barrier
   const float inverse = 1.0f / unit;
   auto slab = [&](Raw16 (&p)[PIECES], int first, int turn) {
     auto &part = lds[turn];
@@ -227,12 +230,13 @@ __global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
     if (!o.turned) return;
     const int at = 32 * wave + 16 * (lane >> 5) + (lane & 15), eight = (lane >> 4) & 1;
     const int64_t block = ((int64_t)2 * k + (lane >> 5)) * o.kt + (group >> 1);
+    const int4v rows = *reinterpret_cast<const int4v *>(&passed[8 * eight]);
 #pragma unroll
     for (int q = 0; q < P; ++q) {
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        w[e] = part[q][8 * eight + 2 * e][at] | (uint32_t)part[q][8 * eight + 2 * e + 1][at] << 16;
+        w[e] = (part[q][8 * eight + 2 * e][at] | (uint32_t)part[q][8 * eight + 2 * e + 1][at] << 16) & (uint32_t)rows[e];
       o.turned[(block * P + q) * 64 + 16 * (2 * (group & 1) + eight) + (lane & 15)] =
           int4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
     }
@@ -399,8 +403,8 @@ struct LogitsOut {
 // A wave per row; a first workgroup finds the largest factors.
 __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ parts, int64_t ld_parts, int count, int rows,
                                                    const List l, float *__restrict__ loss, RowInfo *__restrict__ info,
-                                                   const float *__restrict__ turned_factor, const float *__restrict__ unit_n,
-                                                   int cols, Maxima *__restrict__ maxima) {
+                                                   const float *__restrict__ factor, const float *__restrict__ turned_factor,
+                                                   const float *__restrict__ unit_n, int cols, Maxima *__restrict__ maxima) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (info && blockIdx.x == 0) {
     __shared__ float share[2][4];
@@ -443,7 +447,9 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ pa
   if (lane) return;
   const bool some = sums.y != 0.0f;   // NaN too
   if (loss) loss[row] = !some ? 0.0f : sums.y == sums.y ? sum : sums.y;
-  if (info) info[row] = RowInfo{base_of(p.top), log_sum, some ? sums.x / sums.y : 0.0f, sums.y};
+  if (!info) return;
+  const bool passes = some && factor[row] != 0.0f;   // else u is 0, whatever the row holds
+  info[row] = RowInfo{base_of(p.top), log_sum, passes ? sums.x / sums.y : 0.0f, passes ? sums.y : 0.0f};
 }
 
 // ---- the logits' gradient --------------------------------------------------------------------------------------------
@@ -529,7 +535,7 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
   __syncthreads();
   // the targets among these columns, each once
   auto aim = [&](int j, int c) {
-    if (r0 + lane >= rows || j >= l.k || c < c0 || c >= c0 + kGradCols) return;
+    if (r0 + lane >= rows || j >= l.k || c < c0 || c >= c0 + kGradCols || mine.whole == 0.0f) return;
     const int64_t from = j * l.ld + r0 + lane;
     u[lane][c - c0] = mine.share * exp2_of((l.logit[from] - mine.top) * kLog2e - mine.log_sum) - l.weight[from] / mine.whole;
   };
@@ -828,7 +834,7 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     if (c.grads()) logits(std::integral_constant<Keep, KEPT>{});
     else logits(std::integral_constant<Keep, kNothing>{});
     hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4) + c.grads()), dim3(256), 0, st, stat, s.parts, parts, rows, list,
-                       g.loss ? g.loss + first : nullptr, info, floats(s.turned), unit_w, (int)c.v, maxima);
+                       g.loss ? g.loss + first : nullptr, info, floats(s.factor), floats(s.turned), unit_w, (int)c.v, maxima);
     check_launch("read-out loss");
     if (!c.grads()) continue;
     hipLaunchKernelGGL((k_logits_grad<H, P, KEPT>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, at(s.z),

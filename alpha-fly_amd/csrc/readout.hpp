@@ -41,7 +41,8 @@ struct Given {
   int64_t ldgx, ldgw;
 };
 
-// What a row's gradient is made of: p = exp2((z - top) log2 e - log_sum), u = share p - a / whole.
+// What a row's gradient is made of: p = exp2((z - top) log2 e - log_sum), u = share p - a / whole; 0 where the
+// factor is 0 (share and whole 0).
 struct RowInfo {
   float top, log_sum, share, whole;
 };

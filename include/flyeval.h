@@ -522,7 +522,8 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
  * Sums are float32; float32 operands of more than a few rows are multiplied as two float16 each, 22 bits.  The workspace,
  * 256-byte aligned, holds both operands laid out and logits of as many rows as fit 4 GiB; it depends on `wanted`, the gradients
  * that are not NULL.  The outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums,
- * but for rows of x without a target, which count as zeros whatever they hold. */
+ * but for rows of x without a target, which count as zeros whatever they hold, and in the gradients those whose row_scale or
+ * grad_scale is 0: what selects some rows' losses keeps the others' out, however many rows there are. */
 enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };
 size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t k, int32_t wanted);
 int fly_readout_loss(const void *x_dev, int32_t type, int64_t ldx, int64_t rows, int64_t d, const void *w_dev, int64_t ldw,

@@ -46,3 +46,47 @@ def test_nothing_but_zeros(dtype, rows):
         loss, grads = got = call(*t)
         check(got, t, dtype)
         assert not (grads.x if not t[1].any() else grads.weight).any()
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_rows_whose_factor_is_0_keep_what_they_hold(dtype, rows):
+    """row_scale 0 takes a row's loss out of the sum: its NaN and infinities reach no gradient, its loss is what it is."""
+    t = list(case(rows, 50, 60, dtype, k=3, legal=True))
+    out = [8, 9, 13, rows - 1]
+    t[3][out] = t[3][out].abs()
+    t[5][out] = True
+    scale = torch.ones(rows)
+    scale[out] = 0.0
+    want = call(*t, row_scale=scale.to(DEV))
+    check(want, t, dtype, scale.double().numpy())
+    x = t[0].clone()
+    x[8], x[9, 3], x[13, 49], x[rows - 1] = float("nan"), float("inf"), -float("inf"), float("inf")
+    loss, grads = call(x, *t[1:], row_scale=scale.to(DEV))
+    kept = scale.to(DEV) != 0
+    assert loss[~kept].isnan().all() and torch.equal(loss[kept], want[0][kept])
+    assert not grads.x[~kept].any() and all(torch.equal(p, q) for p, q in zip(grads, want[1]))
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_part_of_the_losses_taken_for_the_gradient(dtype, rows):
+    """Selecting some rows' losses gives the others an upstream gradient of 0."""
+    from chessfly.readout import Visits, readout_loss
+    x, w, b, index, weight, _ = on(*case(rows, 50, 60, dtype, k=3))
+    keep = torch.arange(rows, device=DEV) % 3 != 0
+    bad = x.clone()
+    bad[~keep] = float("inf")
+    grads = []
+    for rows_of_x in (x, bad):
+        leaves = [p.clone().requires_grad_() for p in (rows_of_x, w, b)]
+        readout_loss(*leaves, Visits(index, weight), reduction="none")[keep].mean().backward()
+        grads.append([p.grad for p in leaves])
+    assert all(p.isfinite().all() and torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_all_factors_0(rows):
+    t = case(rows, 50, 60, "float32", k=3)
+    loss, grads = call(*t, grad_scale=0.0)
+    assert loss.isfinite().all() and not any(g.any() for g in grads)
