@@ -140,6 +140,8 @@ class _ReadoutLoss(torch.autograd.Function):
     def backward(ctx, up):
         x, weight, bias, legal, index, share = ctx.saved_tensors
         ldx, ldw, ldl = ctx.rest
+        if not any(ctx.needs_input_grad[:3]):
+            return (None,) * 9
         c = _Call(x, ldx, weight, ldw, bias, legal, ldl, index, share)
         grads = _run(c, None, up.float().contiguous(), 1.0, ctx.needs_input_grad[:3])
         return (*grads,) + (None,) * 6
@@ -149,8 +151,8 @@ def readout_loss(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
                  reduction: str = "mean") -> torch.Tensor:
     """Softmax cross entropy of x (rows, d) W^T + b against `target`: Visits, or one column a row (rows) int32 or int64 (negative:
     the row is left out).  x and weight (columns, d) float32, float16 or bfloat16, bias of that type or float32; legal (rows,
-    columns) bool hides columns.  Differentiable once by x, weight and bias.  reduction: "mean" or "sum" over all rows, or "none"
-    (rows) float32.
+    columns) bool hides columns.  Differentiable once by x, weight and bias; a backward pass to the targets' weights raises.
+    reduction: "mean" or "sum" over all rows, or "none" (rows) float32.
 
     A target that `legal` hides, or of weight 0, is left out; a row with none left has loss and gradients 0, whatever it holds, and one
     whose loss gets an upstream gradient of 0 reaches no gradient.  A target past the columns makes its row NaN."""
@@ -158,10 +160,12 @@ def readout_loss(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if reduction not in ("mean", "sum", "none"):
         raise RuntimeError(f"{what}: reduction must be mean, sum or none, got {reduction!r}")
     c = _checked(x, weight, bias, target, legal, what)
-    if any(t is not None and _hip.tracked(t) for t in (x, weight, bias)):
+    share = c.share
+    if share is not None and _hip.tracked(share):
+        share = _hip.undifferentiated(f"{what} by its targets' weights", c.share.clone, c.share)
+    if any(t is not None and _hip.tracked(t) for t in (x, weight, bias, share)):
         nodes = _hip.held_leaves(what, x, weight, bias)  # noqa: F841  (alive until the graph has them)
-        loss = _ReadoutLoss.apply(c.x, c.weight, c.bias, c.legal, c.index, c.share.detach() if c.share is not None else None, c.ldx,
-                                  c.ldw, c.ldl)
+        loss = _ReadoutLoss.apply(c.x, c.weight, c.bias, c.legal, c.index, share, c.ldx, c.ldw, c.ldl)
     else:
         loss = torch.empty(c.x.shape[0], dtype=torch.float32, device=c.x.device)
         _run(c, loss, None, 1.0, (False, False, False))
