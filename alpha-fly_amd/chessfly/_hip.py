@@ -228,14 +228,15 @@ def undifferentiated(what: str, run, *tensors):
 _STREAM, _PROBE = "chessfly.stream", "chessfly.probe"
 
 
-def held_leaves(what: str, *tensors) -> list:
+def held_leaves(what: str, *tensors, refuse: bool = True) -> list:
     """The autograd nodes that collect the gradients of the leaves among the tensors, to be kept until an operator has taken
     them.  A leaf has one such node while any graph of it lives, and the backward pass waits for the stream that was current when
     it was made.  In a captured backward pass a wait for a stream outside the capture ends the process, so a leaf whose node an
-    eager call has made, and whose graph still lives, is refused while its stream is captured."""
+    eager call of this function has made, and whose graph still lives, is refused while its stream is captured.  Nodes made by other
+    operators carry no mark and are taken as they are.  Without `refuse` the nodes are marked alone."""
     nodes = []
     for t in tensors:
-        if t is None or not (t.requires_grad and t.is_leaf):
+        if t is None or not (t.is_cuda and t.requires_grad and t.is_leaf):
             continue
         node = torch.autograd.graph.get_gradient_edge(t).node
         here, made = _raw_stream(t.device.index), node.metadata.get(_STREAM)
@@ -246,7 +247,7 @@ def held_leaves(what: str, *tensors) -> list:
             node = torch.autograd.graph.get_gradient_edge(t).node
             if node.metadata.pop(_PROBE, None) is None:
                 node.metadata[_STREAM] = here
-        elif made != here and torch.cuda.is_current_stream_capturing():
+        elif refuse and made != here and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what}: a graph of a leaf made outside this capture is still alive: drop its results before "
                                "capturing, or capture on its stream")
         nodes.append(node)

@@ -186,11 +186,24 @@ class FlyChessNet(nn.Module):
         u_in = (enc * self.cfg.input_gain).to(dtype).T.contiguous()
         return self.norm(self.brain.forward_io(u_in, self.in_idx, self.out_idx, self.cfg.steps).T.float())
 
+    def _marked(self) -> list:
+        """Marks the graph that a forward under autograd is about to make, so that a capture finds it (_hip.held_leaves).  Every output
+        depends on the encoder's and the recurrence's parameters, so the first one that learns stands for all; where none does, the
+        first of each map's."""
+        if not torch.is_grad_enabled():
+            return []
+        policy = (self.policy, self.policy_from, self.policy_to)
+        first = lambda *modules: next((p for m in modules for p in m.parameters() if p.requires_grad), None)
+        trunk = first(self.encoder, self.brain)
+        leaves = (trunk,) if trunk is not None else (first(*policy), first(self.value))
+        return _hip.held_leaves("FlyChessNet.forward", *leaves, refuse=False)
+
     def _forward_layers(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The forward as separate differentiable layers (chessfly/model.py:95-105): training, or any call
         with autograd enabled.  Under autograd the recurrence is float32 (its sparse products on the device);
         without it, in training mode, the recurrence is the fused device forward_io in infer_dtype and the
         normaliser updates its running statistics."""
+        nodes = self._marked()  # noqa: F841  (alive until the graph has them)
         r = self._outputs(x)
         logits = self.policy(r) + self.policy_from(r) @ self.move_from_onehot + self.policy_to(r) @ self.move_to_onehot
         return logits, self.value(r)

@@ -41,3 +41,61 @@ def test_the_targets_weights_have_no_forward_derivative():
     x, w, b, index, weight, _ = on(*case(20, 9, 12, "float32", k=3))
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         readout_loss(x, w, b, Visits(index, forward_ad.make_dual(weight, torch.ones_like(weight))))
+
+
+def _net():
+    from chessfly.synthetic import GraphSpec, synthetic_net
+    net, _ = synthetic_net(GraphSpec(n=1500, edges=40_000, n_sensory=150, n_output=60, seed=5), steps=3, seed=0, device=DEV)
+    return net.train()
+
+
+def _mark(p):
+    return torch.autograd.graph.get_gradient_edge(p).node.metadata.get("chessfly.stream")
+
+
+@pytest.mark.parametrize("learns", ["all", "recurrence", "maps"])
+@pytest.mark.parametrize("kept", ["logits", "wdl"])
+def test_a_forwards_graph_is_found_by_a_capture(kept, learns):
+    """An eager forward of the network whose results live: a captured policy_loss of the same leaves is refused before any layer
+    runs.  Once they are dropped, nothing is left of it."""
+    from chessfly.synthetic import synthetic_boards
+    net = _net()
+    for name, p in net.named_parameters():
+        trunk = name.startswith(("encoder", "brain"))
+        p.requires_grad_(learns == "all" or (name.startswith("brain") if learns == "recurrence" else not trunk))
+    x = torch.as_tensor(synthetic_boards(8, seed=0), dtype=torch.float32, device=DEV)
+    target = torch.zeros(8, dtype=torch.int64, device=DEV)
+    marked = [p for p in net.parameters() if p.requires_grad]
+    assert not any(_mark(p) is not None for p in marked)
+    alive = net(x)[kept == "wdl"]
+    assert any(_mark(p) is not None for p in marked)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(graph):
+            net.policy_loss(x, target)
+    alive.sum().backward()
+    del alive
+    assert not any(_mark(p) is not None for p in marked)
+    with torch.no_grad():
+        out = net(x)
+    assert not any(_mark(p) is not None for p in marked) and out[0].isfinite().all()
+
+
+def test_a_captured_forward_beside_an_eager_graph_still_runs():
+    """Only its backward pass would wait for the other stream: the forward is marked, not refused."""
+    from chessfly import _hip
+    w = torch.ones(3, device=DEV, requires_grad=True)
+    nodes = _hip.held_leaves("eager", w)
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros(3, device=DEV)
+    with torch.cuda.graph(graph):
+        assert _hip.held_leaves("captured", w, refuse=False)[0] is not None
+        with pytest.raises(RuntimeError, match="captured: .* still alive"):
+            _hip.held_leaves("captured", w)
+        out.add_(w.detach())
+    for n in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, torch.full_like(out, float(n)))
+    assert len(nodes) == 1 and _hip.held_leaves("host", torch.ones(2, requires_grad=True)) == []
