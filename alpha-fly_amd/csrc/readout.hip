@@ -22,13 +22,6 @@ namespace fly {
 namespace {
 
 constexpr float kUnit = 16384.0f;            // u is multiplied as 2^14 u: float16 then holds it from 2^-28 on without loss
-constexpr int64_t kPieceBytes = (int64_t)1 << 32;   // of a piece of rows: its logits, u, and x laid out
-constexpr int64_t kPieceRows = (int64_t)1 << 19;    // a piece at most: tiles of rows are counted in 16 bits
-
-// The largest of the weights' units and of the rows' factors times theirs, by which products over columns and over rows are scaled.
-struct Maxima {
-  float weight, row;
-};
 
 // ---- targets ---------------------------------------------------------------------------------------------------------
 
@@ -723,61 +716,6 @@ void product(Shape shape, const Products<EP, COUNT> &p, hipStream_t st) {
   } else if (shape == kMedium) launch_blocks<H, P, 2, 4, 4, 2, 4>(p, st);
   else launch_blocks<H, P, 4, 4, 4, 4, 4>(p, st);
 }
-
-// Where everything lies in the workspace.
-struct Space {
-  int64_t piece;      // rows at a time
-  int64_t db, vb, rb; // blocks of 32
-  int parts;
-  bool several;
-  size_t x, xt, w, wt, z, g, gt, unit_x, unit_w, bias, stat, info, factor, turned, sums, maxima, acc_w, acc_b, column, weight,
-      logit, list_sums, share_x, share_w, bytes;
-  Space(const Call &c, int planes) {
-    db = (c.d + 31) / 32;
-    vb = (c.v + 31) / 32;
-    parts = parts_of(planes, kSmall, vb * 32);   // the most that a shape has, but for a tile's rounding
-    parts = (int)round_up(parts, 4);
-    const int64_t kept = c.grads() ? planes * 2 : 0;   // bytes of a logit
-    const int64_t each = vb * 32 * (kept + 2 * planes * ((c.gx ? 1 : 0) + (c.gw ? 1 : 0))) + db * 64 * planes * (c.gw ? 2 : 1) +
-                         12 * c.k + 8 * parts_of(planes, kSmall, vb * 32);
-    piece = std::min({round_up(c.rows, 64), std::max<int64_t>(kPieceBytes / each / 64 * 64, 64), kPieceRows});
-    several = piece < c.rows;
-    rb = piece / 32;
-    size_t at = 0;
-    auto take = [&](int64_t n) {
-      const size_t was = at;
-      at += align256((size_t)n);
-      return was;
-    };
-    const int64_t block = 2048 * planes;   // of 32 x 32
-    x = take(rb * db * block);
-    xt = c.gw ? take(rb * db * block) : 0;
-    w = take(vb * db * block);
-    wt = c.gx ? take(vb * db * block) : 0;
-    z = kept ? take(piece * vb * 32 * kept) : 0;
-    g = c.gx ? take(rb * vb * block) : 0;
-    gt = c.gw ? take(rb * vb * block) : 0;
-    unit_x = take(rb * 32 * 4);
-    unit_w = take(vb * 32 * 4);
-    bias = take(vb * 32 * 4);
-    stat = take(piece * parts * 8);
-    info = take(piece * sizeof(RowInfo));
-    factor = take(piece * 4);
-    turned = take(piece * 4);
-    sums = c.gb ? take(piece / 64 * vb * 32 * 4) : 0;
-    maxima = take(sizeof(Maxima));
-    acc_w = several && c.gw ? take(c.v * db * 32 * 4) : 0;
-    acc_b = several && c.gb ? take(vb * 32 * 4) : 0;
-    column = take(piece * c.k * 4);
-    weight = take(piece * c.k * 4);
-    logit = take(piece * c.k * 4);
-    list_sums = take(piece * 8);
-    const Splits p = splits_of(planes, c, piece < c.rows ? piece : c.rows);
-    share_x = several && c.gx ? take(kShareBytes / 2) : p.x > 1 ? take(p.x * c.rows * db * 128) : 0;
-    share_w = several && c.gw ? take(kShareBytes / 2) : p.w > 1 ? take(p.w * c.v * db * 128) : 0;
-    bytes = at;
-  }
-};
 
 template <typename T>
 void run(const Call &c, const Given &g, char *ws, hipStream_t st) {

@@ -41,12 +41,6 @@ struct Given {
   int64_t ldgx, ldgw;
 };
 
-// What a row's gradient is made of: p = exp2((z - top) log2 e - log_sum), u = share p - a / whole; 0 where the
-// factor is 0 (share and whole 0).
-struct RowInfo {
-  float top, log_sum, share, whole;
-};
-
 // Piece i of a row of `cols` as it lies in memory, zeros past its end.
 template <typename T>
 __device__ __forceinline__ Raw16 load_raw(const T *__restrict__ row, int i, int64_t cols) {
