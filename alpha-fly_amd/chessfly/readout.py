@@ -4,9 +4,14 @@ fly_readout_loss.
     z_r  = x_r W^T + b over the legal columns
     loss = sum_j a_rj (log sum exp z_r - z_r,t_rj)      a list of columns t with weights a (visits), or one column with weight 1
 
-and its gradients by x, W and b.  Logits exist for a bounded number of rows at a time, so memory does not grow with rows times
-columns; sums are float32 whatever the type, and results do not depend on scheduling.  No counterpart in the reference, whose
-training takes torch's softmax over all logits.
+and its gradients by x, W and b.  The loss alone keeps no logits; with gradients those of a piece of rows at a time are kept with their
+gradients, 12 bytes of a float32 logit and 6 of a 16-bit one, 4 GiB at most, beside both operands laid out for the matrix cores.  Past
+that size memory no longer grows with rows times columns; below it, a call takes more than float32 logits alone would.
+
+Sums are float32 whatever the type, and results do not depend on scheduling.  From some dozens of rows on float32 operands are
+multiplied in 22 bits, and with 16-bit ones the logits' gradient is rounded to their type before its products (include/flyeval.h): the
+gradients then err by 1.2 times what rounding them to the type does, in the norm.  float32 operands avoid that.  No counterpart in the
+reference, whose training takes torch's softmax over all logits.
 """
 
 from __future__ import annotations

@@ -519,11 +519,18 @@ int fly_distill(const void *z_dev, int32_t type, int64_t ldz, int64_t rows, int6
  *   loss[r] = sum_j a_rj (log sum exp z_r - z_r,t_rj), 0 of a row with none;  any of loss, gx, gw, gb may be NULL
  *   gx (rows, ldgx), gw (v, ldgw) of `type` and gb (v) of bias_type: grad_scale times the gradient of sum_r row_scale[r] loss[r]
  *   (row_scale NULL: 1) by x, w and bias; of no rows they are 0.
- * Sums are float32; float32 operands of more than a few rows are multiplied as two float16 each, 22 bits.  The workspace,
- * 256-byte aligned, holds both operands laid out and logits of as many rows as fit 4 GiB; it depends on `wanted`, the gradients
- * that are not NULL.  The outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums,
- * but for rows of x without a target, which count as zeros whatever they hold, and in the gradients those whose row_scale or
- * grad_scale is 0: what selects some rows' losses keeps the others' out, however many rows there are. */
+ * Sums are float32.  What is held in fewer bits, beside the outputs' own rounding to their types, is so from the sizes on at which
+ * laying the operands out pays (more than 32 rows; float32 with gradients 64; small products 96), and not below:
+ *   float32      x and w are multiplied as two float16 each, 22 bits of a row's largest value, and the logits' gradient u too, 22 bits
+ *                or 2^-50 of the largest row of w (for gx) or of x times its factor (for gw), whichever is coarser
+ *   16-bit types u is rounded to the type before its products, as the matrix cores take it: half a step of each of its elements.  Beside
+ *                the targets it comes from logits held to 2^-12, and is 0 where they lie more than 32 below the largest of their 64
+ * A caller who wants u unrounded gives float32.  The workspace, 256-byte aligned, holds both operands laid out, in one direction or with
+ * gradients in both, and of a piece of rows at a time the logits and u, 12 bytes of a float32 logit with gradients gx and gw, 6 of a
+ * 16-bit one, and of the loss alone 8 bytes for 32 columns: up to 4 GiB a piece and 2^19 rows.  It depends on `wanted`, the gradients that
+ * are not NULL.  The outputs must not overlap the inputs or each other.  Infinities and NaN of x and w go through the sums, but for rows
+ * of x without a target, which count as zeros whatever they hold, and in the gradients those whose row_scale or grad_scale is 0: what
+ * selects some rows' losses keeps the others' out, however many rows there are. */
 enum fly_readout_grads { FLY_GRAD_X = 1, FLY_GRAD_W = 2, FLY_GRAD_B = 4 };
 size_t fly_readout_loss_workspace(int32_t type, int64_t rows, int64_t d, int64_t v, int32_t k, int32_t wanted);
 int fly_readout_loss(const void *x_dev, int32_t type, int64_t ldx, int64_t rows, int64_t d, const void *w_dev, int64_t ldw,

@@ -4,10 +4,12 @@ is 0, batches in pieces.  Against the float64 oracle within its bounds, on the k
 from __future__ import annotations
 
 import numpy as np
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_readout import DEV, FEW, MANY, call, case, check, on
+from oracle import readout as O
+from test_gpu_readout import DEV, FEW, MANY, call, case, check, numpy, on
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +92,43 @@ def test_all_factors_0(rows):
     t = case(rows, 50, 60, "float32", k=3)
     loss, grads = call(*t, grad_scale=0.0)
     assert loss.isfinite().all() and not any(g.any() for g in grads)
+
+
+def _within(got, want, most):
+    off = np.abs(got.double().cpu().numpy() - want)
+    assert (off <= most).all(), float((off / most).max())
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_large_rows_of_the_weight_that_no_row_sees(rows):
+    """The others, 2^20 times smaller, are within the bounds of a weight without any large row."""
+    x, w, b, index, weight, legal = case(rows, 64, 90, "float32", seed=rows, k=3, legal=True)
+    hidden = torch.arange(90) % 6 == 1
+    legal = legal & ~hidden
+    small = w * 2.0 ** -20
+    w = torch.where(hidden[:, None], w, small)
+    loss, grads = call(x, w, b, index, weight, legal)
+    args = numpy(x, w, b, index, weight, legal)
+    n = lambda m: (m[0], m[1], m[2], m[3], "float32", *m[4:])
+    want, most = O.loss(*args), O.bounds(*n(numpy(x, small, b, index, weight, legal)))
+    for got, e, m in zip((loss, *grads), want, most):
+        _within(got, e, m)
+
+
+@pytest.mark.parametrize("rows", [2 * FEW, MANY])
+def test_large_rows_of_x_that_see_other_columns(rows):
+    """What rows 2^20 times smaller give their columns is within the bounds of those rows alone."""
+    x, w, b, index, weight, _ = case(rows, 64, 90, "float32", seed=rows, k=3)
+    half = rows // 2
+    legal = torch.zeros(rows, 90, dtype=torch.bool)
+    legal[:half, :45] = legal[half:, 45:] = True
+    index = index % 45
+    index[half:] += 45
+    x[half:] *= 2.0 ** -20
+    loss, grads = call(x, w, b, index, weight, legal)
+    part = numpy(*(t[half:] if t.shape[0] == rows else t for t in (x, w, b, index, weight, legal)))
+    want, most = O.loss(*part), O.bounds(*part[:4], "float32", *part[4:])
+    _within(loss[half:], want[0], most[0])
+    _within(grads.x[half:], want[1], most[1])
+    _within(grads.weight[45:], want[2][45:], most[2][45:])
+    _within(grads.bias[45:], want[3][45:], most[3][45:])
