@@ -117,8 +117,9 @@ constexpr int kSlab = 512;   // columns that pass through LDS at a time
 // its maximum to its planes; 0: rows of any length, read from memory once more for the maximum.
 // Bound by memory: a float32 weight of 4,168 x 2,333 with 256 rows 27 us (41 MB in, 82 out: 4.5 TB/s), a bfloat16 one with 16,384 rows
 // 67 us (96 MB in, 192 out).
+// 64 registers at most, for two workgroups a CU: with 66 the calls of 256 and of 1,120 float32 positions take 3 us more.
 template <typename T, int SLABS>
-__global__ __launch_bounds__(1024) void k_lay(const Lays<T> lays) {
+__global__ __launch_bounds__(1024, 8) void k_lay(const Lays<T> lays) {
   using H = typename Multiplied<T>::H;
   constexpr int P = Multiplied<T>::P, N = Piece<T>::N, PIECES = kSlab / (64 * N), HELD = SLABS ? SLABS : 1;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2][P][16][kSlab + 8];
