@@ -2,8 +2,9 @@
 
     norm = sqrt(sum g^2) or max |g|,    g <- g * min(1, limit / (norm + 1e-6))
 
-Arguments as torch.nn.utils.clip_grad_norm_ takes them.  Gradients may differ in type (float32, float16, bfloat16) and size;
-squares are summed in float64.  Gradients of norm below the limit are read and not written.
+Arguments as torch.nn.utils.clip_grad_norm_ takes them, but for `foreach`; the norms are 2 and inf, all gradients lie on one device and
+each parameter is given once.  Gradients may differ in type (float32, float16, bfloat16) and size; squares are summed in float64.
+Gradients of norm below the limit are read and not written.
 """
 
 from __future__ import annotations

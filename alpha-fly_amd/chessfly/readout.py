@@ -10,7 +10,7 @@ that size memory no longer grows with rows times columns; below it, a call takes
 
 Sums are float32 whatever the type, and results do not depend on scheduling.  From some dozens of rows on float32 operands are
 multiplied in 22 bits, and with 16-bit ones the logits' gradient is rounded to their type before its products (include/flyeval.h): the
-gradients then err by 1.2 times what rounding them to the type does, in the norm.  float32 operands avoid that.  No counterpart in the
+gradients then err by 1.1 to 1.4 times what rounding them to the type does, in the norm.  float32 operands avoid that.  No counterpart in the
 reference, whose training takes torch's softmax over all logits.
 """
 
