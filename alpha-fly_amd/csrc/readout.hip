@@ -104,7 +104,8 @@ struct Lay {
   List list;
   const float *row_scale;
   float grad_scale;
-  float *factor, *turned_factor;   // B row_scale grad_scale of a row, and times its unit (0 of zeros held as halves); or null
+  float *factor;           // B row_scale grad_scale of a row, or null
+  double *turned_factor;   // and times its unit (0 of zeros held as halves)
 };
 template <typename T>
 struct Lays {
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(1024, 8) void k_lay(const Lays<T> lays) {
   if (o.factor && lane == 0 && row < o.rows) {
     if (in) f = whole * (o.row_scale ? o.row_scale[row] : 1.0f) * o.grad_scale;
     o.factor[row] = f;
-    o.turned_factor[row] = f * (zeros ? 0.0f : unit);
+    o.turned_factor[row] = (double)f * (zeros ? 0.0f : unit);
   }
   if (lane == 0) passed[wave] = !o.factor || f != 0.0f ? 0xffff : 0;   // read behind the first slab's barrier
   const float inverse = 1.0f / unit;
@@ -397,15 +398,17 @@ struct LogitsOut {
 // A wave per row; a first workgroup finds the largest factors.
 __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ parts, int64_t ld_parts, int count, int rows,
                                                    const List l, float *__restrict__ loss, RowInfo *__restrict__ info,
-                                                   const float *__restrict__ factor, const float *__restrict__ turned_factor,
+                                                   const float *__restrict__ factor, const double *__restrict__ turned_factor,
                                                    const float *__restrict__ unit_n, int cols, Maxima *__restrict__ maxima) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (info && blockIdx.x == 0) {
-    __shared__ float share[2][4];
-    float w = 0.0f, r = 0.0f;
-    auto raise = [](float &most, float v) {   // finite ones
-      v = fabsf(v);
-      if (v <= 3.4028234663852886e38f) most = fmaxf(most, v);
+    __shared__ float weight[4];
+    __shared__ double factors[4];
+    float w = 0.0f;
+    double r = 0.0;
+    auto raise = [](auto &most, auto v) {   // finite ones
+      v = v < 0 ? -v : v;
+      if (v > most && v < INFINITY) most = v;
     };
     if (unit_n)
 #pragma unroll 8
@@ -413,12 +416,15 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2 *__restrict__ pa
 #pragma unroll 8
     for (int i = threadIdx.x; i < rows; i += 256) raise(r, turned_factor[i]);
     w = wave_max(w);
-    r = wave_max(r);
-    if (lane == 0) share[0][wave] = w, share[1][wave] = r;
+    for (int d = 1; d < 64; d <<= 1) raise(r, __shfl_xor(r, d));
+    if (lane == 0) weight[wave] = w, factors[wave] = r;
     __syncthreads();
-    if (threadIdx.x == 0)
-      *maxima = Maxima{fmaxf(fmaxf(share[0][0], share[0][1]), fmaxf(share[0][2], share[0][3])),
-                       fmaxf(fmaxf(share[1][0], share[1][1]), fmaxf(share[1][2], share[1][3]))};
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 4; ++i) raise(w, weight[i]), raise(r, factors[i]);
+      int e;
+      const double fraction = frexp(r, &e);
+      *maxima = Maxima{r, w, ldexpf(1.0f, e), (float)fraction};
+    }
     return;
   }
   const int64_t row = (blockIdx.x - (info ? 1 : 0)) * (int64_t)4 + wave;
@@ -458,7 +464,7 @@ template <typename H, int P, Keep KEEP>
 __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z, int64_t ldz, int rows, int cols, const List l,
                                                      const float2 *__restrict__ parts, int64_t ld_parts, int shift,
                                                      const RowInfo *__restrict__ info, const float *__restrict__ factor,
-                                                     const float *__restrict__ turned_factor,
+                                                     const double *__restrict__ turned_factor,
                                                      const float *__restrict__ unit_n, const Maxima *__restrict__ maxima,
                                                      int rb, int vb, int4v *__restrict__ out, int4v *__restrict__ turned,
                                                      float *__restrict__ sums, int64_t ld_sums) {
@@ -479,12 +485,14 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
 #pragma unroll
   for (int j = 0; j < 8; ++j) column[j] = l.column[min(wave + 4 * j, l.k - 1) * l.ld + list_row];
   const RowInfo mine = info[list_row];   // of a row of the lists
-  const float most = maxima->row, most_weight = maxima->weight;
+  const double most = maxima->row;
+  const float most_weight = maxima->weight;
   if (tid < kGradRows) {
     const bool in = r0 + tid < rows;
-    const float f = factor[list_row], ft = turned_factor[list_row];
+    const float f = factor[list_row];
+    const double ft = turned_factor[list_row];
     f_row[tid] = in ? f : 0.0f;
-    ft_row[tid] = in && most > 0.0f ? ft / most * kUnit : 0.0f;
+    ft_row[tid] = in ? (float)(most > 0.0 ? ft / most : ft) * kUnit : 0.0f;
   }
   if (tid >= 128) {
     const int c = c0 + tid - 128;
@@ -593,13 +601,13 @@ __global__ __launch_bounds__(256) void k_logits_grad(const void *__restrict__ z,
 
 // ---- gradients -------------------------------------------------------------------------------------------------------
 
-// out[m][n] = sum * row[m] * *scale / 2^14, after what earlier pieces of rows gave.  Where k runs in parts, the sums of each go
-// to `share` and k_finish adds them up.
+// out[m][n] = sum * *power / 2^14 * row[m] * *times, after what earlier pieces of rows gave.  The power of 2 comes first: with the row's
+// factor it may pass float32's range where the gradient does not.  Where k runs in parts, the sums of each go to `share` and k_finish
+// adds them up.
 template <typename T>
 struct GradOut {
   static constexpr bool kLogits = false;
-  const float *row;          // or null
-  const float *scale;        // a maximum, or null
+  const float *row, *power, *times;   // or null: 1
   int rows, cols;
   const float *before;
   float *after;              // or null: the last piece, into out
@@ -607,12 +615,12 @@ struct GradOut {
   T *out;
   int64_t ld;
   float *share;              // (part, row, column) or null
-  __device__ __forceinline__ float unit() const { return (scale ? *scale : 1.0f) / kUnit; }
-  __device__ __forceinline__ void put(int m, int n, const float4v &sum, float unit) const {
-    const float f = row ? unit * row[m] : unit;
+  __device__ __forceinline__ float2 scale() const { return make_float2((power ? *power : 1.0f) / kUnit, times ? *times : 1.0f); }
+  __device__ __forceinline__ void put(int m, int n, const float4v &sum, float2 scale) const {
+    const float f = row ? row[m] : scale.y;
     float4v w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = sum[e] * f;
+    for (int e = 0; e < 4; ++e) w[e] = sum[e] * scale.x * f;
     if (before) w += *reinterpret_cast<const float4v *>(before + m * ld_sum + n);
     if (after) {
       *reinterpret_cast<float4v *>(after + m * ld_sum + n) = w;
@@ -632,7 +640,7 @@ struct GradOut {
   }
   template <int FN, int FM>
   __device__ __forceinline__ void tile(float4v (&acc)[FN][FM], int m0, int n0, int lane, int, int split, float *turn) const {
-    const float s = unit();
+    const float2 s = scale();
     float *to = share ? share + (int64_t)split * rows * ld_sum : nullptr;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
@@ -688,7 +696,7 @@ __global__ __launch_bounds__(1024) void k_finish(const BiasOut<B> b, int bias_gr
   if (group >= x.groups) group -= x.groups;
   const GradOut<T> &g = j.out;
   const int64_t per = g.ld_sum / 4, all = g.rows * per, stride = g.rows * g.ld_sum;
-  const float s = g.unit();
+  const float2 s = g.scale();
   for (int64_t i = group * (int64_t)1024 + threadIdx.x; i < all; i += (int64_t)j.groups * 1024) {
     const int m = (int)(i / per), n = 4 * (int)(i % per);
     if (n >= g.cols) continue;
@@ -749,7 +757,7 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     lays.of[1] = Lay<T>{static_cast<const T *>(g.x) + first * g.ldx, g.ldx, rows, c.d, (int)s.db, rb, blocks(s.x),
                         c.gw ? blocks(s.xt) : nullptr, unit_x, nullptr, 0, nullptr, t, list,
                         g.row_scale ? g.row_scale + first : nullptr, g.grad_scale, c.grads() ? floats(s.factor) : nullptr,
-                        floats(s.turned)};
+                        reinterpret_cast<double *>(at(s.turned))};
     const unsigned groups = (unsigned)(2 * (lays.of[0].kt + rb));
     auto lay = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(groups), dim3(1024), 0, st, lays); };
     const int64_t slabs = (s.db * 32 + kSlab - 1) / kSlab;   // up to six slabs of a row stay in registers
@@ -774,12 +782,13 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     if (c.grads()) logits(std::integral_constant<Keep, KEPT>{});
     else logits(std::integral_constant<Keep, kNothing>{});
     hipLaunchKernelGGL(k_loss_rows, dim3(blocks_for(rows, 4) + c.grads()), dim3(256), 0, st, stat, s.parts, parts, rows, list,
-                       g.loss ? g.loss + first : nullptr, info, floats(s.factor), floats(s.turned), unit_w, (int)c.v, maxima);
+                       g.loss ? g.loss + first : nullptr, info, floats(s.factor), reinterpret_cast<double *>(at(s.turned)), unit_w,
+                       (int)c.v, maxima);
     check_launch("read-out loss");
     if (!c.grads()) continue;
     hipLaunchKernelGGL((k_logits_grad<H, P, KEPT>), dim3(blocks_for(c.v, kGradCols), tiles), dim3(256), 0, st, at(s.z),
                        (int64_t)padded, rows, (int)c.v, list, stat, s.parts, part_shift(P, wide), info, floats(s.factor),
-                       floats(s.turned), unit_w, maxima, 2 * rb, (int)s.vb, c.gx ? blocks(s.g) : nullptr,
+                       reinterpret_cast<double *>(at(s.turned)), unit_w, maxima, 2 * rb, (int)s.vb, c.gx ? blocks(s.g) : nullptr,
                        c.gw ? blocks(s.gt) : nullptr, c.gb ? floats(s.sums) : nullptr, (int64_t)padded);
     check_launch("read-out gradient");
     const Shape shape = grad_shape(P, c, rows);
@@ -787,10 +796,10 @@ void run(const Call &c, const Given &g, char *ws, hipStream_t st) {
     const int64_t ld_sum = s.db * 32;
     const Blocks by_rows{blocks(s.wt), blocks(s.g), (int)(2 * s.db), 2 * rb, (int)s.vb, splits.x, 0, 0, 0};
     const Blocks by_columns{blocks(s.xt), blocks(s.gt), (int)(2 * s.db), (int)(2 * s.vb), rb, splits.w, 0, 0, 0};
-    const GradOut<T> to_x{floats(s.factor), P == 2 ? &maxima->weight : nullptr, rows, (int)c.d, nullptr, nullptr, ld_sum,
+    const GradOut<T> to_x{floats(s.factor), P == 2 ? &maxima->weight : nullptr, nullptr, rows, (int)c.d, nullptr, nullptr, ld_sum,
                           c.gx ? static_cast<T *>(g.gx) + first * g.ldgx : nullptr, g.ldgx,
                           splits.x > 1 ? floats(s.share_x) : nullptr};
-    const GradOut<T> to_w{nullptr, &maxima->row, (int)c.v, (int)c.d, first ? floats(s.acc_w) : nullptr,
+    const GradOut<T> to_w{nullptr, &maxima->power, &maxima->fraction, (int)c.v, (int)c.d, first ? floats(s.acc_w) : nullptr,
                           last ? nullptr : floats(s.acc_w), ld_sum, static_cast<T *>(g.gw), g.ldgw,
                           splits.w > 1 ? floats(s.share_w) : nullptr};
     if (c.gx && c.gw)   // the longer sums first

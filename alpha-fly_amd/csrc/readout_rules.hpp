@@ -102,9 +102,11 @@ struct RowInfo {
   float top, log_sum, share, whole;
 };
 
-// The largest of the weights' units and of the rows' factors times theirs, by which products over columns and over rows are scaled.
+// The largest of the weights' units and of the rows' factors times theirs, by which products over columns and over rows are scaled.  A
+// factor times a unit may pass float32's range where the gradient does not: it is a double, and as floats power times fraction.
 struct Maxima {
-  float weight, row;
+  double row;
+  float weight, power, fraction;
 };
 
 // Rows run in pieces whose logits, u and x laid out take this much at most, and of as many rows: tiles of rows are counted in 16 bits.
@@ -150,7 +152,7 @@ struct Space {
     stat = take(piece * parts * 8);
     info = take(piece * sizeof(RowInfo));
     factor = take(piece * 4);
-    turned = take(piece * 4);
+    turned = take(piece * 8);
     sums = c.gb ? take(piece / 64 * vb * 32 * 4) : 0;
     maxima = take(sizeof(Maxima));
     acc_w = several && c.gw ? take(c.v * db * 32 * 4) : 0;

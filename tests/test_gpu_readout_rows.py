@@ -132,3 +132,13 @@ def test_large_rows_of_x_that_see_other_columns(rows):
     _within(grads.x[half:], want[1], most[1])
     _within(grads.weight[45:], want[2][45:], most[2][45:])
     _within(grads.bias[45:], want[3][45:], most[3][45:])
+
+
+@pytest.mark.parametrize("of", ["x", "weight"])
+@pytest.mark.parametrize("size", [1e-20, 1e-28, 1e-30, 1e-32, 1e-34])
+@pytest.mark.parametrize("rows", [FEW, MANY])
+def test_small_rows_and_the_mean_over_them(rows, size, of):
+    """The largest of the gradients about size / rows: far above float32's smallest number, as the factors on the way there need not be."""
+    t = list(case(rows, 64, 90, "float32", seed=rows, k=3))
+    t[of == "weight"] = t[of == "weight"] * size
+    check(call(*t, grad_scale=1 / rows), t, "float32", np.full(rows, 1 / rows))

@@ -43,12 +43,12 @@ int main() {
       part(s.stat, ((n - 1) * s.parts + parts_of(planes, logits_shape(planes, n, v), padded)) * 8);
       part(s.info, n * 16);
       part(s.factor, n * 4);
-      part(s.turned, n * 4);
+      part(s.turned, n * 8);
       part(s.column, ((k - 1) * s.piece + n) * 4);
       part(s.weight, ((k - 1) * s.piece + n) * 4);
       part(s.logit, ((k - 1) * s.piece + n) * 4);
       part(s.list_sums, n * 8);
-      if (c.grads()) part(s.maxima, 8);
+      if (c.grads()) part(s.maxima, sizeof(Maxima));
       if (c.gb) part(s.sums, ((tiles - 1) * padded + v) * 4);
       if (s.piece < rows && c.gw) part(s.acc_w, v * s.db * 128);
       if (s.piece < rows && c.gb) part(s.acc_b, v * 4);
